@@ -60,13 +60,13 @@ __global__ __launch_bounds__(256) MPE_ACTOR_ATTR void actor_forward_kernel(int64
   const int64_t ge = active ? env : B - 1;  // tail lanes shadow the last env, their stores are skipped
   const float *W1 = wts, *b1 = W1 + (int64_t)in_dim * H, *W2 = b1 + H;
   const float *b2 = W2 + H * H, *W3 = b2 + H, *b3 = W3 + H * OP;
-  typedef float f2 __attribute__((ext_vector_type(2)));  // packed f32 FMAs (v_pk_fma_f32): two units per instruction
+  typedef float f2 __attribute__((ext_vector_type(2)));  // two units per element (two v_fma_f32: the build has no packed f32 instructions)
   float h1[H], out[O];
   {
     f2 h1p[H / 2];
 #pragma unroll
     for (int q = 0; q < H / 2; ++q) h1p[q] = f2{b1[2 * q], b1[2 * q + 1]};
-    for (int i = 0; i < in_dim; ++i) {  // one coalesced row load per input, 32 packed FMAs with scalar weights
+    for (int i = 0; i < in_dim; ++i) {  // one coalesced row load per input, 64 FMAs with scalar weights
       const float x = ld_stream(obs + (int64_t)i * ld_obs + ge);
       const f2 xx = f2{x, x};
       const float *w = W1 + (int64_t)i * H;

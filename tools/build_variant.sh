@@ -7,7 +7,7 @@ set -e
 NAME="$1"; UNIT="$2"; shift 2
 ROOT="$(cd "$(dirname "$0")/.." && pwd)"
 C="$ROOT/marl_amd/csrc"; V="$ROOT/tools/variants"; mkdir -p "$V/$NAME"
-FLAGS="-O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -Wno-unused-function"
+FLAGS="-O3 -std=c++17 -fPIC --offload-arch=gfx950 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-function"
 /opt/rocm/bin/hipcc $FLAGS "$@" -c -o "$V/$NAME/$UNIT.o" "$C/$UNIT.hip"
 OBJS=$(ls "$C"/build/*.o | grep -v "/$UNIT.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o "$V/lib_$NAME.so" $OBJS "$V/$NAME/$UNIT.o"

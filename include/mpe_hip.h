@@ -557,6 +557,37 @@ int mpe_stats_reduce(const double *stats, int64_t rows, int width, double *out, 
 int mpe_env_step_stats_static(const mpe_scenario_desc *desc, int64_t B, int64_t ld, const mpe_buffers *buf,
                               int dtype_bytes, double *stats_out, void *stream);
 
+/*
+ * GROUPED PRODUCTS: the dense layers of many networks (an agent's, an expert's) in one launch, rows ragged.
+ * Row r of x [rows][k] belongs to group g when ends[g-1] <= r < ends[g] (ends[-1] = 0); weight [groups][n][k] and bias
+ * [groups][n] are contiguous; accumulation in f32, one rounding to dtype at the end.
+ *   mpe_grouped_linear     y = act(x W_g^T + b_g)            bias may be NULL; relu: 0 / 1 (NaN stays NaN)
+ *   mpe_grouped_linear_dx  dx = d W_g                        d = dy, or with y (the saved relu output) dy where not y <= 0
+ *   mpe_grouped_linear_dw  dweight_g = d_g^T x_g, dbias_g = column sums of d_g (dbias may be NULL); a group without rows
+ *                          gets zeros.  Fixed summation order: the same inputs give the same bits
+ * ends is a device array of int32 (ends64 = 0) or int64 and is read by the kernel as its running maximum clamped to
+ * [0, rows].  Rows behind the last group: untouched, or zeros with zero_tail = 1.  ld_* are row strides in elements, inner
+ * stride 1, any alignment of an element.  dtype is of all float arrays.  1 <= groups <= 1024, rows and n * k below 2^31.
+ * mpe_grouped_dw_workspace: bytes that mpe_grouped_linear_dw needs (>= 0, or MPE_ERR_*); the array is scratch of that
+ * call, 16-byte aligned; calls that may overlap (other streams, concurrent graph replays) need one each.
+ */
+#define MPE_F32 0
+#define MPE_BF16 1
+#define MPE_F16 2
+typedef struct mpe_grouped_desc {
+  const void *ends;
+  int64_t rows;
+  int32_t groups, n, k, dtype, ends64, pad_;
+} mpe_grouped_desc;
+int mpe_grouped_linear(const mpe_grouped_desc *desc, const void *x, int64_t ld_x, const void *weight, const void *bias,
+                       void *y, int64_t ld_y, int relu, int zero_tail, void *stream);
+int mpe_grouped_linear_dx(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
+                          const void *weight, void *dx, int64_t ld_dx, int zero_tail, void *stream);
+int64_t mpe_grouped_dw_workspace(const mpe_grouped_desc *desc);
+int mpe_grouped_linear_dw(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
+                          const void *x, int64_t ld_x, void *dweight, void *dbias, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

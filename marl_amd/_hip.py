@@ -34,6 +34,7 @@ FLAG_SILENT_COMM_ZERO = 8   # silent agents' comm rows already hold zeros: the s
 FLAG_DEVICE_NOISE = 16      # u_noise / c_noise normals the caller does not supply are drawn inside the step kernels
 SPLIT_MAX_ENVS = 32768
 HIER_SPLIT_MAX_ENVS = 65536
+F32, BF16, F16 = 0, 1, 2
 ACTOR_AUTO, ACTOR_VALU, ACTOR_MFMA, ACTOR_MFMA_F16 = 0, 1, 2, 3
 
 # MARL_AMD_LIB: alternative build of the same library (kernel tuning / ablation builds only)
@@ -116,6 +117,12 @@ class ActorJob(C.Structure):
                 ('in_dim', C.c_int32), ('s0', C.c_int32), ('s1', C.c_int32), ('seed', C.c_uint64)]
 
 
+class GroupedDesc(C.Structure):
+    """mpe_grouped_desc (include/mpe_hip.h): sizes of one grouped product."""
+    _fields_ = [('ends', C.c_void_p), ('rows', C.c_int64), ('groups', C.c_int32), ('n', C.c_int32), ('k', C.c_int32),
+                ('dtype', C.c_int32), ('ends64', C.c_int32), ('pad_', C.c_int32)]
+
+
 class MpeError(RuntimeError):
     def __init__(self, code, where):
         self.code = code
@@ -180,6 +187,16 @@ def _load():
         f.argtypes = [ci, C.POINTER(ReplayJob), C.POINTER(vp), i64, vp]
     L.mpe_actor_forward_multi_f32.restype = ci
     L.mpe_actor_forward_multi_f32.argtypes = [ci, C.POINTER(ActorJob), i64, i64, i64, u32, u64, ci, vp]
+    gp = C.POINTER(GroupedDesc)
+    L.mpe_grouped_linear.restype = ci             # desc, x, ld_x, weight, bias, y, ld_y, relu, zero_tail, stream
+    L.mpe_grouped_linear.argtypes = [gp, vp, i64, vp, vp, vp, i64, ci, ci, vp]
+    L.mpe_grouped_linear_dx.restype = ci          # desc, dy, ld_dy, y, ld_y, weight, dx, ld_dx, zero_tail, stream
+    L.mpe_grouped_linear_dx.argtypes = [gp, vp, i64, vp, i64, vp, vp, i64, ci, vp]
+    L.mpe_grouped_dw_workspace.restype = i64
+    L.mpe_grouped_dw_workspace.argtypes = [gp]
+    # desc, dy, ld_dy, y, ld_y, x, ld_x, dweight, dbias, workspace, workspace_bytes, stream
+    L.mpe_grouped_linear_dw.restype = ci
+    L.mpe_grouped_linear_dw.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp]
     L.mpe_stats_rows.restype = i64
     L.mpe_stats_rows.argtypes = [dp, i64, ci, u32]
     L.mpe_stats_reduce.restype = ci

@@ -1,0 +1,314 @@
+"""marl_amd.grouped: products grouped by agent with ragged row counts against plain 64-bit products, forward and backward."""
+import ctypes as C
+
+import pytest
+import torch
+
+from marl_amd import _hip, grouped
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}     # half a step, relative
+
+
+# ---- refusals (no GPU needed) --------------------------------------------------------------------------------------------
+def test_group_ends_checks_its_sizes():
+    assert grouped.group_ends([3, 0, 2], device='cpu').tolist() == [3, 3, 5]
+    for bad in ([], [1, -1], [1.5], [1] * 1025, [1 << 30, 1 << 30]):
+        with pytest.raises(ValueError):
+            grouped.group_ends(bad, device='cpu')
+
+
+def test_cpu_tensors_are_refused():
+    x, w, e = torch.zeros(4, 3), torch.zeros(2, 5, 3), torch.tensor([2, 4], dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        grouped.grouped_linear(x, w, e)
+    with pytest.raises(RuntimeError):
+        grouped.grouped_linear_backward(torch.zeros(4, 5), x, w, e)
+
+
+def _desc(**kw):
+    d = dict(ends=4096, rows=4, groups=2, n=5, k=3, dtype=_hip.F32, ends64=0)
+    d.update(kw)
+    return _hip.GroupedDesc(**d)
+
+
+@pytest.mark.parametrize('change,code', [
+    (dict(ends=None), -1), (dict(dtype=3), -5), (dict(groups=0), -6), (dict(groups=1025), -6), (dict(n=0), -6), (dict(k=0), -6),
+    (dict(rows=-1), -6), (dict(rows=1 << 31), -6), (dict(n=1 << 16, k=1 << 15), -6), (dict(ends=4098), -4),
+    (dict(ends=4100, ends64=1), -4), (dict(ends64=2), -6)])
+def test_c_abi_refuses_bad_descriptors(change, code):
+    """Nothing is launched: the pointers are never read."""
+    d, p = _desc(**change), 1 << 20
+    assert _hip.lib.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 0, None) == code
+    assert _hip.lib.mpe_grouped_linear_dx(d, p, 5, None, 0, p, p, 3, 0, None) == code
+    assert _hip.lib.mpe_grouped_dw_workspace(d) == code
+    assert _hip.lib.mpe_grouped_linear_dw(d, p, 5, None, 0, p, 3, p, None, None, 0, None) == code
+
+
+def test_c_abi_refuses_bad_arrays():
+    L, d, p = _hip.lib, _desc(), 1 << 20
+    assert L.mpe_grouped_linear(None, p, 3, p, None, p, 5, 0, 0, None) == -1
+    assert L.mpe_grouped_linear(d, None, 3, p, None, p, 5, 0, 0, None) == -1
+    assert L.mpe_grouped_linear(d, p, 2, p, None, p, 5, 0, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 4, 0, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 2, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 2, None) == -6
+    assert L.mpe_grouped_linear(d, p + 2, 3, p, None, p, 5, 0, 0, None) == -4
+    assert L.mpe_grouped_linear(d, p, 3, p, p + 1, p, 5, 0, 0, None) == -4
+    assert L.mpe_grouped_linear_dx(d, p, 5, p, 4, p, p, 3, 0, None) == -6
+    assert L.mpe_grouped_linear_dw(d, p, 5, None, 0, p, 3, None, None, None, 0, None) == -1
+    big = _desc(rows=1 << 20)                                     # rows split over workgroups: partial sums need an array
+    need = L.mpe_grouped_dw_workspace(big)
+    assert need > 0
+    assert L.mpe_grouped_linear_dw(big, p, 5, None, 0, p, 3, p, None, None, need, None) == -1
+    assert L.mpe_grouped_linear_dw(big, p, 5, None, 0, p, 3, p, None, p, need - 1, None) == -7
+    assert C.sizeof(_hip.GroupedDesc) == 40
+
+
+# ---- against 64 bits -----------------------------------------------------------------------------------------------------
+def _case(sizes, k, n, dtype, tail=0, seed=0, device='cuda'):
+    g = torch.Generator().manual_seed(seed)
+    t = sum(sizes) + tail
+    mk = lambda *s: torch.randn(*s, generator=g).to(dtype).to(device)     # noqa: E731
+    return (mk(t, k), (mk(len(sizes), n, k).float() * k ** -0.5).to(dtype), mk(len(sizes), n), mk(t, n),
+            grouped.group_ends(sizes, device))
+
+
+def _reference(x, w, b, grad, sizes, relu, y_saved=None):
+    """(y, dx, dw, db) in 64 bits, and for each the sum of the absolute values of its terms."""
+    x, w, b, grad = x.double(), w.double(), b.double(), grad.double()
+    y, dx = torch.zeros(grad.shape, dtype=torch.float64, device=x.device), torch.zeros_like(x)
+    dw, db = torch.zeros_like(w), torch.zeros_like(b)
+    ya, dxa, dwa, dba = (torch.zeros_like(t) for t in (y, dx, dw, db))
+    r = 0
+    for g, s in enumerate(sizes):
+        p = slice(r, r + s)
+        r += s
+        y[p], ya[p] = x[p] @ w[g].t().contiguous() + b[g], x[p].abs() @ w[g].abs().t().contiguous() + b[g].abs()
+        if relu:
+            y[p] = y[p].clamp(min=0)
+        d = grad[p] if y_saved is None else grad[p] * (y_saved[p].double() > 0)
+        dx[p], dxa[p] = d @ w[g], d.abs() @ w[g].abs()
+        dw[g], dwa[g] = d.t().contiguous() @ x[p], d.abs().t().contiguous() @ x[p].abs()
+        db[g], dba[g] = d.sum(0), d.abs().sum(0)
+    return (y, dx, dw, db), (ya, dxa, dwa, dba)
+
+
+def _close(got, want, terms, count, dtype, what):
+    """Sum of ``count`` products in f32, any order: each product and addition is off by at most 2^-23 of a partial sum, which
+    is at most the sum of the terms' absolute values (2^-23, not 2^-24: the matrix unit may cut off what it aligns); then one
+    rounding to the type (half a step; f16 below its normal range: half of 2^-24)."""
+    tol = (count + 2) * 2.0 ** -23 * terms + HALF[dtype] * want.abs() * (1 + 1e-3) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    bad = (got.double() - want).abs() > tol
+    assert got.dtype == dtype and not bool(bad.any()), (what, int(bad.sum()), float(((got.double() - want).abs() / tol).max()))
+
+
+SHAPES = [
+    ([1], 1, 1), ([5], 3, 2), ([0, 1, 0], 7, 9), ([3, 0, 64, 65, 1], 16, 64), ([63, 64, 65], 33, 65), ([256] * 4, 64, 64),
+    ([1000, 1, 0, 500], 226, 64), ([128, 129], 64, 5), ([17, 300, 3], 333, 517), ([200, 0, 56], 512, 256), ([0, 0], 8, 8),
+    ([2500], 130, 40), ([1] * 70, 20, 24), ([700, 900], 128, 136), ([1, 2, 1, 0, 3], 1024, 520)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('relu', [False, True], ids=['linear', 'relu'])
+@pytest.mark.parametrize('sizes,k,n', SHAPES, ids=['%dx%d_%d_%d' % (len(s), sum(s), k, n) for s, k, n in SHAPES])
+def test_forward_and_backward(sizes, k, n, relu, dtype):
+    x, w, b, grad, ends = _case(sizes, k, n, dtype)
+    y = grouped.grouped_linear(x, w, ends, bias=b, relu=relu)
+    dx, dw, db = grouped.grouped_linear_backward(grad, x, w, ends, y=y if relu else None)
+    want, terms = _reference(x, w, b, grad, sizes, relu, y if relu else None)
+    most = max(sizes)
+    for got, ref, ab, count, what in zip((y, dx, dw, db), want, terms, (k + 1, n, most, most), ('y', 'dx', 'dw', 'db')):
+        _close(got, ref, ab, count, dtype, what)
+    for g, s in enumerate(sizes):
+        if s == 0:
+            assert not dw[g].any() and not db[g].any()
+    y0 = grouped.grouped_linear(x, w, ends, relu=relu)                       # no bias
+    ref0, terms0 = _reference(x, w, torch.zeros_like(b), grad, sizes, relu)
+    _close(y0, ref0[0], terms0[0], k, dtype, 'y without bias')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_strides_alignment_and_rows_of_no_group(dtype):
+    """Row strides that are no multiple of anything, bases in the middle of a 16-byte word, columns that are not adjacent,
+    int64 ends; rows behind the last group are zeros, or left as they were in ``out``."""
+    sizes, k, n, tail = [70, 0, 131, 9], 45, 77, 100
+    x, w, b, grad, ends = _case(sizes, k, n, dtype, tail=tail)
+    want, terms = _reference(x, w, b, grad, sizes, False)
+    t, live = x.shape[0], sum(sizes)
+    xs = torch.full((t, k + 6), 7.0, dtype=dtype, device='cuda')[:, 3:3 + k]
+    xs.copy_(x)
+    gs = torch.full((t, n + 4), 7.0, dtype=dtype, device='cuda')[:, 1:1 + n]
+    gs.copy_(grad)
+    ws = torch.empty(w.numel() + 1, dtype=dtype, device='cuda')[1:].view(w.shape).copy_(w)
+    for xx, ww, gg in ((xs, ws, gs), (x.t().contiguous().t(), w.transpose(0, 1).contiguous().transpose(0, 1), grad.t().contiguous().t())):
+        y = grouped.grouped_linear(xx, ww, ends.long(), bias=b)
+        dx, dw, db = grouped.grouped_linear_backward(gg, xx, ww, ends.long())
+        for got, ref, ab, count, what in zip((y, dx, dw, db), want, terms, (k + 1, n, 131, 131), ('y', 'dx', 'dw', 'db')):
+            _close(got, ref, ab, count, dtype, what)
+        assert not y[live:].any() and not dx[live:].any()
+    out = torch.full((t, n + 3), 5.0, dtype=dtype, device='cuda')
+    assert grouped.grouped_linear(xs, ws, ends, bias=b, out=out[:, 2:2 + n]).data_ptr() == out[:, 2:].data_ptr()
+    _close(out[:live, 2:2 + n], want[0][:live], terms[0][:live], k + 1, dtype, 'out')
+    assert (out[live:] == 5).all() and (out[:, :2] == 5).all() and (out[:, 2 + n:] == 5).all()
+
+
+@pytest.mark.gpu
+def test_ends_outside_the_rows_are_clamped():
+    """Running maximum, clamped to [0, rows]: decreasing, negative and far too large entries touch nothing they should not."""
+    x, w, b, grad, _ = _case([50, 30, 20, 10], 24, 40, torch.float32)
+    ends = torch.tensor([-7, 60, 40, 1 << 30], dtype=torch.int32, device='cuda')
+    sizes = [0, 60, 0, 50]
+    y = grouped.grouped_linear(x, w, ends, bias=b)
+    got = (y,) + grouped.grouped_linear_backward(grad, x, w, ends)
+    want, terms = _reference(x, w, b, grad, sizes, False)
+    for o, ref, ab, count, what in zip(got, want, terms, (25, 40, 60, 60), ('y', 'dx', 'dw', 'db')):
+        _close(o, ref, ab, count, torch.float32, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+def test_infinities_and_nan_stay_in_their_rows(dtype):
+    sizes, k, n = [40, 33], 70, 50
+    x, w, b, grad, ends = _case(sizes, k, n, dtype)
+    clean = grouped.grouped_linear(x, w, ends, bias=b, relu=True)
+    x[39, 69], x[40, 0] = float('inf'), float('nan')                # the last row of group 0, the first of group 1
+    y = grouped.grouped_linear(x, w, ends, bias=b, relu=True)
+    rest = [i for i in range(73) if i not in (39, 40)]
+    assert torch.equal(y[rest], clean[rest])
+    assert y[40].isnan().all()                                      # relu keeps NaN
+    plus = w[0, :, 69] > 0
+    assert (y[39][plus] == float('inf')).all() and (y[39][~plus] == 0).all()
+    dx, dw, db = grouped.grouped_linear_backward(grad, x, w, ends, y=y)
+    assert torch.isfinite(dx).all() and torch.isfinite(dw[0][:, :69]).all() and torch.isfinite(db).all()
+    assert dw[1][:, 0].isnan().all() and torch.isfinite(dw[1][:, 1:]).all()
+
+
+@pytest.mark.gpu
+def test_autograd_matches_the_formula_and_differences():
+    sizes, k, n = [9, 0, 14], 6, 7
+    x, w, b, grad, ends = _case(sizes, k, n, torch.float32)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = grouped.grouped_linear(x, w, ends, bias=b, relu=True)
+    (y * grad).sum().backward()
+    plain = grouped.grouped_linear_backward(grad, x.detach(), w.detach(), ends, y=y.detach())
+    for t, p in zip((x, w, b), plain):
+        assert torch.equal(t.grad, p)
+
+    def loss(xx, ww, bb):                                           # the formula in 64 bits
+        return float((_reference(xx, ww, bb, grad, sizes, True)[0][0] * grad.double()).sum())
+    h = 1e-6
+    for pos, (t, gr) in enumerate(((x, x.grad), (w, w.grad), (b, b.grad))):
+        flat, r = t.detach().double().flatten(), torch.Generator().manual_seed(pos)
+        for i in torch.randperm(flat.numel(), generator=r)[:12].tolist():
+            args = [x.detach().double(), w.detach().double(), b.detach().double()]
+            up, dn = flat.clone(), flat.clone()
+            up[i] += h
+            dn[i] -= h
+            args[pos] = up.view(t.shape)
+            hi = loss(*args)
+            args[pos] = dn.view(t.shape)
+            lo = loss(*args)
+            # central difference of a piecewise linear function, 64 bits: rounding ~1e-15 / h; the f32 gradient: < 1e-5
+            assert abs((hi - lo) / (2 * h) - float(gr.flatten()[i])) < 2e-5, (pos, i)
+    only_w = torch.autograd.grad(grouped.grouped_linear(x.detach(), w, ends).sum(), w)[0]
+    assert only_w.shape == w.shape
+    with pytest.raises(RuntimeError):                               # out= has no gradient
+        grouped.grouped_linear(x, w, ends, out=torch.empty(23, n, device='cuda'))
+
+
+@pytest.mark.gpu
+def test_expanded_gradient_and_shared_weight():
+    """``sum().backward()`` hands a stride-0 gradient; one weight shared by every group gets the sum of their gradients."""
+    sizes, k, n = [5, 8], 6, 4
+    x, w, b, _, ends = _case(sizes, k, n, torch.float32)
+    shared = w[:1].clone().requires_grad_()
+    grouped.grouped_linear(x, shared.expand(2, n, k), ends).sum().backward()
+    want = x.double().sum(0).expand(n, k)
+    assert (shared.grad[0].double() - want).abs().max() < 13 * 2.0 ** -22 * x.double().abs().sum(0).max()
+
+
+@pytest.mark.gpu
+def test_results_repeat_and_follow_a_graph():
+    """The same bits on every call, eager or replayed; a replay reads what `ends` and the arrays hold then; another stream."""
+    sizes, k, n = [300, 500, 200], 96, 80
+    x, w, b, grad, ends = _case(sizes, k, n, torch.float32)
+
+    def both():
+        y = grouped.grouped_linear(x, w, ends, bias=b, relu=True)
+        return (y,) + grouped.grouped_linear_backward(grad, x, w, ends, y=y)
+    eager = [t.clone() for t in both()]
+    assert all(torch.equal(a, c) for a, c in zip(eager, both()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(eager, other))
+    graphs = []
+    torch.cuda.synchronize()
+    for _ in range(2):                                              # two graphs: each has its own scratch memory
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, capture_error_mode='thread_local'):
+            out = both()
+        graphs.append((g, out))
+    for step in range(3):
+        ends.copy_(grouped.group_ends([[300, 500, 200], [0, 700, 300], [1000, 0, 0]][step]))
+        x.mul_(1.25)
+        torch.cuda.synchronize()
+        for g, _ in graphs:
+            g.replay()
+        want = both()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(out, want)), step
+
+
+@pytest.mark.gpu
+def test_arguments_are_checked():
+    x, w, b, grad, ends = _case([3, 4], 6, 5, torch.float32)
+    ok = dict(x=x, weight=w, ends=ends, bias=b)
+    bad = [dict(x=x.double()), dict(x=x.half()), dict(x=x[:, :5]), dict(x=x[0]), dict(weight=w[0]), dict(weight=w.bfloat16()),
+           dict(bias=b[:, :4]), dict(bias=b.half()), dict(bias=b.cpu()), dict(ends=ends[:1]), dict(ends=ends.float()),
+           dict(ends=ends.cpu()), dict(ends=[3, 7]), dict(weight=w[:, :0]), dict(weight=w[:, :, :0], x=x[:, :0]),
+           dict(weight=w.expand(2, 5, 6)[:0], bias=None, ends=ends[:0]), dict(out=x), dict(out=torch.empty(7, 4, device='cuda')),
+           dict(out=torch.empty(7, 5, device='cuda').half()), dict(out=torch.empty(5, 7, device='cuda').t())]
+    for change in bad:
+        with pytest.raises((TypeError, ValueError)):
+            grouped.grouped_linear(**dict(ok, **change))
+    sq = torch.zeros(7, 7, device='cuda')
+    with pytest.raises(ValueError):                                 # the result would overwrite what it reads
+        grouped.grouped_linear(sq[:, :6], w, ends, out=sq[:, 2:])
+    for kw in (dict(grad=grad[:, :4]), dict(grad=grad.half()), dict(y=grad[:3])):
+        with pytest.raises(ValueError):
+            grouped.grouped_linear_backward(**dict(dict(grad=grad, x=x, weight=w, ends=ends), **kw))
+    empty = grouped.grouped_linear(x[:0], w, ends, bias=b)
+    assert empty.shape == (0, 5)
+    dx, dw, db = grouped.grouped_linear_backward(grad[:0], x[:0], w, ends)
+    assert dx.shape == (0, 6) and not dw.any() and not db.any()
+    dx, dw, db = grouped.grouped_linear_backward(grad, x, w, ends, need_dx=False, need_dbias=False)
+    assert dx is None and db is None and dw.shape == w.shape
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows whose element offsets pass 2^31 (x) and 2^32 bytes: the last rows equal those of a call of their own."""
+    t, k, n = (1 << 20) + 77, 2080, 8
+    x = torch.zeros(t, k, dtype=torch.bfloat16, device='cuda')
+    g = torch.Generator(device='cuda').manual_seed(1)
+    x[-300:] = torch.randn(300, k, generator=g, device='cuda').bfloat16()
+    w = torch.randn(2, n, k, generator=g, device='cuda').bfloat16()
+    ends = torch.tensor([t - 200, t], dtype=torch.int64, device='cuda')
+    y = grouped.grouped_linear(x, w, ends)
+    small = grouped.grouped_linear(x[-300:], w, ends - (t - 300))
+    assert torch.equal(y[-300:], small) and not y[:-300].any()
+    grad = torch.zeros(t, n, dtype=torch.bfloat16, device='cuda')
+    grad[-300:] = torch.randn(300, n, generator=g, device='cuda').bfloat16()
+    dx, dw, db = grouped.grouped_linear_backward(grad, x, w, ends)
+    sx, sw, sb = grouped.grouped_linear_backward(grad[-300:], x[-300:], w, ends - (t - 300))
+    assert torch.equal(dx[-300:], sx) and not dx[:-300].any()
+    want, terms = _reference(x[-300:], w, torch.zeros(2, n, device='cuda'), grad[-300:], [100, 200], False)
+    for got, ref, ab, what in ((dw, want[2], terms[2], 'dw'), (db, want[3], terms[3], 'db')):
+        _close(got, ref, ab, 200, torch.bfloat16, what)

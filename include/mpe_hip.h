@@ -588,6 +588,42 @@ int mpe_grouped_linear_dw(const mpe_grouped_desc *desc, const void *dy, int64_t 
                           const void *x, int64_t ld_x, void *dweight, void *dbias, void *workspace,
                           int64_t workspace_bytes, void *stream);
 
+/*
+ * ADAMW over many tensors in one or a few launches, moments in 32 or in 8 bits, with the clip of each variable's gradient
+ * (tf_util.py:137-149) before it and the polyak step of its target (maddpg.py:20-26) behind it:
+ *     g' = g c / max(|g|, c);  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps);  target = polyak target + (1 - polyak) p
+ * param, target and gradient of a call share dtype (MPE_F32 / MPE_BF16 / MPE_F16), are contiguous and need an element's
+ * alignment; target NULL: none.  exp_avg / exp_avg_sq: float arrays (state_bits 32) or byte codes (8), 16-byte aligned, of
+ * ceil(count / 128) * 128 elements; 8 bits: int16 exp_avg_base / exp_avg_sq_base, one per 128 elements.  Byte c with base b
+ * stands for the float with bits (|c| + b) << 20 (c's low 7 bits for exp_avg, bit 7 its sign; all 8 for exp_avg_sq), 0 for
+ * zero.  Rounding to 8 bits is stochastic, keyed by (seed, step, index0 + tensor, element): the same call gives the same bits.
+ *   mpe_adamw_plan   writes the device plan of these tensors into the HOST array blob (NULL: only the size); returns its
+ *                    bytes, or MPE_ERR_*.  The caller copies it to the device once and passes that copy to every step
+ *   mpe_adamw_step   tensors: the same host array; grads: host array of device pointers, NULL = no gradient (only the
+ *                    target moves).  step >= 1 counts this step, or clock (device, 32 bytes: int64 step, then 16 bytes that
+ *                    the call writes) holds the steps taken so far and is moved on by one (for graph capture).
+ *                    max_norm 0: no clip.  The plan holds the clip's scratch: steps on one plan must not overlap
+ *   mpe_adamw_moments  byte codes of count (a multiple of 128) elements as the values they stand for (MPE_F32 / MPE_BF16)
+ */
+typedef struct mpe_adamw_tensor {
+  void *param, *target, *exp_avg, *exp_avg_base, *exp_avg_sq, *exp_avg_sq_base;
+  int64_t count;
+} mpe_adamw_tensor;
+typedef struct mpe_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay, max_norm, polyak;
+  int64_t step;
+  void *clock;
+  uint64_t seed;
+  uint32_t index0;
+  int32_t dtype, state_bits, pad_;
+} mpe_adamw_args;
+int64_t mpe_adamw_plan(int n, const mpe_adamw_tensor *tensors, int dtype, int state_bits, void *blob, int64_t blob_bytes);
+int mpe_adamw_step(const mpe_adamw_args *args, int n, const mpe_adamw_tensor *tensors, const void *plan,
+                   const void *const *grads, void *stream);
+int mpe_adamw_moments(const void *codes, const void *base, void *out, int64_t count, int is_signed, int dtype,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

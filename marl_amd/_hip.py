@@ -123,6 +123,19 @@ class GroupedDesc(C.Structure):
                 ('dtype', C.c_int32), ('ends64', C.c_int32), ('pad_', C.c_int32)]
 
 
+class AdamTensor(C.Structure):
+    """mpe_adamw_tensor (include/mpe_hip.h): one variable of an AdamW step."""
+    _fields_ = [(n, C.c_void_p) for n in ('param', 'target', 'exp_avg', 'exp_avg_base', 'exp_avg_sq',
+                                          'exp_avg_sq_base')] + [('count', C.c_int64)]
+
+
+class AdamArgs(C.Structure):
+    """mpe_adamw_args (include/mpe_hip.h): what the variables of an AdamW step share."""
+    _fields_ = [(n, C.c_double) for n in ('lr', 'beta1', 'beta2', 'eps', 'weight_decay', 'max_norm', 'polyak')] + [
+        ('step', C.c_int64), ('clock', C.c_void_p), ('seed', C.c_uint64), ('index0', C.c_uint32), ('dtype', C.c_int32),
+        ('state_bits', C.c_int32), ('pad_', C.c_int32)]
+
+
 class MpeError(RuntimeError):
     def __init__(self, code, where):
         self.code = code
@@ -197,6 +210,13 @@ def _load():
     # desc, dy, ld_dy, y, ld_y, x, ld_x, dweight, dbias, workspace, workspace_bytes, stream
     L.mpe_grouped_linear_dw.restype = ci
     L.mpe_grouped_linear_dw.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp]
+    ap = C.POINTER(AdamTensor)
+    L.mpe_adamw_plan.restype = i64                # n, tensors, dtype, state_bits, blob (host), blob_bytes
+    L.mpe_adamw_plan.argtypes = [ci, ap, ci, ci, vp, i64]
+    L.mpe_adamw_step.restype = ci                 # args, n, tensors (host), plan (device), grads (host array), stream
+    L.mpe_adamw_step.argtypes = [C.POINTER(AdamArgs), ci, ap, vp, C.POINTER(vp), vp]
+    L.mpe_adamw_moments.restype = ci              # codes, base, out, count, is_signed, dtype, stream
+    L.mpe_adamw_moments.argtypes = [vp, vp, vp, i64, ci, ci, vp]
     L.mpe_stats_rows.restype = i64
     L.mpe_stats_rows.argtypes = [dp, i64, ci, u32]
     L.mpe_stats_reduce.restype = ci

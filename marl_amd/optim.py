@@ -1,0 +1,290 @@
+"""AdamW over many tensors in one or a few launches, with moments in 32 or in 8 bits (libmpe_hip.so: mpe_adamw_step).
+
+What a learner's update does behind its backward pass -- clip every variable's gradient to a norm (tf_util.py:137-149), Adam
+(maddpg/maddpg/trainer/maddpg.py:130-145), polyak step of the target networks (maddpg.py:20-26) -- is one pass over the
+variables' memory here:
+
+    g' = g * max_norm / max(|g|, max_norm)                                                  (max_norm given)
+    m  = b1 m + (1 - b1) g';   v = b2 v + (1 - b2) g'^2
+    p  = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+    target = polyak target + (1 - polyak) p                                                 (targets given)
+
+Parameters are float32, bfloat16 or float16 (one type a group; their gradients and targets alike); the arithmetic is in
+32 bits, the norms in 64, and p is rounded once.  ``state_bits=32`` holds the moments in float32; ``state_bits=8`` in one byte
+each, plus one int16 for 128 of them: a logarithmic code (eighths of a binade; m 16 binades and a sign, v 32 binades) below
+the largest element of its block, rounded stochastically from (seed, step, tensor, element), so that a moment is right on
+average and a run repeats bit for bit.  A gradient that is not finite makes its element (32 bits) or its block of 128
+(8 bits) useless, as it does any Adam."""
+import ctypes as C
+
+import torch
+
+from . import _hip
+
+BLOCK = 128                       # elements that share the base of their 8-bit moments; every variable starts a new one
+_DTYPES = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
+
+
+def dequantize(codes, base, signed, dtype=torch.float32):
+    """The values that 8-bit moments stand for: ``codes`` (uint8, a multiple of 128), ``base`` (int16, one per 128);
+    ``signed``: first moments.  float32 and bfloat16 hold them exactly."""
+    if codes.dtype != torch.uint8 or base.dtype != torch.int16 or codes.numel() != base.numel() * BLOCK:
+        raise ValueError('dequantize: uint8 codes with one int16 base per %d expected' % BLOCK)
+    if codes.device.type != 'cuda' or base.device != codes.device:
+        raise RuntimeError('dequantize works on GPU tensors (no CPU fallback)')
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError('dequantize returns float32 or bfloat16, not %r' % (dtype,))
+    codes, base = codes.contiguous(), base.contiguous()
+    out = torch.empty(codes.numel(), dtype=dtype, device=codes.device)
+    with _hip.on_device(codes.device):
+        _hip.check(_hip.lib.mpe_adamw_moments(codes.data_ptr(), base.data_ptr(), out.data_ptr(), codes.numel(), int(signed),
+                                              _DTYPES[dtype], _hip.stream_of(codes.device)), 'mpe_adamw_moments')
+    return out
+
+
+class _Plan(object):
+    """One parameter group: its flat moments and what the kernels read about its variables."""
+
+    def __init__(self, params, targets, state_bits):
+        p0 = params[0]
+        self.params, self.targets, self.bits = list(params), targets, state_bits
+        self.device, self.dtype = p0.device, p0.dtype
+        self.counts = [p.numel() for p in self.params]
+        self.first, total = [], 0
+        for c in self.counts:                       # every variable starts at a multiple of BLOCK
+            self.first.append(total)
+            total += -(-c // BLOCK) * BLOCK
+        dev = self.device
+        if state_bits == 8:
+            self.flat = {'exp_avg': torch.zeros(total, dtype=torch.uint8, device=dev),
+                         'exp_avg_base': torch.zeros(total // BLOCK, dtype=torch.int16, device=dev),
+                         'exp_avg_sq': torch.zeros(total, dtype=torch.uint8, device=dev),
+                         'exp_avg_sq_base': torch.zeros(total // BLOCK, dtype=torch.int16, device=dev)}
+        else:
+            self.flat = {'exp_avg': torch.zeros(total, dtype=torch.float32, device=dev),
+                         'exp_avg_sq': torch.zeros(total, dtype=torch.float32, device=dev)}
+        self.grads = (C.c_void_p * len(self.params))()
+        self.build()
+
+    def views(self, j):
+        """The moments of variable j, as views of the flat arrays."""
+        o, c, out = self.first[j], self.counts[j], {}
+        for name, t in self.flat.items():
+            if name.endswith('_base'):
+                out[name] = t[o // BLOCK:-(-(o + c) // BLOCK)]
+            else:
+                out[name] = t[o:o + c].view(self.params[j].shape)
+        return out
+
+    def build(self):
+        """The host table of pointers and its device plan."""
+        if not all(t.is_contiguous() for t in self.params + (self.targets or [])):
+            raise ValueError('AdamW: parameters and targets are contiguous')
+        n = len(self.params)
+        self.table = (_hip.AdamTensor * n)()
+        for j, p in enumerate(self.params):
+            o = self.first[j]
+            at = {k: t.data_ptr() + (o // BLOCK if k.endswith('_base') else o) * t.element_size() for k, t in self.flat.items()}
+            self.table[j] = _hip.AdamTensor(param=p.data_ptr(), count=self.counts[j],
+                                            target=None if self.targets is None else self.targets[j].data_ptr(), **at)
+        code = _DTYPES[self.dtype]
+        size = _hip.lib.mpe_adamw_plan(n, self.table, code, self.bits, None, 0)
+        _hip.check(min(size, 0), 'mpe_adamw_plan')
+        blob = torch.empty(size, dtype=torch.uint8)
+        _hip.check(min(_hip.lib.mpe_adamw_plan(n, self.table, code, self.bits, blob.data_ptr(), size), 0), 'mpe_adamw_plan')
+        self.plan = blob.to(self.device)
+        self.ptrs = self.pointers()
+
+    def pointers(self):
+        ptrs = [p.data_ptr() for p in self.params]
+        if self.targets is not None:
+            ptrs += [t.data_ptr() for t in self.targets]
+        return ptrs
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.Optimizer`` with ``step()`` as above (parameter groups and learning-rate schedulers work as usual).
+
+    ``targets``: tensors like the parameters, in their order (of a parameter group: its ``'targets'`` entry), that follow
+    them by ``polyak``; ``max_norm``: clip of each variable's gradient on its own; ``seed``: of the 8-bit rounding.
+    ``capturable=True`` keeps the step count on the device, so that ``step()`` can be recorded in a HIP graph: every replay
+    is one more step, with the learning rate and the other settings of the recording.  Gradients are read where they lie:
+    a recording reads the same addresses again, so let them stay (``zero_grad(set_to_none=False)``).
+
+    A parameter without a gradient keeps its value and moments (its target still moves); the step count is the group's.
+    ``state_dict`` / ``load_state_dict`` hold the moments as they are stored."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None,
+                 targets=None, polyak=0.99, seed=0, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError('state_bits: 8 or 32, got %r' % (state_bits,))
+        params = list(params)
+        if targets is not None:
+            if params and isinstance(params[0], dict):
+                raise ValueError("targets: give each parameter group its own 'targets'")
+            params = [dict(params=params, targets=list(targets))]
+        self._bits, self._seed, self._capturable = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF, bool(capturable)
+        self._plans, self._clocks = [], []
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm,
+                                      polyak=polyak, step=0))
+
+    # -- construction ------------------------------------------------------------------------------------------------------
+    @staticmethod
+    def _check_group(g):
+        b1, b2 = g['betas']
+        if not (0 <= g['lr'] < float('inf')) or not 0 <= b1 < 1 or not 0 <= b2 < 1 or not g['eps'] >= 0 \
+                or not g['weight_decay'] >= 0 or not 0 <= g['polyak'] <= 1:
+            raise ValueError('AdamW: lr %r, betas %r, eps %r, weight_decay %r, polyak %r' % (
+                g['lr'], g['betas'], g['eps'], g['weight_decay'], g['polyak']))
+        if g['max_norm'] is not None and not 0 < g['max_norm'] < float('inf'):
+            raise ValueError('AdamW: max_norm is positive and finite, or None, got %r' % (g['max_norm'],))
+
+    def add_param_group(self, group):
+        group = dict(group)
+        targets = group.pop('targets', None)
+        if torch.is_tensor(group.get('params')):
+            group['params'] = [group['params']]
+        params = group['params'] = list(group.get('params', ()))
+        if not params:
+            raise ValueError('AdamW: an empty parameter group')
+        if targets is not None:
+            targets = list(targets)
+            if len(targets) != len(params):
+                raise ValueError('AdamW: %d targets for %d parameters' % (len(targets), len(params)))
+        p0 = params[0]
+        for t in params + (targets or []):
+            if not torch.is_tensor(t):
+                raise TypeError('AdamW: parameters and targets are tensors, got %r' % (type(t),))
+            if t.device.type != 'cuda':
+                raise RuntimeError('marl_amd.optim.AdamW works on GPU tensors (no CPU fallback)')
+            if t.dtype not in _DTYPES:
+                raise TypeError('AdamW supports float32, bfloat16 and float16 parameters, got %r' % (t.dtype,))
+            if t.dtype != p0.dtype or t.device != p0.device:
+                raise ValueError('AdamW: the tensors of a parameter group share type and device')
+            if not t.is_contiguous():
+                raise ValueError('AdamW: parameters and targets are contiguous')
+        if targets is not None and any(t.shape != p.shape for t, p in zip(targets, params)):
+            raise ValueError('AdamW: a target has the shape of its parameter')
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in params + (targets or []) if t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError('AdamW: two of the tensors share memory')
+        for key, value in self.defaults.items():
+            group.setdefault(key, value)
+        self._check_group(group)
+        super().add_param_group(group)
+        plan = _Plan(params, targets, self._bits)
+        self._plans.append(plan)
+        self._clocks.append(torch.zeros(4, dtype=torch.int64, device=plan.device) if self._capturable else None)
+        for j, p in enumerate(params):
+            self.state[p] = plan.views(j)
+
+    # -- step count --------------------------------------------------------------------------------------------------------
+    @property
+    def step_count(self):
+        """Steps taken (of the first parameter group; reads the device where it is kept there)."""
+        return self._steps(0)
+
+    @step_count.setter
+    def step_count(self, value):
+        for i in range(len(self._plans)):
+            self._set_steps(i, value)
+
+    def _steps(self, i):
+        return int(self._clocks[i][0]) if self._clocks[i] is not None else self.param_groups[i]['step']
+
+    def _set_steps(self, i, value):
+        if int(value) < 0:
+            raise ValueError('AdamW: a step count is >= 0, got %r' % (value,))
+        self.param_groups[i]['step'] = int(value)
+        if self._clocks[i] is not None:
+            self._clocks[i][0] = int(value)
+
+    # -- the step ----------------------------------------------------------------------------------------------------------
+    def _gradients(self, plan):
+        """Fills the plan's pointers; returns what must outlive the launch."""
+        keep, arr, dtype, device = [], plan.grads, plan.dtype, plan.device
+        for j, p in enumerate(plan.params):
+            g = p.grad
+            if g is None:
+                arr[j] = None
+                continue
+            if g.dtype != dtype or g.device != device or g.layout != torch.strided:
+                raise ValueError('AdamW: a gradient is %s on %s, its parameter %s on %s' % (g.dtype, g.device, dtype, device))
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            arr[j] = g.data_ptr()
+        return keep
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step of every parameter group, on the current stream of its device."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        index0 = 0
+        for i, (group, plan) in enumerate(zip(self.param_groups, self._plans)):
+            self._check_group(group)
+            if plan.pointers() != plan.ptrs:                      # a parameter's storage was replaced
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError('AdamW: a parameter moved since the last step; take one step before recording')
+                plan.build()
+            keep = self._gradients(plan)
+            clock = self._clocks[i]
+            args = _hip.AdamArgs(lr=group['lr'], beta1=group['betas'][0], beta2=group['betas'][1], eps=group['eps'],
+                                 weight_decay=group['weight_decay'], max_norm=group['max_norm'] or 0.0, polyak=group['polyak'],
+                                 step=group['step'] + 1, clock=_hip.ptr(clock), seed=self._seed, index0=index0,
+                                 dtype=_DTYPES[plan.dtype], state_bits=self._bits)
+            with _hip.on_device(plan.device):
+                _hip.check(_hip.lib.mpe_adamw_step(args, len(plan.params), plan.table, plan.plan.data_ptr(), plan.grads,
+                                                   _hip.stream_of(plan.device)), 'mpe_adamw_step')
+            del keep
+            if clock is None:
+                group['step'] += 1
+            index0 += len(plan.params)
+            torch.autograd.graph.increment_version(plan.params + (plan.targets or []))
+        return loss
+
+    # -- the moments -------------------------------------------------------------------------------------------------------
+    def buffers(self):
+        """For every parameter group the flat arrays that hold its moments (``exp_avg``, ``exp_avg_sq``, and with 8 bits
+        their ``_base``): variables in order, each from a multiple of 128 on, zeros in between."""
+        return [dict(plan.flat) for plan in self._plans]
+
+    def moments(self, dtype=torch.float32):
+        """For every parameter group its flat ``(exp_avg, exp_avg_sq)`` as values (laid out as in ``buffers``): the arrays
+        themselves with ``state_bits=32``, what the codes stand for with 8."""
+        if self._bits == 32:
+            if dtype != torch.float32:
+                raise TypeError('32-bit moments are float32')
+            return [(plan.flat['exp_avg'], plan.flat['exp_avg_sq']) for plan in self._plans]
+        return [(dequantize(plan.flat['exp_avg'], plan.flat['exp_avg_base'], True, dtype),
+                 dequantize(plan.flat['exp_avg_sq'], plan.flat['exp_avg_sq_base'], False, dtype)) for plan in self._plans]
+
+    def state_dict(self):
+        for i in range(len(self._plans)):
+            self.param_groups[i]['step'] = self._steps(i)
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        """Settings, step counts and moments of an optimizer with the same groups, shapes and ``state_bits``; the moments are
+        copied into this optimizer's arrays, which stay where they are."""
+        groups = state_dict['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
+            raise ValueError('AdamW: the state dict has other parameter groups')
+        todo = []
+        for plan, saved in zip(self._plans, groups):
+            for j, key in enumerate(saved['params']):
+                have, got = plan.views(j), state_dict['state'].get(key)
+                if got is None or set(got) != set(have) or any(
+                        got[k].shape != have[k].shape or got[k].dtype != have[k].dtype for k in have):
+                    raise ValueError('AdamW: the moments of parameter %r have other names, shapes or types' % (key,))
+                todo += [(have[k], got[k]) for k in have]
+        for saved in groups:
+            self._check_group(saved)
+        for dst, src in todo:
+            dst.copy_(src)
+        for i, (group, saved) in enumerate(zip(self.param_groups, groups)):
+            group.update({k: v for k, v in saved.items() if k != 'params'})
+            self._set_steps(i, saved['step'])

@@ -1,0 +1,483 @@
+"""marl_amd.optim.AdamW: one step over many tensors against the formulas in 64 bits, and its 8-bit moments against a
+restatement in numpy's float32, bit for bit."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from marl_amd import _hip, optim
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+# ---- refusals (no GPU needed) --------------------------------------------------------------------------------------------
+def test_cpu_parameters_and_bad_settings_are_refused():
+    with pytest.raises(RuntimeError):
+        optim.AdamW([torch.zeros(3)])
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.zeros(3)], state_bits=16)
+    with pytest.raises(ValueError):
+        optim.AdamW([])
+    with pytest.raises(ValueError):
+        optim.dequantize(torch.zeros(128), torch.zeros(1, dtype=torch.int16), True)
+    with pytest.raises(RuntimeError):
+        optim.dequantize(torch.zeros(128, dtype=torch.uint8), torch.zeros(1, dtype=torch.int16), True)
+
+
+def _args(**kw):
+    d = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, max_norm=0.0, polyak=0.99, step=1, dtype=_hip.F32,
+             state_bits=32)
+    d.update(kw)
+    return _hip.AdamArgs(**d)
+
+
+def _table(**kw):
+    p = 1 << 20
+    d = dict(param=p, exp_avg=p, exp_avg_sq=p, exp_avg_base=p, exp_avg_sq_base=p, count=300)
+    d.update(kw)
+    return (_hip.AdamTensor * 1)(_hip.AdamTensor(**d))
+
+
+def test_c_abi_refuses_bad_arguments():
+    """Nothing is launched: the pointers are never read."""
+    L, p, inf, nan = _hip.lib, 1 << 20, float('inf'), float('nan')
+    grads = (C.c_void_p * 1)(p)
+    for change, code in ((dict(lr=-1.0), -6), (dict(lr=nan), -6), (dict(lr=inf), -6), (dict(beta1=1.0), -6), (dict(beta2=-0.1), -6),
+                         (dict(eps=-1.0), -6), (dict(eps=nan), -6), (dict(weight_decay=-1.0), -6), (dict(polyak=1.1), -6),
+                         (dict(max_norm=-1.0), -6), (dict(max_norm=inf), -6), (dict(step=0), -6), (dict(dtype=7), -5),
+                         (dict(state_bits=16), -5), (dict(clock=p + 4, step=0), -4)):
+        assert L.mpe_adamw_step(_args(**change), 1, _table(), p, grads, None) == code, change
+    for change, code in ((dict(param=None), -1), (dict(exp_avg=None), -1), (dict(exp_avg_sq=None), -1), (dict(count=-1), -6),
+                         (dict(param=p + 2), -4), (dict(target=p + 1), -4), (dict(exp_avg=p + 4), -4), (dict(exp_avg_sq=p + 8), -4)):
+        assert L.mpe_adamw_step(_args(), 1, _table(**change), p, grads, None) == code, change
+        assert L.mpe_adamw_plan(1, _table(**change), _hip.F32, 32, None, 0) == code, change
+    assert L.mpe_adamw_step(_args(state_bits=8), 1, _table(exp_avg_base=None), p, grads, None) == -1
+    assert L.mpe_adamw_step(_args(state_bits=8), 1, _table(exp_avg_sq_base=p + 1), p, grads, None) == -4
+    assert L.mpe_adamw_step(_args(), 1, _table(), p, (C.c_void_p * 1)(p + 2), None) == -4
+    assert L.mpe_adamw_step(_args(), 1, _table(), p + 4, grads, None) == -4
+    assert L.mpe_adamw_step(None, 1, _table(), p, grads, None) == -1
+    assert L.mpe_adamw_step(_args(), 1, _table(), None, grads, None) == -1
+    assert L.mpe_adamw_step(_args(), 1, None, p, grads, None) == -1
+    assert L.mpe_adamw_step(_args(), 1, _table(), p, None, None) == -1
+    assert L.mpe_adamw_step(_args(), 0, _table(), p, grads, None) == -6
+    need = L.mpe_adamw_plan(1, _table(), _hip.F32, 32, None, 0)
+    blob = torch.empty(need, dtype=torch.uint8)
+    assert need > 0 and L.mpe_adamw_plan(1, _table(), _hip.F32, 32, blob.data_ptr(), need) == need
+    assert L.mpe_adamw_plan(1, _table(), _hip.F32, 32, blob.data_ptr(), need - 1) == -7
+    for bad in ((p, p, p, 100, 1, 0), (p, p, p, 128, 2, 0), (p, p, p, -128, 1, 0)):
+        assert L.mpe_adamw_moments(*bad, None) == -6
+    assert L.mpe_adamw_moments(p, p, p, 128, 1, 2, None) == -5
+    assert L.mpe_adamw_moments(None, p, p, 128, 1, 0, None) == -1
+    assert L.mpe_adamw_moments(p + 4, p, p, 128, 1, 0, None) == -4
+    assert C.sizeof(_hip.AdamTensor) == 56 and C.sizeof(_hip.AdamArgs) == 96
+
+
+# ---- the 8-bit moments in numpy ------------------------------------------------------------------------------------------
+def _mix(h):
+    h = h ^ (h >> np.uint32(16))
+    h = h * np.uint32(0x85EBCA6B)
+    h = h ^ (h >> np.uint32(13))
+    h = h * np.uint32(0xC2B2AE35)
+    return h ^ (h >> np.uint32(16))
+
+
+def _random_bits(seed, step, tensor, index):
+    with np.errstate(over='ignore'):
+        k = _mix(np.array([(seed + step * 0x9E3779B9) & 0xFFFFFFFF], dtype=np.uint32)) ^ np.uint32(seed >> 32)
+        k = _mix(k + np.uint32((tensor * 0x85EBCA77) & 0xFFFFFFFF))
+        return _mix(index.astype(np.uint32) ^ (k + (index >> 32).astype(np.uint32) * np.uint32(0x9E3779B1)))
+
+
+def _encode(x, rnd, signed):
+    top = 127 if signed else 255
+    pad = -x.size % 128
+    bits = np.pad(x.view(np.uint32) & np.uint32(0x7FFFFFFF), (0, pad)).astype(np.int64)
+    neg = np.pad(x.view(np.uint32) >> np.uint32(31), (0, pad)).astype(np.int64)
+    rnd = np.pad(rnd.astype(np.int64), (0, pad))
+    base = np.maximum((bits.reshape(-1, 128).max(1) >> 20) + 1 - top, 0)
+    code = np.maximum((np.minimum(bits + rnd, 0x7FFFFFFF) >> 20) - np.repeat(base, 128), 0)
+    code = code | neg << 7 if signed else np.maximum(code, bits > 0)
+    return code[:x.size].astype(np.uint8), base.astype(np.int16)
+
+
+def _decode(code, base, signed):
+    mag = (code & 127 if signed else code).astype(np.int64)
+    b = np.repeat(base.astype(np.int64), 128)[:code.size]
+    x = np.where(mag > 0, (mag + b) << 20, 0).astype(np.uint32).view(np.float32)
+    return np.where(code > 127, -x, x).astype(np.float32) if signed else x
+
+
+def _step8(code_m, base_m, code_v, base_v, g, scale, step, seed, tensor, index, b1=0.9, b2=0.999):
+    f = np.float32
+    gc = g * f(scale)
+    m = _decode(code_m, base_m, True) * f(b1) + gc * f(1 - b1)
+    v = _decode(code_v, base_v, False) * f(b2) + (gc * gc) * f(1 - b2)
+    r = _random_bits(seed, step, tensor, index)
+    return _encode(m, (r >> np.uint32(16)) << np.uint32(4), True) + _encode(v, (r & np.uint32(0xFFFF)) << np.uint32(4), False) + (m, v)
+
+
+def test_the_restated_code_holds_what_the_text_says():
+    """Every code's value survives the round trip; rounding errs by less than an eighth of a binade, zero on average."""
+    r = np.random.RandomState(0)
+    x = (r.standard_normal(128 * 64) * np.exp(r.standard_normal(128 * 64))).astype(np.float32)
+    rnd = r.randint(0, 1 << 16, x.size).astype(np.uint32) << np.uint32(4)
+    for signed, y in ((True, x), (False, x * x)):
+        code, base = _encode(y, rnd, signed)
+        held = _decode(code, base, signed)
+        big = np.abs(y) > np.repeat(np.abs(y).reshape(-1, 128).max(1), 128) * 2.0 ** -14
+        assert (np.abs(held - y)[big] <= np.abs(y)[big] / 8).all()
+        # mean error of n roundings, each below 1/8 with zero mean: 5 sigma of a uniform-like error
+        assert abs(float(np.mean((held - y)[big] / y[big]))) < 5 * 0.125 / math.sqrt(int(big.sum()))
+        again, base2 = _encode(held, np.zeros_like(rnd), signed)
+        assert np.array_equal(_decode(again, base2, signed)[big], held[big])
+    code, base = _encode(np.array([1.0, 1e-20, 0.0], dtype=np.float32), np.zeros(3, np.uint32), False)
+    assert code.tolist()[1:] == [1, 0]                                 # v > 0 is never held as zero
+
+
+# ---- steps against 64 bits -----------------------------------------------------------------------------------------------
+SIZES = [(1,), (7,), (128,), (129, 3), (64, 64), (5,), (8192,), (8193,), (0,), (300, 100), (64,), (31, 17)]
+
+
+def _tensors(sizes, dtype, seed, scale=1.0, offset=0):
+    """Tensors in one array, ``offset`` elements apart: bases of every alignment."""
+    g = torch.Generator().manual_seed(seed)
+    out, flat = [], torch.zeros(sum(math.prod(s) + offset for s in sizes) + offset, dtype=dtype, device='cuda')
+    at = offset
+    for s in sizes:
+        c = math.prod(s)
+        t = flat[at:at + c].view(s)
+        t.copy_(torch.randn(s, generator=g) * scale)
+        out.append(t)
+        at += c + offset
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('clip,target,offset', [(None, False, 0), (0.5, True, 1), (3.0, False, 3), (None, True, 5)])
+def test_steps_follow_the_formulas(bits, dtype, clip, target, offset):
+    """Three steps.  32 bits: m and v to 4 roundings of f32; the parameter to its own rounding and those of the step.
+    8 bits: the codes equal numpy's float32 restatement; the parameter follows from the moments before they are rounded."""
+    lr, b1, b2, eps, wd, rho, seed = 1e-2, 0.9, 0.999, 1e-8, 0.1, 0.9, (5 << 32) + 77
+    ps = _tensors(SIZES, dtype, 1, 0.3, offset)
+    ts = _tensors(SIZES, dtype, 2, 0.3, offset) if target else None
+    opt = optim.AdamW(ps, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd, state_bits=bits, max_norm=clip, targets=ts,
+                      polyak=rho, seed=seed)
+    e, h = 2.0 ** -24, HALF[dtype]
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0               # half a step under f16's normal range
+    for step in range(1, 4):
+        gs = _tensors(SIZES, dtype, 10 + step, 0.05, offset)
+        before = [(p.double().flatten(), None if not target else t.double().flatten(), {k: v.clone() for k, v in opt.state[p].items()})
+                  for p, t in zip(ps, ts or ps)]
+        for p, g in zip(ps, gs):
+            p.grad = g
+        opt.step()
+        assert opt.step_count == step
+        for j, (p, g, (p0, t0, st)) in enumerate(zip(ps, gs, before)):
+            if p.numel() == 0:
+                continue
+            gd = g.double().flatten()
+            norm = float(gd.norm())
+            s32 = np.float32(clip) / max(np.float32(norm), np.float32(clip)) if clip else np.float32(1)
+            gc = gd * float(s32)
+            if bits == 32:
+                m0, v0 = st['exp_avg'].double().flatten(), st['exp_avg_sq'].double().flatten()
+            else:
+                cm, bm, cv, bv = (st[k].cpu().numpy().ravel() for k in ('exp_avg', 'exp_avg_base', 'exp_avg_sq', 'exp_avg_sq_base'))
+                want = _step8(cm, bm, cv, bv, g.float().flatten().cpu().numpy(), s32, step, seed, j, np.arange(p.numel()))
+                for k, w in zip(('exp_avg', 'exp_avg_base', 'exp_avg_sq', 'exp_avg_sq_base'), want):
+                    assert np.array_equal(opt.state[p][k].cpu().numpy().ravel(), w), (j, k)
+                m0 = torch.from_numpy(_decode(cm, bm, True)).double().cuda()
+                v0 = torch.from_numpy(_decode(cv, bv, False)).double().cuda()
+            m, v = b1 * m0 + (1 - b1) * gc, b2 * v0 + (1 - b2) * gc * gc
+            dm = 4 * e * (b1 * m0.abs() + (1 - b1) * gc.abs())       # g scale, two products, one sum, the factors' own rounding
+            dv = 6 * e * v
+            if bits == 32:
+                assert bool(((opt.state[p]['exp_avg'].double().flatten() - m).abs() <= dm + 1e-44).all())
+                assert bool(((opt.state[p]['exp_avg_sq'].double().flatten() - v).abs() <= dv + 1e-44).all())
+            denom = (v / (1 - b2 ** step)).sqrt() + eps
+            upd = lr / (1 - b1 ** step) * m / denom
+            pn = p0 * (1 - lr * wd) - upd
+            # m off by dm, denom by half of v's error and its own four roundings; quotient, two products, one sum
+            dp = lr / (1 - b1 ** step) * dm / denom + 12 * e * upd.abs() + 3 * e * p0.abs()
+            tol = dp + h * (pn.abs() + dp) * (1 + 1e-3) + tiny
+            assert bool(((p.double().flatten() - pn).abs() <= tol).all()), (j, step)
+            if target:
+                tn = rho * t0 + (1 - rho) * p.double().flatten()
+                tol = 4 * e * (t0.abs() + p.double().flatten().abs()) + h * tn.abs() * (1 + 1e-3) + tiny
+                assert bool(((ts[j].double().flatten() - tn).abs() <= tol).all()), (j, step)
+    if offset:                                                         # what lies between the tensors is still zero
+        flat = ps[0]._base
+        used = torch.zeros(flat.numel(), dtype=torch.bool, device='cuda')
+        for p in ps:
+            o = (p.data_ptr() - flat.data_ptr()) // p.element_size()
+            used[o:o + p.numel()] = True
+        assert not flat[~used].any()
+
+
+@pytest.mark.gpu
+def test_one_step_matches_torch_adam_at_zero_decay():
+    """weight_decay = 0: the learner's Adam (torch's, whose eps stands outside the corrected root as here)."""
+    torch.manual_seed(0)
+    a = [torch.randn(s, device='cuda') for s in SIZES]
+    b = [t.clone() for t in a]
+    for x in a + b:
+        x.requires_grad_()
+    mine, ref = optim.AdamW(a, lr=1e-2, weight_decay=0.0), torch.optim.Adam(b, lr=1e-2)
+    for k in range(5):
+        for x, y in zip(a, b):
+            x.grad = torch.randn(x.shape, device='cuda')
+            y.grad = x.grad.clone()
+        mine.step()
+        ref.step()
+    for x, y in zip(a, b):                                             # five steps of at most ~1e-2, each to a few 2^-24
+        assert torch.allclose(x, y, rtol=1e-6, atol=5 * 1e-2 * 20 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+def test_more_tensors_than_one_launch_holds_and_missing_gradients():
+    """600 variables (three launches), every third without a gradient: value and moments stay, the target still follows."""
+    sizes = [(1 + (i * 37) % 300,) for i in range(599)] + [(20000,)]
+    ps, ts = _tensors(sizes, torch.float32, 1), _tensors(sizes, torch.float32, 2)
+    gs = _tensors(sizes, torch.float32, 3)
+    p0, t0 = [p.clone() for p in ps], [t.clone() for t in ts]
+    opt = optim.AdamW(ps, lr=0.1, weight_decay=0.0, max_norm=0.5, targets=ts, polyak=0.75)
+    for i, (p, g) in enumerate(zip(ps, gs)):
+        p.grad = g if i % 3 else None
+    opt.step()
+    for i, p in enumerate(ps):
+        if i % 3 == 0:
+            assert torch.equal(p, p0[i]) and not opt.state[p]['exp_avg'].any()
+        else:                   # the first step: m / (1 - b1) = g', sqrt(v / (1 - b2)) = |g'|, so lr g' / (|g'| + eps): with
+            live = gs[i].abs() > 1e-3                                 # 20 000 elements clipped to 0.5, |g'| is down to 3.5e-6
+            gc = gs[i].double() * (0.5 / max(0.5, float(gs[i].double().norm())))
+            assert torch.allclose((p0[i] - p)[live].double(), (0.1 * gc / (gc.abs() + 1e-8))[live], rtol=1e-5, atol=1e-6)
+        assert torch.allclose(ts[i], 0.75 * t0[i] + 0.25 * p, rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_eight_bit_moments_are_right_on_average():
+    """1 500 steps of unit normal gradients: the mean of the held v over 16 384 elements follows the exact average.  One
+    element's v walks by 25 % (an eighth of a binade with probability 0.8 % a step, forgotten at 0.1 % a step); the mean
+    over 16 384 of them by 0.2 %, ten times which is allowed."""
+    p = torch.zeros(16384, device='cuda')
+    opt = optim.AdamW([p], lr=0.0, state_bits=8, seed=3)
+    g = torch.Generator(device='cuda').manual_seed(0)
+    v = torch.zeros(16384, device='cuda', dtype=torch.float64)
+    m = torch.zeros_like(v)
+    for _ in range(1500):
+        p.grad = torch.randn(16384, generator=g, device='cuda')
+        opt.step()
+        v = 0.999 * v + 0.001 * p.grad.double() ** 2
+        m = 0.9 * m + 0.1 * p.grad.double()
+    hm, hv = opt.moments()[0]
+    assert abs(float(hv.double().mean() / v.mean()) - 1) < 0.02
+    # m: rounding noise of at most 1/8 of |m| a step, remembered 5 steps (variance 1 / (1 - 0.81)), zero on average
+    assert abs(float((hm.double() - m).mean())) < 10 * 0.125 * float(m.abs().mean()) * math.sqrt(5.3) / 128
+    assert float((hm.double() - m).abs().mean()) < 0.3 * float(m.abs().mean())
+    assert torch.equal(opt.moments(torch.bfloat16)[0][0].float(), hm)     # bfloat16 holds the values
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_captured_steps_equal_eager_steps(bits):
+    """capturable: the step count lives on the device; replays between eager steps and other work, all equal to eager ones."""
+    def make():
+        ps, ts = _tensors(SIZES, torch.float32, 1), _tensors(SIZES, torch.float32, 2)
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        return ps, ts
+    (pa, ta), (pb, tb) = make(), make()
+    kw = dict(lr=1e-2, state_bits=bits, max_norm=0.5, seed=9)
+    a, b = optim.AdamW(pa, targets=ta, **kw), optim.AdamW(pb, targets=tb, capturable=True, **kw)
+    grads = [_tensors(SIZES, torch.float32, 20 + k) for k in range(5)]
+
+    def load(ps, k):
+        for p, g in zip(ps, grads[k]):
+            p.grad.copy_(g)
+    for k in range(2):
+        load(pa, k)
+        a.step()
+    load(pb, 0)
+    b.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode='thread_local'):
+        b.step()
+    assert b.step_count == 1                                          # a recording executes nothing
+    load(pb, 1)
+    graph.replay()
+    for k in range(2, 5):
+        load(pa, k)
+        a.step()
+        load(pb, k)
+        if k == 3:
+            b.step()
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert a.step_count == b.step_count == k + 1
+        for x, y in zip(pa + ta, pb + tb):
+            # the device's pow and the host's may differ in a last place of 64 bits: one rounding of each factor
+            assert torch.allclose(x, y, rtol=2.0 ** -21, atol=1e-2 * 2.0 ** -20)
+        for x, y in zip(a.buffers()[0].values(), b.buffers()[0].values()):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_state_dict_continues_a_run(bits):
+    sizes = [(40, 9), (3,)]
+    pa, pb = _tensors(sizes, torch.float32, 1), _tensors(sizes, torch.float32, 1)
+    a = optim.AdamW([dict(params=pa[:1], lr=0.1), dict(params=pa[1:])], state_bits=bits, seed=4)
+
+    def go(ps, opt, k):
+        for p, g in zip(ps, _tensors(sizes, torch.float32, 30 + k)):
+            p.grad = g
+        opt.step()
+    for k in range(3):
+        go(pa, a, k)
+    saved = a.state_dict()
+    for x, y in zip(pb, pa):
+        x.copy_(y)
+    b = optim.AdamW([dict(params=pb[:1]), dict(params=pb[1:])], state_bits=bits, seed=4, capturable=bits == 8)
+    held = b.buffers()[0]['exp_avg'].data_ptr()
+    b.load_state_dict(saved)
+    assert b.step_count == 3 and b.param_groups[0]['lr'] == 0.1 and b.buffers()[0]['exp_avg'].data_ptr() == held
+    for k in range(3, 5):
+        go(pa, a, k)
+        go(pb, b, k)
+    for x, y in zip(pa, pb):
+        assert torch.allclose(x, y, rtol=2.0 ** -21, atol=1e-1 * 2.0 ** -20)
+    for ga, gb in zip(a.buffers(), b.buffers()):
+        assert all(torch.equal(ga[k], gb[k]) for k in ga)
+    for bad in (optim.AdamW(pb, state_bits=bits), optim.AdamW([dict(params=pb[:1]), dict(params=pb[1:])], state_bits=40 - bits)):
+        with pytest.raises(ValueError):
+            bad.load_state_dict(saved)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+def test_values_that_are_not_finite(bits):
+    """An infinite or NaN gradient reaches its element (8 bits: its block of 128) and nothing else; with a clip its variable."""
+    sizes = [(400,), (300,)]
+    ps = _tensors(sizes, torch.float32, 1)
+    gs = _tensors(sizes, torch.float32, 2)
+    clean = [p.clone() for p in ps]
+    ref = optim.AdamW(clean, lr=0.1, state_bits=bits)
+    for p, g in zip(clean, gs):
+        p.grad = g.clone()
+    ref.step()
+    gs[0][130], gs[0][140] = float('inf'), float('nan')
+    opt = optim.AdamW(ps, lr=0.1, state_bits=bits)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt.step()
+    rest = [i for i in range(400) if i not in (130, 140)]
+    assert torch.equal(ps[0][rest], clean[0][rest]) and torch.equal(ps[1], clean[1]) and ps[0][[130, 140]].isnan().all()
+    m, v = opt.moments()[0]
+    rm, rv = ref.moments()[0]
+    out = [i for i in range(512 + 384) if not 128 <= i < 256]
+    assert torch.equal(m[out], rm[out]) and torch.equal(v[out], rv[out])
+    assert m[140].isnan() and v[140].isnan() and v[130] == float('inf')
+    clipped = optim.AdamW(ps, lr=0.1, state_bits=bits, max_norm=1.0)
+    before = ps[1].clone()
+    clipped.step()
+    assert ps[0].isnan().all() and torch.isfinite(ps[1]).all() and not torch.equal(ps[1], before)
+
+
+@pytest.mark.gpu
+def test_zero_gradients_and_zero_moments():
+    p = torch.randn(1000, device='cuda')
+    for bits in (8, 32):
+        x = p.clone()
+        x.grad = torch.zeros_like(x)
+        opt = optim.AdamW([x], lr=0.1, weight_decay=0.0, state_bits=bits, max_norm=0.5)
+        opt.step()
+        assert torch.equal(x, p) and not any(t.any() for t in opt.buffers()[0].values())
+
+
+@pytest.mark.gpu
+def test_groups_streams_versions_and_moved_parameters():
+    """Groups of different types and settings; a scheduler; a step on another stream; autograd notices the write; a
+    parameter whose storage was replaced is followed."""
+    a, b = torch.nn.Parameter(torch.ones(300, device='cuda')), torch.nn.Parameter(torch.ones(40, device='cuda').bfloat16())
+    opt = optim.AdamW([dict(params=[a], lr=0.5), dict(params=[b], weight_decay=0.0, max_norm=1.0)], lr=0.25, weight_decay=0.0)
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+    a.grad, b.grad = torch.ones_like(a), -torch.ones_like(b)
+    kept = (a * a).sum()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    sched.step()
+    assert torch.allclose(a, torch.full_like(a, 0.5)) and torch.allclose(b.float(), torch.full((40,), 1.25, device='cuda'))
+    with pytest.raises(RuntimeError):                                  # a changed behind the saved product
+        kept.backward()
+    a.data = a.data.clone()
+    a.grad = torch.ones(10, 30, device='cuda').t().reshape(300)
+    opt.step()
+    assert torch.allclose(a, torch.full_like(a, 0.25), atol=1e-6)
+    a.grad = None
+    loss = opt.step(lambda: torch.tensor(3.0))
+    assert float(loss) == 3.0
+    a.data = torch.ones(600, device='cuda')[::2]
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+@pytest.mark.gpu
+def test_arguments_are_checked():
+    p = torch.zeros(8, 4, device='cuda')
+    for kw in (dict(lr=-1), dict(lr=float('inf')), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1), dict(weight_decay=-1),
+               dict(max_norm=0.0), dict(max_norm=float('inf')), dict(polyak=2.0), dict(targets=[]), dict(targets=[torch.zeros(4, 8, device='cuda')]),
+               dict(targets=[p]), dict(targets=[torch.zeros(8, 4, device='cuda').half()])):
+        with pytest.raises(ValueError):
+            optim.AdamW([p], **kw)
+    for bad in ([p.t()], [p, p[:2].clone().half()], [p, p[1:]], [dict(params=[])]):
+        with pytest.raises(ValueError):
+            optim.AdamW(bad)
+    for bad in ([p.double()], [3.0]):
+        with pytest.raises(TypeError):
+            optim.AdamW(bad)
+    with pytest.raises(ValueError):
+        optim.AdamW([dict(params=[p])], targets=[p.clone()])
+    opt = optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    opt.param_groups[0]['lr'] = -1.0
+    with pytest.raises(ValueError):
+        opt.step()
+    with pytest.raises(ValueError):
+        opt.step_count = -1
+    with pytest.raises(TypeError):
+        opt.moments(torch.bfloat16)
+    with pytest.raises(TypeError):
+        optim.dequantize(torch.zeros(128, dtype=torch.uint8, device='cuda'), torch.zeros(1, dtype=torch.int16, device='cuda'), True, torch.float16)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A variable of more than 2^31 elements (its byte offsets pass 2^32): the last elements' step, 8-bit codes and target."""
+    n, last = (1 << 31) + 300, 1000
+    p = torch.zeros(n, dtype=torch.bfloat16, device='cuda')
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device='cuda')
+    g = torch.Generator(device='cuda').manual_seed(0)
+    p.grad[-last:] = torch.randn(last, generator=g, device='cuda').bfloat16()
+    opt = optim.AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, seed=11)
+    opt.step()
+    first = n - last
+    lo = first // 128 * 128
+    gn = p.grad[lo:].float().cpu().numpy()
+    z, zb = np.zeros(gn.size, np.uint8), np.zeros(-(-gn.size // 128), np.int16)
+    want = _step8(z, zb, z, zb, gn, 1.0, 1, 11, 0, np.arange(lo, n))
+    st = opt.state[p]
+    for k, w in zip(('exp_avg', 'exp_avg_base', 'exp_avg_sq', 'exp_avg_sq_base'), want):
+        got = st[k][lo // 128:] if k.endswith('base') else st[k][lo:]
+        assert np.array_equal(got.cpu().numpy(), w), k
+    assert not p[:first].any() and not st['exp_avg'][:lo].any()
+    live = p.grad[first:].float().abs() > 1e-3
+    assert torch.allclose(p[first:].float()[live], -0.5 * p.grad[first:].float().sign()[live], rtol=2.0 ** -7)

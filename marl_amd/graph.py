@@ -350,3 +350,53 @@ class CapturedUpdates(object):
         self._draw()
         self.graph.replay()
         return self.last
+
+
+class CapturedLearners(object):
+    """``CapturedUpdates`` for a ``marl_amd.learners.Learners``: all learners' updates of a due step (grouped products, one
+    AdamW step per network kind) as ONE HIP-graph replay, whose launch count does not grow with the number of agents.
+
+    Construct it at a step where the update is due: the constructor performs that update eagerly and records the same calls;
+    ``replay()`` performs one update per call.  Batch indices are drawn outside the graph; nothing of it goes through
+    autograd, so eager graphs of the networks may live beside it.  Returns every trainer's statistics as device scalars
+    (overwritten by the next replay)."""
+
+    def __init__(self, learners):
+        if not learners.due(0):
+            raise RuntimeError('every replay buffer must hold max_replay_buffer_len transitions (maddpg.py:162)')
+        self.learners = learners
+        from .maddpg import pack_actor
+        for tr in learners.trainers:
+            if tr._packed is None:
+                tr._packed = pack_actor(tr.p)
+        self.index = torch.zeros(learners.n, learners.batch, dtype=torch.int64, device=learners.device)
+        self._draw()
+        first = learners.update_from_index(self.index)
+        self.graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize(learners.device)
+        checks = [tr.replay_buffer.check_index for tr in learners.trainers]
+        try:
+            for tr in learners.trainers:
+                tr.replay_buffer.check_index = False   # the range check reads the indices back on the host
+            with _hip.on_device(learners.device):
+                with torch.cuda.graph(self.graph, capture_error_mode='thread_local'):
+                    self.last = learners.update_from_index(self.index)
+        finally:
+            for tr, c in zip(learners.trainers, checks):
+                tr.replay_buffer.check_index = c
+        for outs, eager in zip(self.last, first):      # a capture computes nothing: `last` reports the eager update
+            for o, e in zip(outs, eager):
+                o.copy_(e)
+
+    def _draw(self):
+        for tr in self.learners.trainers:
+            if tr.replay_buffer.compact:               # as in CapturedUpdates
+                tr.replay_buffer._flush_pending()
+        self.index.copy_(self.learners.draw())
+        for tr, idx in zip(self.learners.trainers, self.index):
+            tr.replay_sample_index = idx
+
+    def replay(self):
+        self._draw()
+        self.graph.replay()
+        return self.last

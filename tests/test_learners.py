@@ -1,0 +1,171 @@
+"""marl_amd.learners: all learners' updates as grouped products and AdamW steps against the loop over trainers."""
+import types
+
+import pytest
+import torch
+
+from marl_amd import maddpg
+from marl_amd.maddpg import MADDPGAgentTrainer, mlp_model
+from marl_amd.spaces import Discrete
+
+pytestmark = pytest.mark.gpu
+
+
+def _setup(scenario='simple_tag', B=512, local=False, batch=256, **kw):
+    from marl_amd import make_env
+    env = make_env(scenario, num_envs=B, dtype=torch.float32, seed=0)
+    args = types.SimpleNamespace(lr=1e-2, gamma=0.95, batch_size=batch, num_units=64, max_episode_len=4)
+    obs_shape_n = [env.observation_space[i].shape for i in range(env.n)]
+    torch.manual_seed(123)
+    trainers = [MADDPGAgentTrainer('agent_%d' % i, obs_shape_n, env.action_space, i, args, local_q_func=local, replay_size=B * 20,
+                                   seed=0, **kw) for i in range(env.n)]
+    obs_n = env.reset()
+    for k in range(6):
+        action_n = maddpg.act_all(trainers, obs_n)
+        new_obs_n, rew_n, done_n, _ = env.step(action_n)
+        for i, tr in enumerate(trainers):
+            tr.experience(obs_n[i], action_n[i], rew_n[i], new_obs_n[i], done_n[i], k == 5)
+        obs_n = new_obs_n
+    return env, trainers
+
+
+def _fixed(monkeypatch):
+    """u = 1/2 everywhere: the soft sample without its noise."""
+    monkeypatch.setattr(maddpg, 'soft_sample', lambda flat, sizes, generator=None: torch.cat(
+        [torch.softmax(p, dim=-1) for p in torch.split(flat, sizes, dim=-1)], dim=-1))
+
+
+def _index(trainers, k):
+    r = torch.Generator().manual_seed(k)
+    tr = trainers[0]
+    return torch.stack([torch.randint(0, len(tr.replay_buffer), (tr.args.batch_size,), generator=r) for _ in trainers]).cuda()
+
+
+NETS = ('p', 'q', 'target_p', 'target_q')
+
+
+@pytest.mark.parametrize('local', [False, True], ids=['joint', 'local'])
+@pytest.mark.parametrize('scenario', ['simple_tag', 'S1L2F2_3Targets_100observe'])
+def test_the_update_equals_the_loop_over_trainers_with_targets_held(scenario, local, monkeypatch):
+    """Two updates.  The loop runs every trainer from the networks as they were before the step.  Gradients: sums of 256
+    products through three layers in f32, ~2^-24 a rounding: within 1e-4 of the variable's largest; parameters: Adam turns a
+    gradient into a step of its sign, so all but the few elements whose gradient is itself rounding agree to 1e-4 (1 % of a
+    step); statistics to 1e-4."""
+    from marl_amd.learners import Learners
+    _fixed(monkeypatch)
+    (_, ta), (_, tb) = _setup(scenario, local=local), _setup(scenario, local=local)
+    seen, clip = [], maddpg.clip_by_norm_
+    monkeypatch.setattr(maddpg, 'clip_by_norm_', lambda params, c: (lambda ps: (seen.append([p.grad.clone() for p in ps]), clip(ps, c)))(list(params)))
+    learners = Learners(tb)
+    mine, step = [], Learners._step
+    monkeypatch.setattr(Learners, '_step', staticmethod(lambda opt, grads: (mine.append([g.clone() for g in grads]), step(opt, grads))))
+    for k in range(2):
+        index = _index(ta, k)
+        before = [{n: [w.detach().clone() for w in getattr(tr, n).parameters()] for n in NETS} for tr in ta]
+        after, stats = [], []
+        for i, tr in enumerate(ta):
+            stats.append([float(x) for x in tr.update_from_index(ta, index[i])])
+            after.append({n: [w.detach().clone() for w in getattr(tr, n).parameters()] for n in NETS})
+            with torch.no_grad():
+                for n in NETS:
+                    for w, w0 in zip(getattr(tr, n).parameters(), before[i][n]):
+                        w.copy_(w0)
+        got = learners.update_from_index(index)
+        for i, tr in enumerate(ta):
+            for kind in range(2):                                           # the critic's, the policy's
+                for a, b in zip(seen[2 * i + kind], mine[kind]):
+                    b = b[i]
+                    part = b[tuple(slice(s) for s in a.shape)]
+                    assert float((a - part).abs().max()) <= 1e-4 * float(a.abs().max()), (k, i, kind)
+                    assert int((part != 0).sum()) == int((b != 0).sum())    # nothing in the padding
+            assert torch.allclose(torch.tensor([float(x) for x in got[i]]), torch.tensor(stats[i]), rtol=1e-4, atol=1e-4)
+            with torch.no_grad():
+                for n in NETS:
+                    for w, w1, mw in zip(getattr(tr, n).parameters(), after[i][n], getattr(tb[i], n).parameters()):
+                        off = (w1 - mw).abs()
+                        assert float((off > 1e-4).float().mean()) < 0.01 and float(off.max()) <= 2.1e-2 * (k + 1), (k, i, n)
+                        w.copy_(mw)                                         # go on from the same networks
+        seen.clear()
+        mine.clear()
+
+
+def test_captured_learners_equal_eager_ones(monkeypatch):
+    """Three updates: the first eager, two replays with acting, an eager autograd graph of the same networks and a host
+    synchronisation in between; networks, targets, packed actors and statistics equal the eager run's, bit for bit."""
+    from marl_amd.graph import CapturedLearners
+    from marl_amd.learners import Learners
+    _fixed(monkeypatch)
+    (_, ta), (_, tb) = _setup(), _setup()
+    la, lb = Learners(ta), Learners(tb)
+    draws = {'a': 0, 'b': 0}
+
+    def draw(name, trainers):
+        draws[name] += 1
+        return _index(trainers, draws[name])
+    la.draw, lb.draw = (lambda: draw('a', ta)), (lambda: draw('b', tb))
+    want, got = [], []
+    for t in (100, 200, 300):
+        want.append([[float(x) for x in row] for row in la.update(t)])
+    cap = CapturedLearners(lb)
+    got.append([[float(x) for x in row] for row in cap.last])
+    for _ in range(2):
+        loss = tb[0].q(torch.randn(8, tb[0].q[0].in_features, device='cuda')).sum()     # lives across the replay
+        rows = cap.replay()
+        torch.cuda.synchronize()
+        got.append([[float(x) for x in row] for row in rows])
+        del loss
+    assert want == got
+    for a, b in zip(ta, tb):
+        for n in NETS:
+            assert all(torch.equal(x, y) for x, y in zip(getattr(a, n).parameters(), getattr(b, n).parameters())), n
+        assert torch.equal(b._packed, maddpg.pack_actor(b.p)) and torch.equal(a._packed, b._packed)
+        assert torch.equal(a.replay_sample_index, b.replay_sample_index)
+    assert la.p_opt.step_count == lb.p_opt.step_count == 3
+
+
+@pytest.mark.parametrize('compact', [False, True], ids=['full', 'compact'])
+def test_a_training_loop_with_eight_bit_moments(compact):
+    """Acting, storing and updating go on through the stacked networks; update() keeps the trainers' gates."""
+    from marl_amd.learners import Learners
+    env, trainers = _setup('simple_spread', replay_compact=compact)
+    learners = Learners(trainers, state_bits=8, seed=1)
+    assert learners.update(99) is None
+    w0 = [tr.target_q[0].weight.detach().clone() for tr in trainers]
+    for t in (100, 200, 300):
+        out = learners.update(t)
+        assert len(out) == len(trainers) and all(torch.isfinite(x) for row in out for x in row)
+        acts = maddpg.act_all(trainers, env.reset())
+        assert all(torch.isfinite(a).all() for a in acts)
+    for tr, w in zip(trainers, w0):
+        assert torch.equal(tr._packed, maddpg.pack_actor(tr.p)) and not torch.equal(tr.target_q[0].weight, w)
+    assert len(trainers[0].replay_sample_index) == 256
+
+
+def test_networks_and_trainers_that_do_not_fit_are_refused():
+    from marl_amd.graph import CapturedLearners
+    from marl_amd.learners import Learners
+
+    def make(n=2, local=(False, False), model=mlp_model, dtype=torch.float32, units=(64, 64)):
+        return [MADDPGAgentTrainer('a%d' % i, [(6,), (4,)][:n], [Discrete(5), Discrete(5)][:n], i,
+                                   types.SimpleNamespace(lr=1e-2, gamma=0.95, batch_size=8, num_units=units[i], max_episode_len=2),
+                                   local_q_func=local[i], model=model, dtype=dtype, replay_size=64) for i in range(n)]
+    trainers = make()
+    with pytest.raises(ValueError):
+        Learners(trainers[::-1])
+    with pytest.raises(ValueError):
+        Learners(trainers[:1])
+    with pytest.raises(NotImplementedError):
+        Learners(make(local=(False, True)))
+    with pytest.raises(NotImplementedError):
+        Learners(make(units=(64, 32)))
+    with pytest.raises(NotImplementedError):
+        Learners(make(model=lambda a, b, num_units: torch.nn.Sequential(torch.nn.Linear(a, b))))
+    with pytest.raises(TypeError):
+        Learners(make(dtype=torch.float64))
+    learners = Learners(trainers)
+    assert learners.update(100) is None                                     # empty buffers: no update is due
+    with pytest.raises(ValueError):
+        learners.update_from_index(torch.zeros(2, 7, dtype=torch.int64, device='cuda'))
+    with pytest.raises(RuntimeError):
+        CapturedLearners(learners)
+    assert Learners(make(n=1)).n == 1

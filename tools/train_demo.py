@@ -1,12 +1,14 @@
 """The reference's training loop shape (experiments/simple_train.py:257-300) entirely on one GPU: batched env
 step -> per-agent replay rings -> MADDPG updates every 100 steps.  Prints agent-steps/s with the learner in the
 loop (run on the GPU box from the repo root):
-    python tools/train_demo.py [scenario] [num_envs] [steps] [eager|graph] [compact|full|store] [f16actor]
+    python tools/train_demo.py [scenario] [num_envs] [steps] [eager|graph] [compact|full|store] [f16actor] [grouped|adam8]
 One episode (25 iterations) is one HIP-graph replay (marl_amd.graph.CapturedTrainSteps) and the learners' updates
 another (CapturedUpdates) unless `eager` is given.  `compact`: replay rings that store obs_tp1 once
 (marl_amd.replay_buffer.ReplayBuffer(compact=True)).  `store`: no append at all -- the actors and the env step write
 into the slots of a marl_amd.replay_buffer.StepStore (104 slots = 4 windows of 26; CapturedStoreSteps).  `f16actor`: the
-opt-in actor kernel on two f16 pieces per operand (MPE_ACTOR_MFMA_F16: ~1e-6 instead of ~4e-7 against PyTorch f32)."""
+opt-in actor kernel on two f16 pieces per operand (MPE_ACTOR_MFMA_F16: ~1e-6 instead of ~4e-7 against PyTorch f32).
+`grouped`: all learners' updates at once (marl_amd.learners.Learners, recorded by CapturedLearners); `adam8`: the same with
+the Adam moments in 8 bits."""
 import os
 import sys
 import time
@@ -16,7 +18,8 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from marl_amd import make_env  # noqa: E402
-from marl_amd.graph import CapturedStoreSteps, CapturedTrainSteps, CapturedUpdates  # noqa: E402
+from marl_amd.graph import CapturedLearners, CapturedStoreSteps, CapturedTrainSteps, CapturedUpdates  # noqa: E402
+from marl_amd.learners import Learners  # noqa: E402
 from marl_amd.maddpg import MADDPGAgentTrainer, act_all  # noqa: E402
 from marl_amd.replay_buffer import StepStore, add_all  # noqa: E402
 
@@ -34,6 +37,7 @@ def main():
     eager = len(sys.argv) > 4 and sys.argv[4] == 'eager'
     use_store = len(sys.argv) > 5 and sys.argv[5] == 'store'
     actor_kernel = 3 if 'f16actor' in sys.argv[6:] else 0
+    learners = Learners(trainers, state_bits=8 if 'adam8' in sys.argv[6:] else 32) if {'grouped', 'adam8'} & set(sys.argv[6:]) else None
     obs_n = env.reset()
     t0 = None
     store = None
@@ -74,21 +78,24 @@ def main():
         for tr in trainers:
             tr.preupdate()
         due = t % 100 == 0 and all(len(tr.replay_buffer) >= tr.max_replay_buffer_len for tr in trainers)
-        if eager or not due:
+        if learners is not None and (eager or not due):
+            out = learners.update(t)
+            out = out and out[-1]
+        elif eager or not due:
             for tr in trainers:
                 out = tr.update(trainers, t)            # every 100 steps (maddpg.py:161-163), i.e. every 4th episode
         elif updates is None:
-            updates = CapturedUpdates(trainers)         # performs this step's update and records it
+            updates = CapturedLearners(learners) if learners is not None else CapturedUpdates(trainers)   # performs this step's update and records it
             out = updates.last[-1]
         else:
-            out = updates.replay()[-1]                  # all four learners' updates: one HIP-graph replay
+            out = updates.replay()[-1]                  # all the learners' updates: one HIP-graph replay
         if out is not None:
             print('step %5d  q_loss %.4f  p_loss %.4f  mean reward %.3f' % (t, float(out[0]), float(out[1]), float(out[3])))
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     print('%s: %d envs x %d steps with %d learners in the loop (%s, replay: %s): %.3f ms/step, %.3e agent-steps/s'
           % (scenario, B, steps, env.n, 'eager' if eager else 'one graph replay per episode',
-             ('step store (no append)' if use_store else ('compact records' if compact else 'full records')) + ('; f16 actor kernel' if actor_kernel else ''), 1e3 * dt / steps,
+             ('step store (no append)' if use_store else ('compact records' if compact else 'full records')) + ('; f16 actor kernel' if actor_kernel else '') + ('; grouped updates' if learners is not None else ''), 1e3 * dt / steps,
              B * env.n * steps / dt))
 
 

@@ -3,6 +3,17 @@
 #include "mpe_grouped_kernel.h"
 
 using namespace mpe;
+#ifndef MKC
+#define MKC 4
+#define MST 4
+#endif
+#ifndef SKC
+#define SKC 8
+#define SST 2
+#endif
+#ifndef LARGE_MEAN
+#define LARGE_MEAN 384
+#endif
 
 namespace {
 
@@ -22,14 +33,31 @@ int grouped_check(const mpe_grouped_desc *d) {
   return MPE_OK;
 }
 
-struct DwPlan { int tiles_i, tiles_j, splits; };
+// Tiles (rows x columns of the output, wavefronts): small 64 x 64 (2 x 2), middle 128 x 128 (2 x 2), large 256 x 256 (2 x 4).
+enum Tile { SMALL = 0, MIDDLE = 1, LARGE = 2 };
+constexpr int kTile[3] = {64, 128, 256};
 
-constexpr int kBM = 64, kBN = 64;
+// A 16-bit product is bound by what the tile reads from LDS per matrix instruction: the largest tile that still leaves every
+// CU a workgroup and does not mostly overhang its group's rows.  f32 matrix instructions are 16 times slower: small tiles.
+Tile pick_tile(int dtype, bool fast, int64_t mean_rows, int64_t cols, int64_t groups_rows, int64_t others) {
+  if (dtype == MPE_F32) return SMALL;
+  const auto tiles = [&](int64_t t) { return (groups_rows + t - 1) / t * ((cols + t - 1) / t) * others; };
+  if (fast && mean_rows >= LARGE_MEAN && cols >= 256 && tiles(256) >= 256) return LARGE;
+  if (mean_rows >= 96 && cols >= 96 && tiles(128) >= 256) return MIDDLE;
+  return SMALL;
+}
+
+struct DwPlan { Tile tile; int tiles_i, tiles_j, splits; };
 
 DwPlan dw_plan(const mpe_grouped_desc *d) {
-  DwPlan p{(d->n + kBM - 1) / kBM, (d->k + kBN - 1) / kBN, 1};
-  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * d->groups;
   const int64_t mean = d->rows / d->groups;
+  DwPlan p;
+  // here rows and columns are n and k; the contraction runs over the group's rows
+  p.tile = pick_tile(d->dtype, false, d->n, d->k, d->n, d->groups);
+  p.tiles_i = (d->n + kTile[p.tile] - 1) / kTile[p.tile];
+  p.tiles_j = (d->k + kTile[p.tile] - 1) / kTile[p.tile];
+  p.splits = 1;
+  const int64_t tiles = (int64_t)p.tiles_i * p.tiles_j * d->groups;
   while (p.splits < 64 && tiles * p.splits < 512 && mean / (p.splits * 2) >= 64) p.splits *= 2;
   return p;
 }
@@ -46,26 +74,46 @@ GroupedArgs base_args(const mpe_grouped_desc *d) {
   return a;
 }
 
-template <typename T, int MODE>
-int launch_rows(GroupedArgs a, int cols, hipStream_t s) {
-  a.tiles_j = (cols + kBN - 1) / kBN;
-  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;  // groups (and the tail) with rows: each may add a partial tile
-  const int64_t grid = (a.rows / kBM + most) * a.tiles_j;
+template <typename T, int MODE, int TILE, int WM, int WN, int PATH, int KC, int STAGES>
+int launch_tile(const GroupedArgs &a, int64_t grid, hipStream_t s) {
   if (grid > kMaxGrid) return MPE_ERR_ARG;
-  hipLaunchKernelGGL((grouped_kernel<T, MODE, kBM, kBN, 2, 2>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((grouped_kernel<T, MODE, TILE, TILE, WM, WN, PATH, KC, STAGES>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, a);
   return (int)hipGetLastError();
 }
 
+template <typename T, int MODE, int PATH>
+int launch_as(const GroupedArgs &a, Tile tile, int64_t grid, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (PATH != GROUPED_ANY && MODE != GROUPED_DW)
+      if (tile == LARGE) return launch_tile<T, MODE, 256, 2, 4, PATH, PATH == GROUPED_FAST ? 4 : 8, PATH == GROUPED_FAST ? 4 : 2>(a, grid, s);
+    if (tile != SMALL) return launch_tile<T, MODE, 128, 2, 2, PATH, PATH == GROUPED_FAST ? MKC : 8, PATH == GROUPED_FAST ? MST : 2>(a, grid, s);
+  }
+  return launch_tile<T, MODE, 64, 2, 2, PATH, PATH == GROUPED_FAST ? SKC : 8, PATH == GROUPED_FAST ? SST : 2>(a, grid, s);
+}
+
+template <typename T, int MODE>
+int launch(const GroupedArgs &a, bool fast, Tile tile, int64_t grid, hipStream_t s) {
+  if (!fast) return launch_as<T, MODE, GROUPED_ANY>(a, tile, grid, s);
+  if constexpr (MODE != GROUPED_FWD)
+    if (a.mask) return launch_as<T, MODE, GROUPED_FAST_MASK>(a, tile, grid, s);
+  return launch_as<T, MODE, GROUPED_FAST>(a, tile, grid, s);
+}
+
+template <typename T, int MODE>
+int launch_rows(GroupedArgs a, bool fast, int dtype, int cols, hipStream_t s) {
+  const Tile tile = pick_tile(dtype, fast, a.rows / a.groups, cols, a.rows, 1);
+  a.tiles_j = (cols + kTile[tile] - 1) / kTile[tile];
+  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;  // groups (and the tail) with rows: each may add a partial tile
+  return launch<T, MODE>(a, fast, tile, (a.rows / kTile[tile] + most) * a.tiles_j, s);
+}
+
 template <typename T>
-int launch_dw(GroupedArgs a, const DwPlan &p, hipStream_t s) {
+int launch_dw(GroupedArgs a, bool fast, const DwPlan &p, hipStream_t s) {
   a.tiles_i = p.tiles_i;
   a.tiles_j = p.tiles_j;
   a.splits = p.splits;
-  const int64_t grid = (int64_t)p.tiles_i * p.tiles_j * p.splits * a.groups;
-  if (grid > kMaxGrid) return MPE_ERR_ARG;
-  hipLaunchKernelGGL((grouped_kernel<T, GROUPED_DW, kBM, kBN, 2, 2>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return (int)e;
+  const int rc = launch<T, GROUPED_DW>(a, fast, p.tile, (int64_t)p.tiles_i * p.tiles_j * p.splits * a.groups, s);
+  if (rc || p.splits == 1) return rc;
   const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = (int64_t)a.groups * a.n;
   hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024)), dim3(256), 0, s, a.part, (T *)a.out, cw, p.splits);
   if (a.dbias)
@@ -73,12 +121,18 @@ int launch_dw(GroupedArgs a, const DwPlan &p, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-#define BY_TYPE(dtype, call)                        \
-  ((dtype) == MPE_F32 ? call<float> : (dtype) == MPE_BF16 ? call<__bf16> : call<_Float16>)
+// An array whose rows are whole aligned 16-byte chunks, and a tile of which (256 lines) spans less than kGroupedSpan
+bool chunked(const void *p, int64_t ld, int64_t cols, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * size % 16 == 0 && cols * size % 16 == 0 &&
+         ld < (int64_t)kGroupedSpan / (256 * size);
+}
 
-template <typename T> int fwd(const GroupedArgs &a, hipStream_t s) { return launch_rows<T, GROUPED_FWD>(a, a.n, s); }
-template <typename T> int dx(const GroupedArgs &a, hipStream_t s) { return launch_rows<T, GROUPED_DX>(a, a.k, s); }
-template <typename T> int dw(const GroupedArgs &a, const DwPlan &p, hipStream_t s) { return launch_dw<T>(a, p, s); }
+template <int MODE>
+int launch_type(const GroupedArgs &a, int dtype, bool fast, int cols, hipStream_t s) {
+  return dtype == MPE_F32    ? launch_rows<float, MODE>(a, fast, dtype, cols, s)
+         : dtype == MPE_BF16 ? launch_rows<__bf16, MODE>(a, fast, dtype, cols, s)
+                             : launch_rows<_Float16, MODE>(a, fast, dtype, cols, s);
+}
 
 }  // namespace
 
@@ -102,7 +156,8 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
   a.ld_out = ld_y;
   a.relu = relu;
   a.zero_tail = zero_tail;
-  return BY_TYPE(d->dtype, fwd)(a, (hipStream_t)stream);
+  const bool fast = chunked(x, ld_x, d->k, size) && chunked(weight, d->k, d->k, size);
+  return launch_type<GROUPED_FWD>(a, d->dtype, fast, d->n, (hipStream_t)stream);
 }
 
 extern "C" int mpe_grouped_linear_dx(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
@@ -124,7 +179,8 @@ extern "C" int mpe_grouped_linear_dx(const mpe_grouped_desc *d, const void *dy, 
   a.out = dx_;
   a.ld_out = ld_dx;
   a.zero_tail = zero_tail;
-  return BY_TYPE(d->dtype, dx)(a, (hipStream_t)stream);
+  const bool fast = chunked(dy, ld_dy, d->n, size) && (!y || chunked(y, ld_y, d->n, size)) && chunked(weight, d->k, d->k, size);
+  return launch_type<GROUPED_DX>(a, d->dtype, fast, d->k, (hipStream_t)stream);
 }
 
 extern "C" int64_t mpe_grouped_dw_workspace(const mpe_grouped_desc *d) {
@@ -158,5 +214,9 @@ extern "C" int mpe_grouped_linear_dw(const mpe_grouped_desc *d, const void *dy, 
   a.dbias = dbias;
   a.part = (float *)workspace;
   a.part_bias = a.part + (need > 0 ? (int64_t)p.splits * d->groups * d->n * d->k : 0);
-  return BY_TYPE(d->dtype, dw)(a, p, (hipStream_t)stream);
+  const bool fast = d->rows > 0 && chunked(dy, ld_dy, d->n, size) && (!y || chunked(y, ld_y, d->n, size)) && chunked(x, ld_x, d->k, size);
+  hipStream_t s = (hipStream_t)stream;
+  return d->dtype == MPE_F32    ? launch_dw<float>(a, fast, p, s)
+         : d->dtype == MPE_BF16 ? launch_dw<__bf16>(a, fast, p, s)
+                                : launch_dw<_Float16>(a, fast, p, s);
 }

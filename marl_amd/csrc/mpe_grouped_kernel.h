@@ -68,6 +68,12 @@ __device__ __forceinline__ int64_t grouped_end(const GroupedArgs &a, int g) {
   return a.ends64 ? static_cast<const int64_t *>(a.ends)[g] : (int64_t)static_cast<const int32_t *>(a.ends)[g];
 }
 
+// A value that all lanes hold alike, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
+
 // Rows [r0, r1) of group g (dw).  Every wavefront computes it for itself.
 __device__ __forceinline__ void grouped_rows_of(const GroupedArgs &a, int g, int64_t &r0, int64_t &r1) {
   const int lane = threadIdx.x & 63;
@@ -83,8 +89,8 @@ __device__ __forceinline__ void grouped_rows_of(const GroupedArgs &a, int g, int
     lo = l2 > lo ? l2 : lo;
     hi = h2 > hi ? h2 : hi;
   }
-  r0 = lo < a.rows ? lo : a.rows;
-  r1 = hi < a.rows ? hi : a.rows;
+  r0 = uniform(lo < a.rows ? lo : a.rows);
+  r1 = uniform(hi < a.rows ? hi : a.rows);
 }
 
 // The group of row tile `tile` (tiles of BM rows, counted group by group) and its rows [r0, r1); behind the last group's
@@ -117,9 +123,9 @@ __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int
     const uint64_t hit = __ballot(tile < sum);
     if (hit != 0) {
       const int w = __ffsll((unsigned long long)hit) - 1;
-      const int64_t first = __shfl(s, w), last = __shfl(e, w);
+      const int64_t first = uniform(__shfl(s, w)), last = uniform(__shfl(e, w));
       g = base + w;
-      r0 = first + (int64_t)(tile - __shfl(sum - mine, w)) * BM;
+      r0 = first + (int64_t)(tile - uniform(__shfl(sum - mine, w))) * BM;
       r1 = last < r0 + BM ? last : r0 + BM;
       return true;
     }
@@ -129,16 +135,36 @@ __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int
   return false;
 }
 
-// One operand's tile: ROWS of i (or j) by 128 bytes of c, staged from memory through registers to LDS.
-//   CONTIG (c contiguous in memory): LDS holds [row][8 chunks of 16 bytes], chunk q of row i at place q ^ (i & 7), so that
-//   eight rows' chunks of one column lie in different banks; a fragment is one 16-byte read.
-//   otherwise (row index contiguous): LDS holds [c][ROWS].
-template <typename T, int ROWS, int NT, bool CONTIG>
+__device__ const uint4 kGroupedZero = {0, 0, 0, 0};  // what a chunk outside the arrays is read from
+
+constexpr uint32_t kGroupedSpan = 0x80000000u;  // bytes a tile's copies may reach (the host checks it)
+
+// One operand's tile: ROWS of i (or j) by KC 16-byte chunks of c (KC = 4 or 8), in LDS.
+//   CONTIG (c contiguous in memory): [row][KC chunks], chunk q of row i at place q ^ swizzle(i): the 16 rows of a fragment
+//   are spread over the banks; a fragment is one 16-byte read.
+//   otherwise (row index contiguous in memory): [c][ROWS elements], the 16 elements of a fragment's row range (one unit) at
+//   place unit ^ swizzle(c), so that the c's which one read touches lie in different banks; a fragment is two transposing
+//   reads (16 bits) or four 4-byte reads (f32).
+// Two ways in.  FAST (bases and row strides multiples of 16 bytes, whole chunks: checked on the host): straight from memory
+// to LDS, or through registers where dy is masked; a chunk outside the tile's rows or columns is fetched from a zero.
+// Otherwise through registers, element by element at the edges.
+template <typename T, int ROWS, int KC, int NT, bool CONTIG, bool FAST>
 struct GroupedOperand {
-  static constexpr int CE = 16 / sizeof(T), KE = 128 / sizeof(T), N = ROWS * 8 / NT;
-  static_assert(ROWS * 8 % NT == 0, "whole chunks per thread");
+  static constexpr int CE = 16 / sizeof(T), N = ROWS * KC / NT;
+  static constexpr int kLine = CONTIG ? KC : ROWS / CE;  // chunks of a line (a row, or a c)
+  static constexpr int kUnit = 16 / CE;                 // chunks of 16 elements
+  static_assert(ROWS * KC % NT == 0, "whole chunks per thread");
   uint4 r[N];
 
+  static __device__ __forceinline__ int swizzle(int line) {  // on chunks for CONTIG, on units otherwise
+    if (CONTIG) return KC == 8 ? line & 7 : (line >> 2) & 3;
+    if (sizeof(T) == 4) return (line >> 2) & 3;
+    if (ROWS == 64) return ((line >> 1) & 1) | ((line >> 3) & 1) << 1;
+    return (line & 3) | ((line >> 3) & 1) << 2;
+  }
+  static __device__ __forceinline__ int place(int line, int pos) {  // of chunk pos of a line; its own inverse in pos
+    return CONTIG ? pos ^ swizzle(line) : (((pos / kUnit) ^ swizzle(line)) * kUnit + pos % kUnit);
+  }
   static __device__ __forceinline__ uint4 load(const T *p, int64_t off, int valid) {
     if (valid >= CE) return __builtin_bit_cast(uint4, *reinterpret_cast<const Chunk16<T> *>(p + off));
     Chunk16<T> c;
@@ -146,53 +172,104 @@ struct GroupedOperand {
     for (int e = 0; e < CE; ++e) c.v[e] = e < valid ? p[off + e] : T(0);
     return __builtin_bit_cast(uint4, c);
   }
-  // keeps the elements of v whose saved output is > 0 or NaN (as relu's derivative: zero where y <= 0)
+  // keeps the elements of v whose saved output is > 0 or NaN (relu's derivative: zero where y <= 0)
   static __device__ __forceinline__ uint4 keep(uint4 v, uint4 y) {
-    Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, v), m = __builtin_bit_cast(Chunk16<T>, y);
+    if constexpr (sizeof(T) == 4) {
+      Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, v), m = __builtin_bit_cast(Chunk16<T>, y);
 #pragma unroll
-    for (int e = 0; e < CE; ++e) c.v[e] = (float)m.v[e] <= 0.0f ? T(0) : c.v[e];
-    return __builtin_bit_cast(uint4, c);
+      for (int e = 0; e < CE; ++e) c.v[e] = m.v[e] <= 0.0f ? 0.0f : c.v[e];
+      return __builtin_bit_cast(uint4, c);
+    } else {
+    // two elements an instruction: positive bits stay, of the others only what lies above -infinity (NaN); times 0 or 1
+    typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+    typedef short i2 __attribute__((ext_vector_type(2)));
+    const unsigned short ninf = __builtin_bit_cast(unsigned short, (T)(-__builtin_inff()));
+    uint32_t *c = reinterpret_cast<uint32_t *>(&v);
+    const uint32_t *m = reinterpret_cast<const uint32_t *>(&y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const u2 b = __builtin_bit_cast(u2, m[e]);
+      const u2 nan = __builtin_elementwise_sub_sat(b, u2{ninf, ninf});
+      const u2 pos = __builtin_bit_cast(u2, __builtin_elementwise_max(__builtin_bit_cast(i2, b), i2{0, 0}));
+      c[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u2, c[e]) * __builtin_elementwise_min(nan | pos, u2{1, 1}));
+    }
+    return v;
+    }
   }
   // p: element (row 0, c 0) of the tile column; rows / cs: how many of them from there exist
   __device__ __forceinline__ void fetch(const T *p, int64_t ld, const T *mask, int64_t ld_mask, int64_t rows, int64_t cs) {
     const int t = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int id = t + u * NT;
-      int64_t line, valid;
-      int pos;
-      if (CONTIG) {
-        line = id >> 3;
-        pos = (id & 7) * CE;
-        valid = line < rows ? cs - pos : 0;
+      const int id = t + u * NT, line = id / kLine, pos = (id % kLine) * CE;
+      const int64_t valid = CONTIG ? (line < rows ? cs - pos : 0) : (line < cs ? rows - pos : 0);
+      if (FAST) {
+        const T *zero = reinterpret_cast<const T *>(&kGroupedZero);
+        r[u] = *reinterpret_cast<const uint4 *>(valid > 0 ? p + line * ld + pos : zero);
+        if (mask != nullptr) r[u] = keep(r[u], *reinterpret_cast<const uint4 *>(valid > 0 ? mask + line * ld_mask + pos : zero));
       } else {
-        line = id / (ROWS / CE);
-        pos = (id % (ROWS / CE)) * CE;
-        valid = line < cs ? rows - pos : 0;
+        const int v = valid < 0 ? 0 : (valid < CE ? (int)valid : CE);
+        r[u] = v > 0 ? load(p, line * ld + pos, v) : uint4{0, 0, 0, 0};
+        if (mask != nullptr && v > 0) r[u] = keep(r[u], load(mask, line * ld_mask + pos, v));
       }
-      const int v = valid < 0 ? 0 : (valid < CE ? (int)valid : CE);
-      r[u] = v > 0 ? load(p, line * ld + pos, v) : uint4{0, 0, 0, 0};
-      if (mask != nullptr && v > 0) r[u] = keep(r[u], load(mask, line * ld_mask + pos, v));
     }
   }
   __device__ __forceinline__ void put(uint4 *lds) const {
-    const int t = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int id = t + u * NT;
-      if (CONTIG) lds[(id >> 3) * 8 + ((id & 7) ^ ((id >> 3) & 7))] = r[u];
-      else lds[id] = r[u];
+      const int id = threadIdx.x + u * NT, line = id / kLine;
+      lds[line * kLine + place(line, id % kLine)] = r[u];
     }
   }
-  // lane l's share of k-step kk: row i0 + l % 16, c = kk * 4 CE + (l / 16) * CE .. + CE
-  static __device__ __forceinline__ uint4 frag(const uint4 *lds, int i0, int kk) {
-    const int lane = threadIdx.x & 63, i = i0 + (lane & 15), q = kk * 4 + (lane >> 4);
-    if (CONTIG) return lds[i * 8 + (q ^ (i & 7))];
-    const T *s = reinterpret_cast<const T *>(lds);
-    Chunk16<T> c;
+  // Without registers: a wavefront's 64 chunks land side by side in LDS, so each lane fetches what belongs at its place.
+  // at: the chunks' byte offsets in the tile; left: how many c's exist from there on (none for a chunk outside the rows).
+  // A chunk with nothing left is given an offset outside the buffer, which reads as zeros.
+  uint32_t at[N];
+  int left[N];
+  __device__ __forceinline__ void aim(int64_t ld, int64_t rows, int64_t cs) {
 #pragma unroll
-    for (int e = 0; e < CE; ++e) c.v[e] = s[(q * CE + e) * ROWS + i];
-    return __builtin_bit_cast(uint4, c);
+    for (int u = 0; u < N; ++u) {
+      const int id = threadIdx.x + u * NT, line = id / kLine, pos = place(line, id % kLine) * CE;
+      at[u] = ((uint32_t)line * (uint32_t)ld + pos) * sizeof(T);
+      left[u] = (CONTIG ? line : pos) < rows ? (int)cs - (CONTIG ? pos : line) : 0;
+    }
+  }
+  __device__ __forceinline__ void copy(uint4 *lds, const T *p) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, kGroupedSpan, 0x00027000);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + u * NT + uniform((int)threadIdx.x & ~63)),
+                                               16, left[u] > 0 ? at[u] : kGroupedSpan, 0, 0, 0);
+      left[u] -= KC * CE;
+    }
+#endif
+  }
+  // lane l's share of k-step kk: row i0 + l % 16, c = kk * 4 CE + (l / 16) * CE .. + CE   (i0: a multiple of 16)
+  static __device__ __forceinline__ uint4 frag(const uint4 *lds, int i0, int kk) {
+    const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
+    if (CONTIG) return lds[(i0 + t) * KC + ((kk * 4 + q) ^ swizzle(t))];
+    if constexpr (sizeof(T) == 4) {
+      const float *s = reinterpret_cast<const float *>(lds);
+      float4 f;
+      float *v = reinterpret_cast<float *>(&f);
+      const int at = q * 4 * ROWS + ((i0 / 16) ^ swizzle(q * 4)) * 16 + t;  // swizzle: the same for every kk and e
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = s[(kk * 16 + e) * ROWS + at];
+      return __builtin_bit_cast(uint4, f);
+    } else {
+      // 16 lanes read 4 c's of 16 elements, 8 bytes a lane; each lane gets its element of the four
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      const short *s = reinterpret_cast<const short *>(lds);
+      uint4 out;
+      s4 *o = reinterpret_cast<s4 *>(&out);
+      const int c = q * 8 + (t >> 2), at = c * ROWS + ((i0 / 16) ^ swizzle(c)) * 16 + (t & 3) * 4;  // swizzle: the same for every kk and h
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4 *)const_cast<short *>(s + (kk * 32 + h * 4) * ROWS + at));
+      return out;
+    }
   }
 };
 
@@ -210,20 +287,34 @@ __device__ __forceinline__ void grouped_store4(T *p, f4v v, int valid) {
   }
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
-  constexpr int NT = 64 * WM * WN, KE = 128 / (int)sizeof(T);
+// Workgroups are handed to the eight dies in turn: consecutive tiles (which share a weight or its rows) go to one die's L2.
+__device__ __forceinline__ int grouped_block() {
+  const int n = gridDim.x, per = n / 8, more = n % 8, die = blockIdx.x % 8, at = blockIdx.x / 8;
+  return die * per + (die < more ? die : more) + at;
+}
+
+enum GroupedPath { GROUPED_ANY = 0, GROUPED_FAST = 1, GROUPED_FAST_MASK = 2 };  // how tiles are loaded; FAST_MASK: A times its mask
+
+// STAGES buffers of KC chunks a row: while one is multiplied, STAGES - 1 are on their way.
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int PATH, int KC, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_kernel(GroupedArgs a) {
+  constexpr bool FAST = PATH != GROUPED_ANY, regs_a = PATH != GROUPED_FAST;
+  constexpr int NT = 64 * WM * WN, KE = KC * 16 / (int)sizeof(T);
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
-  using OpA = GroupedOperand<T, BM, NT, MODE != GROUPED_DW>;
-  using OpB = GroupedOperand<T, BN, NT, MODE == GROUPED_FWD>;
-  __shared__ uint4 la[BM * 8], lb[BN * 8];
+  using OpA = GroupedOperand<T, BM, KC, NT, MODE != GROUPED_DW, FAST>;
+  using OpB = GroupedOperand<T, BN, KC, NT, MODE == GROUPED_FWD, FAST>;
+  static_assert(PATH == GROUPED_FAST || STAGES == 2, "what passes through registers is one stage ahead");
+  // separate arrays: the compiler then knows that a read of one does not wait for copies into another
+  constexpr int kStage = (BM + BN) * KC;  // A's chunks, then B's
+  __shared__ uint4 s0[kStage], s1[kStage], s2[STAGES > 2 ? kStage : 1], s3[STAGES > 3 ? kStage : 1];
   const T *pa = static_cast<const T *>(a.a), *pb = static_cast<const T *>(a.b), *pm = static_cast<const T *>(a.mask);
 
   // ---- which tile ------------------------------------------------------------------------------------------------------
+  const int block = grouped_block();
   int g, tj = 0, split = 0;
   int64_t i0, i_end, j0, j_end, c0, c_end;  // output rows, output columns, contraction
   if (MODE == GROUPED_DW) {
-    int id = blockIdx.x;
+    int id = block;
     tj = id % a.tiles_j;
     id /= a.tiles_j;
     const int ti = id % a.tiles_i;
@@ -240,8 +331,8 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
     j0 = (int64_t)tj * BN;
     j_end = a.k;
   } else {
-    tj = blockIdx.x % a.tiles_j;
-    if (!grouped_tile<BM>(a, blockIdx.x / a.tiles_j, g, i0, i_end)) return;
+    tj = block % a.tiles_j;
+    if (!grouped_tile<BM>(a, block / a.tiles_j, g, i0, i_end)) return;
     j0 = (int64_t)tj * BN;
     j_end = MODE == GROUPED_FWD ? a.n : a.k;
     c0 = 0;
@@ -255,21 +346,28 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
   const bool tail = MODE != GROUPED_DW && c_end == 0;
   if (MODE != GROUPED_DW) pb += (int64_t)g * a.n * a.k;
 
-  // ---- the product -----------------------------------------------------------------------------------------------------
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  // ---- the product: two stages, one barrier a k-step; the next stage is on its way while this one is multiplied ------------
+  const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   f4v acc[MI][NJ] = {}, accb[MI] = {};
   OpA oa;
   OpB ob;
-  auto fetch = [&](int64_t c) {
-    if (MODE == GROUPED_DW) {
-      oa.fetch(pa + c * a.ld_a + i0, a.ld_a, pm ? pm + c * a.ld_mask + i0 : nullptr, a.ld_mask, i_end - i0, c_end - c);
-      ob.fetch(pb + c * a.ld_b + j0, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
+  if constexpr (FAST) {
+    if constexpr (!regs_a) oa.aim(a.ld_a, i_end - i0, c_end - c0);
+    ob.aim(a.ld_b, j_end - j0, c_end - c0);
+  }
+  auto fetch = [&](int64_t c, uint4 *la) {
+    uint4 *lb = la + BM * KC;
+    const T *at = MODE == GROUPED_DW ? pa + c * a.ld_a + i0 : pa + i0 * a.ld_a + c;
+    const T *bt = MODE == GROUPED_FWD ? pb + j0 * a.ld_b + c : pb + c * a.ld_b + j0;
+    if constexpr (regs_a) {
+      const T *mt = pm == nullptr ? nullptr : MODE == GROUPED_DW ? pm + c * a.ld_mask + i0 : pm + i0 * a.ld_mask + c;
+      oa.fetch(at, a.ld_a, mt, a.ld_mask, i_end - i0, c_end - c);
     } else {
-      oa.fetch(pa + i0 * a.ld_a + c, a.ld_a, pm ? pm + i0 * a.ld_mask + c : nullptr, a.ld_mask, i_end - i0, c_end - c);
-      if (MODE == GROUPED_FWD) ob.fetch(pb + j0 * a.ld_b + c, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
-      else ob.fetch(pb + c * a.ld_b + j0, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
+      oa.copy(la, at);
     }
+    if constexpr (FAST) ob.copy(lb, bt);
+    else ob.fetch(bt, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
   };
   uint4 ones;
   {
@@ -279,14 +377,18 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
     ones = __builtin_bit_cast(uint4, o);
   }
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
-  if (c0 < c_end) fetch(c0);
-  for (int64_t c = c0; c < c_end; c += KE) {
-    oa.put(la);
-    ob.put(lb);
-    __syncthreads();
-    if (c + KE < c_end) fetch(c + KE);
+  constexpr int kAhead = (STAGES - 2) * (OpA::N + OpB::N);  // copies of later stages that may still be under way
+  auto step = [&](int64_t c, uint4 *la, uint4 *next) {
+    uint4 *lb = la + BM * KC;
+    if constexpr (regs_a) oa.put(la);
+    if constexpr (!FAST) ob.put(lb);
+    // this wavefront's copies of this stage have landed, its reads and writes of LDS are done; then so are everybody's
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(FAST ? kAhead : 63) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch(c + (STAGES - 1) * KE, next);  // past the end: zeros
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
+    for (int kk = 0; kk < KC / 4; ++kk) {
       uint4 fa[MI], fb[NJ];
 #pragma unroll
       for (int m = 0; m < MI; ++m) fa[m] = OpA::frag(la, wi + m * 16, kk);
@@ -301,42 +403,86 @@ __global__ __launch_bounds__(64 * WM * WN) void grouped_kernel(GroupedArgs a) {
 #pragma unroll
         for (int m = 0; m < MI; ++m) accb[m] = GroupedType<T>::mma(ones, fa[m], accb[m]);
     }
-    __syncthreads();
+  };
+  if (c0 < c_end) {
+    fetch(c0, s0);
+    if constexpr (STAGES > 2) fetch(c0 + KE, s1);
+    if constexpr (STAGES > 3) fetch(c0 + 2 * KE, s2);
+    for (int64_t c = c0; c < c_end; c += STAGES * KE) {  // steps past the end multiply zeros
+      if constexpr (STAGES == 2) {
+        step(c, s0, s1);
+        step(c + KE, s1, s0);
+      } else if constexpr (STAGES == 3) {
+        step(c, s0, s2);
+        step(c + KE, s1, s0);
+        step(c + 2 * KE, s2, s1);
+      } else {
+        step(c, s0, s3);
+        step(c + KE, s1, s0);
+        step(c + 2 * KE, s2, s1);
+        step(c + 3 * KE, s3, s2);
+      }
+    }
   }
 
   // ---- epilogue: lane holds output row i0 + wi + 16 m + lane % 16, columns j0 + wj + 16 n + 4 (lane / 16) .. + 4 ----------
+  const int64_t j_lane = j0 + wj + 4 * (lane >> 4);
+  const auto valid_of = [&](int n) { return j_end - j_lane - n * 16 >= 4 ? 4 : (int)(j_end - j_lane - n * 16); };
+  if constexpr (MODE == GROUPED_FWD) {
+    if (a.bias != nullptr && !tail) {  // all of it first: one wait
+      const T *b = static_cast<const T *>(a.bias) + (int64_t)g * a.n + j_lane;
+      f4v bias[NJ];
 #pragma unroll
-  for (int m = 0; m < MI; ++m) {
-    const int64_t i = i0 + wi + m * 16 + (lane & 15);
-    if (i >= i_end) continue;
-    if (with_bias && lane < 16) {
-      if (a.splits > 1) a.part_bias[((int64_t)split * a.groups + g) * a.n + i] = accb[m][0];
-      else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)accb[m][0];
+      for (int n = 0; n < NJ; ++n) {
+        const int valid = valid_of(n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bias[n][e] = e < valid ? (float)b[n * 16 + e] : 0.0f;
+      }
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) acc[m][n] += bias[n];
+    }
+    if (a.relu) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m][n][e] = acc[m][n][e] < 0.0f ? 0.0f : acc[m][n][e];  // NaN stays
+    }
+  }
+  const auto store = [&](auto *out, int64_t ld) {  // out: the array's row 0
+    auto *p = out + (i0 + wi + (lane & 15)) * ld + j_lane;
+    if (i0 + BM <= i_end && j0 + BN <= j_end) {  // the whole tile: no tests
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) grouped_store4(p + m * 16 * ld + n * 16, acc[m][n], 4);
+      return;
     }
 #pragma unroll
-    for (int n = 0; n < NJ; ++n) {
-      const int64_t j = j0 + wj + n * 16 + 4 * (lane >> 4);
-      const int valid = j_end - j >= 4 ? 4 : (int)(j_end - j);
-      if (valid <= 0) continue;
-      f4v v = acc[m][n];
-      if (MODE == GROUPED_DW) {
-        if (a.splits > 1) grouped_store4(a.part + (((int64_t)split * a.groups + g) * a.n + i) * a.k + j, v, valid);
-        else grouped_store4(static_cast<T *>(a.out) + ((int64_t)g * a.n + i) * a.k + j, v, valid);
-      } else {
-        if (MODE == GROUPED_FWD && !tail) {
-          if (a.bias) {
-            const T *b = static_cast<const T *>(a.bias) + (int64_t)g * a.n + j;
+    for (int m = 0; m < MI; ++m) {
+      if (i0 + wi + m * 16 + (lane & 15) >= i_end) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (e < valid) v[e] += (float)b[e];
-          }
-          if (a.relu)
+      for (int n = 0; n < NJ; ++n) grouped_store4(p + m * 16 * ld + n * 16, acc[m][n], valid_of(n));
+    }
+  };
+  if constexpr (MODE == GROUPED_DW) {
+    const int64_t part = ((int64_t)split * a.groups + g) * a.n;
+    if (with_bias && lane < 16) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];  // NaN stays
-        }
-        grouped_store4(static_cast<T *>(a.out) + i * a.ld_out + j, v, valid);
+      for (int m = 0; m < MI; ++m) {
+        const int64_t i = i0 + wi + m * 16 + lane;
+        if (i >= i_end) continue;
+        if (a.splits > 1) a.part_bias[part + i] = accb[m][0];
+        else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)accb[m][0];
       }
     }
+    if (a.splits > 1) store(a.part + part * a.k, a.k);
+    else store(static_cast<T *>(a.out) + (int64_t)g * a.n * a.k, a.k);
+  } else {
+    store(static_cast<T *>(a.out), a.ld_out);
   }
 }
 

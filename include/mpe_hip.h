@@ -562,14 +562,17 @@ int mpe_env_step_stats_static(const mpe_scenario_desc *desc, int64_t B, int64_t 
  * Row r of x [rows][k] belongs to group g when ends[g-1] <= r < ends[g] (ends[-1] = 0); weight [groups][n][k] and bias
  * [groups][n] are contiguous; accumulation in f32, one rounding to dtype at the end.
  *   mpe_grouped_linear     y = act(x W_g^T + b_g)            bias may be NULL; relu: 0 / 1 (NaN stays NaN)
- *   mpe_grouped_linear_dx  dx = d W_g                        d = dy, or with y (the saved relu output) dy where not y <= 0
- *   mpe_grouped_linear_dw  dweight_g = d_g^T x_g, dbias_g = column sums of d_g (dbias may be NULL); a group without rows
- *                          gets zeros.  Fixed summation order: the same inputs give the same bits
+ *   mpe_grouped_linear_backward, with d = dy, or where y (the saved relu output) is given dy where y is not <= 0:
+ *                          dx = d W_g (dx NULL: not wanted; weight is read for it alone);
+ *                          dweight_g = d_g^T x_g and dbias_g = column sums of d_g (dweight NULL: neither is wanted, x is
+ *                          not read; dbias NULL: not wanted); a group without rows gets zeros.  Fixed summation order: the
+ *                          same inputs give the same bits
  * ends is a device array of int32 (ends64 = 0) or int64 and is read by the kernel as its running maximum clamped to
  * [0, rows].  Rows behind the last group: untouched, or zeros with zero_tail = 1.  ld_* are row strides in elements, inner
  * stride 1, any alignment of an element.  dtype is of all float arrays.  1 <= groups <= 1024, rows and n * k below 2^31.
- * mpe_grouped_dw_workspace: bytes that mpe_grouped_linear_dw needs (>= 0, or MPE_ERR_*); the array is scratch of that
- * call, 16-byte aligned; calls that may overlap (other streams, concurrent graph replays) need one each.
+ * mpe_grouped_backward_workspace: bytes that mpe_grouped_linear_backward needs (>= 0, or MPE_ERR_*) with / without y and
+ * dweight; the array is scratch of that call, 16-byte aligned; calls that may overlap (other streams, concurrent graph
+ * replays) need one each.
  */
 #define MPE_F32 0
 #define MPE_BF16 1
@@ -581,12 +584,10 @@ typedef struct mpe_grouped_desc {
 } mpe_grouped_desc;
 int mpe_grouped_linear(const mpe_grouped_desc *desc, const void *x, int64_t ld_x, const void *weight, const void *bias,
                        void *y, int64_t ld_y, int relu, int zero_tail, void *stream);
-int mpe_grouped_linear_dx(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
-                          const void *weight, void *dx, int64_t ld_dx, int zero_tail, void *stream);
-int64_t mpe_grouped_dw_workspace(const mpe_grouped_desc *desc);
-int mpe_grouped_linear_dw(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
-                          const void *x, int64_t ld_x, void *dweight, void *dbias, void *workspace,
-                          int64_t workspace_bytes, void *stream);
+int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *desc, int with_y, int with_dweight);
+int mpe_grouped_linear_backward(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
+                                const void *x, int64_t ld_x, const void *weight, void *dx, int64_t ld_dx, int zero_tail,
+                                void *dweight, void *dbias, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * ADAMW over many tensors in one or a few launches, moments in 32 or in 8 bits, with the clip of each variable's gradient

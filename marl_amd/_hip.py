@@ -203,13 +203,11 @@ def _load():
     gp = C.POINTER(GroupedDesc)
     L.mpe_grouped_linear.restype = ci             # desc, x, ld_x, weight, bias, y, ld_y, relu, zero_tail, stream
     L.mpe_grouped_linear.argtypes = [gp, vp, i64, vp, vp, vp, i64, ci, ci, vp]
-    L.mpe_grouped_linear_dx.restype = ci          # desc, dy, ld_dy, y, ld_y, weight, dx, ld_dx, zero_tail, stream
-    L.mpe_grouped_linear_dx.argtypes = [gp, vp, i64, vp, i64, vp, vp, i64, ci, vp]
-    L.mpe_grouped_dw_workspace.restype = i64
-    L.mpe_grouped_dw_workspace.argtypes = [gp]
-    # desc, dy, ld_dy, y, ld_y, x, ld_x, dweight, dbias, workspace, workspace_bytes, stream
-    L.mpe_grouped_linear_dw.restype = ci
-    L.mpe_grouped_linear_dw.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, vp, vp, i64, vp]
+    L.mpe_grouped_backward_workspace.restype = i64  # desc, with_y, with_dweight
+    L.mpe_grouped_backward_workspace.argtypes = [gp, ci, ci]
+    # desc, dy, ld_dy, y, ld_y, x, ld_x, weight, dx, ld_dx, zero_tail, dweight, dbias, workspace, workspace_bytes, stream
+    L.mpe_grouped_linear_backward.restype = ci
+    L.mpe_grouped_linear_backward.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, vp, i64, ci, vp, vp, vp, i64, vp]
     ap = C.POINTER(AdamTensor)
     L.mpe_adamw_plan.restype = i64                # n, tensors, dtype, state_bits, blob (host), blob_bytes
     L.mpe_adamw_plan.argtypes = [ci, ap, ci, ci, vp, i64]

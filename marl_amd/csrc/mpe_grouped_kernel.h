@@ -157,9 +157,9 @@ struct GroupedOperand {
   uint4 r[N];
 
   static __device__ __forceinline__ int swizzle(int line) {  // on chunks for CONTIG, on units otherwise
-    if (CONTIG) return KC == 8 ? line & 7 : (line >> 2) & 3;
-    if (sizeof(T) == 4) return (line >> 2) & 3;
-    if (ROWS == 64) return ((line >> 1) & 1) | ((line >> 3) & 1) << 1;
+    if (CONTIG) return KC == 8 ? line & 7 : (line >> 1) & 3;  // 8 lanes' chunks in one pass of 128 bytes: 8 places
+    if (sizeof(T) == 4) return (line >> 2) & 3;               // 32 lanes on two c's four apart
+    if (ROWS == 64) return ((line >> 1) & 1) | ((line >> 3) & 1) << 1;  // 32 lanes on eight c's: 256 bytes
     return (line & 3) | ((line >> 3) & 1) << 2;
   }
   static __device__ __forceinline__ int place(int line, int pos) {  // of chunk pos of a line; its own inverse in pos
@@ -287,10 +287,14 @@ __device__ __forceinline__ void grouped_store4(T *p, f4v v, int valid) {
   }
 }
 
-// Workgroups are handed to the eight dies in turn: consecutive tiles (which share a weight or its rows) go to one die's L2.
+// Workgroups are handed to the eight dies in turn: runs of 32 consecutive tiles (which share a weight or its rows) go to one
+// die's L2.  Not longer runs: the grid has a few tiles too many at its end, which must not all fall to one die.
 __device__ __forceinline__ int grouped_block() {
-  const int n = gridDim.x, per = n / 8, more = n % 8, die = blockIdx.x % 8, at = blockIdx.x / 8;
-  return die * per + (die < more ? die : more) + at;
+  constexpr int kRun = 32;
+  const int b = blockIdx.x, n = gridDim.x;
+  if (b >= n / (8 * kRun) * (8 * kRun)) return b;
+  const int at = b / 8;
+  return at / kRun * (8 * kRun) + b % 8 * kRun + at % kRun;
 }
 
 enum GroupedPath { GROUPED_ANY = 0, GROUPED_FAST = 1, GROUPED_FAST_MASK = 2 };  // how tiles are loaded; FAST_MASK: A times its mask
@@ -349,7 +353,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   // ---- the product: two stages, one barrier a k-step; the next stage is on its way while this one is multiplied ------------
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
-  f4v acc[MI][NJ] = {}, accb[MI] = {};
+  f4v acc[MI][NJ] = {};
+  float sum[MI] = {};  // dbias: this lane's share of its rows' (n's) sums
   OpA oa;
   OpB ob;
   if constexpr (FAST) {
@@ -369,13 +374,6 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     if constexpr (FAST) ob.copy(lb, bt);
     else ob.fetch(bt, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
   };
-  uint4 ones;
-  {
-    Chunk16<T> o;
-#pragma unroll
-    for (int e = 0; e < OpA::CE; ++e) o.v[e] = T(1);
-    ones = __builtin_bit_cast(uint4, o);
-  }
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
   constexpr int kAhead = (STAGES - 2) * (OpA::N + OpB::N);  // copies of later stages that may still be under way
   auto step = [&](int64_t c, uint4 *la, uint4 *next) {
@@ -399,9 +397,14 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
       for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int n = 0; n < NJ; ++n) acc[m][n] = GroupedType<T>::mma(fb[n], fa[m], acc[m][n]);
-      if (with_bias)
+      if (with_bias) {
 #pragma unroll
-        for (int m = 0; m < MI; ++m) accb[m] = GroupedType<T>::mma(ones, fa[m], accb[m]);
+        for (int m = 0; m < MI; ++m) {
+          const Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, fa[m]);
+#pragma unroll
+          for (int e = 0; e < OpA::CE; ++e) sum[m] += (float)c.v[e];
+        }
+      }
     }
   };
   if (c0 < c_end) {
@@ -470,13 +473,15 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   };
   if constexpr (MODE == GROUPED_DW) {
     const int64_t part = ((int64_t)split * a.groups + g) * a.n;
-    if (with_bias && lane < 16) {
+    if (with_bias) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
+        float v = sum[m] + __shfl_xor(sum[m], 16);  // lanes l, l + 16, .. hold the same row's other c's
+        v += __shfl_xor(v, 32);
         const int64_t i = i0 + wi + m * 16 + lane;
-        if (i >= i_end) continue;
-        if (a.splits > 1) a.part_bias[part + i] = accb[m][0];
-        else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)accb[m][0];
+        if (lane >= 16 || i >= i_end) continue;
+        if (a.splits > 1) a.part_bias[part + i] = v;
+        else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)v;
       }
     }
     if (a.splits > 1) store(a.part + part * a.k, a.k);
@@ -484,6 +489,19 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   } else {
     store(static_cast<T *>(a.out), a.ld_out);
   }
+}
+
+// d = dy where y is not <= 0, zero elsewhere: both products of a backward pass then load it like any other operand.
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_mask_kernel(const T *dy, int64_t ld_dy, const T *y, int64_t ld_y, T *d, int64_t rows, int n) {
+  constexpr int CE = 16 / sizeof(T);
+  const int chunks = n / CE;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / chunks;
+  if (row >= rows) return;
+  const int col = (int)(at % chunks) * CE;
+  using Op = GroupedOperand<T, 64, 8, 256, true, true>;
+  *reinterpret_cast<uint4 *>(d + row * n + col) = Op::keep(*reinterpret_cast<const uint4 *>(dy + row * ld_dy + col),
+                                                          *reinterpret_cast<const uint4 *>(y + row * ld_y + col));
 }
 
 // dw over splits: the partial sums in split order, rounded once.

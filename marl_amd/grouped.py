@@ -1,5 +1,5 @@
 """Products grouped by agent (or expert) with ragged row counts: one dense layer of many networks in one launch
-(libmpe_hip.so: mpe_grouped_linear, mpe_grouped_linear_dx, mpe_grouped_linear_dw; no counterpart in the reference, whose
+(libmpe_hip.so: mpe_grouped_linear, mpe_grouped_linear_backward; no counterpart in the reference, whose
 learners evaluate one network at a time, maddpg/maddpg/trainer/maddpg.py:161-196).
 
     y = grouped_linear(x, weight, ends, bias=None, relu=False)       # y[r] = act(x[r] @ weight[g].T + bias[g])
@@ -144,28 +144,27 @@ def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dw
     result itself where it was made with ``relu=True`` (``grad`` counts where ``y`` is not <= 0).  An entry that is not needed
     is None.  ``dx`` is zero in rows of no group, ``dweight`` / ``dbias`` are zero for groups without rows."""
     _check(x, weight, ends)
-    shape = (x.shape[0], weight.shape[1])
+    shape, want_dweight = (x.shape[0], weight.shape[1]), need_dweight
     grad, ld_g = _rows_of(grad, 'grad', shape, x)
     ld_y = 0
     if y is not None:
         y, ld_y = _rows_of(y, 'y', shape, x)
     ends = ends.contiguous()
+    need_dweight = need_dweight or need_dbias
     desc, dx, dw, db = _desc(x, weight, ends), None, None, None
+    ld_x = 0
+    if need_dx:
+        weight = weight.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if need_dweight:
+        x, ld_x = _rows_of(x, 'x')
+        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
+        db = torch.empty(weight.shape[:2], dtype=x.dtype, device=x.device) if need_dbias else None
+    need = _hip.lib.mpe_grouped_backward_workspace(desc, y is not None, need_dweight)
+    _hip.check(min(need, 0), 'mpe_grouped_backward_workspace')
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with _hip.on_device(x.device):
-        stream = _hip.stream_of(x.device)
-        if need_dx:
-            weight = weight.contiguous()
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _hip.check(_hip.lib.mpe_grouped_linear_dx(desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, weight.data_ptr(),
-                                                      dx.data_ptr(), x.shape[1], 1, stream), 'mpe_grouped_linear_dx')
-        if need_dweight or need_dbias:
-            x, ld_x = _rows_of(x, 'x')
-            dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
-            db = torch.empty(weight.shape[:2], dtype=x.dtype, device=x.device) if need_dbias else None
-            need = _hip.lib.mpe_grouped_dw_workspace(desc)
-            _hip.check(min(need, 0), 'mpe_grouped_dw_workspace')
-            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-            _hip.check(_hip.lib.mpe_grouped_linear_dw(desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, x.data_ptr(), ld_x,
-                                                      dw.data_ptr(), _hip.ptr(db), _hip.ptr(ws), need, stream),
-                       'mpe_grouped_linear_dw')
-    return dx, dw if need_dweight else None, db
+        _hip.check(_hip.lib.mpe_grouped_linear_backward(
+            desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, x.data_ptr(), ld_x, weight.data_ptr(), _hip.ptr(dx), x.shape[1], 1,
+            _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need, _hip.stream_of(x.device)), 'mpe_grouped_linear_backward')
+    return dx, dw if want_dweight else None, db

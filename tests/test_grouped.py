@@ -39,9 +39,8 @@ def test_c_abi_refuses_bad_descriptors(change, code):
     """Nothing is launched: the pointers are never read."""
     d, p = _desc(**change), 1 << 20
     assert _hip.lib.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 0, None) == code
-    assert _hip.lib.mpe_grouped_linear_dx(d, p, 5, None, 0, p, p, 3, 0, None) == code
-    assert _hip.lib.mpe_grouped_dw_workspace(d) == code
-    assert _hip.lib.mpe_grouped_linear_dw(d, p, 5, None, 0, p, 3, p, None, None, 0, None) == code
+    assert _hip.lib.mpe_grouped_backward_workspace(d, 0, 1) == code
+    assert _hip.lib.mpe_grouped_linear_backward(d, p, 5, None, 0, p, 3, p, p, 3, 0, p, p, None, 0, None) == code
 
 
 def test_c_abi_refuses_bad_arrays():
@@ -54,13 +53,22 @@ def test_c_abi_refuses_bad_arrays():
     assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 2, None) == -6
     assert L.mpe_grouped_linear(d, p + 2, 3, p, None, p, 5, 0, 0, None) == -4
     assert L.mpe_grouped_linear(d, p, 3, p, p + 1, p, 5, 0, 0, None) == -4
-    assert L.mpe_grouped_linear_dx(d, p, 5, p, 4, p, p, 3, 0, None) == -6
-    assert L.mpe_grouped_linear_dw(d, p, 5, None, 0, p, 3, None, None, None, 0, None) == -1
+    ok = dict(dy=p, ld_dy=5, y=None, ld_y=0, x=p, ld_x=3, w=p, dx=p, ld_dx=3, zero=0, dw=p, db=p, ws=None, size=0)
+
+    def back(desc=d, **kw):
+        return L.mpe_grouped_linear_backward(desc, *dict(ok, **kw).values(), None)
+    for kw, code in ((dict(dy=None), -1), (dict(x=None), -1), (dict(w=None), -1), (dict(dw=None), -1), (dict(ld_dy=4), -6),
+                     (dict(y=p, ld_y=4), -6), (dict(ld_x=2), -6), (dict(ld_dx=2), -6), (dict(zero=2), -6), (dict(dy=p + 1), -4),
+                     (dict(y=p + 2, ld_y=5), -4), (dict(x=p + 2), -4), (dict(w=p + 2), -4), (dict(dx=p + 2), -4), (dict(dw=p + 2), -4),
+                     (dict(db=p + 2), -4), (dict(ws=p + 8), -4)):
+        assert back(**kw) == code, kw
+    assert L.mpe_grouped_backward_workspace(d, 2, 1) == -6 and L.mpe_grouped_backward_workspace(d, 0, -1) == -6
+    assert L.mpe_grouped_backward_workspace(d, 0, 1) == 0
     big = _desc(rows=1 << 20)                                     # rows split over workgroups: partial sums need an array
-    need = L.mpe_grouped_dw_workspace(big)
-    assert need > 0
-    assert L.mpe_grouped_linear_dw(big, p, 5, None, 0, p, 3, p, None, None, need, None) == -1
-    assert L.mpe_grouped_linear_dw(big, p, 5, None, 0, p, 3, p, None, p, need - 1, None) == -7
+    need = L.mpe_grouped_backward_workspace(big, 0, 1)
+    assert need > 0 and L.mpe_grouped_backward_workspace(big, 0, 0) == 0
+    assert back(big, ws=None, size=need) == -1
+    assert back(big, ws=p, size=need - 1) == -7
     assert C.sizeof(_hip.GroupedDesc) == 40
 
 
@@ -105,7 +113,8 @@ def _close(got, want, terms, count, dtype, what):
 SHAPES = [
     ([1], 1, 1), ([5], 3, 2), ([0, 1, 0], 7, 9), ([3, 0, 64, 65, 1], 16, 64), ([63, 64, 65], 33, 65), ([256] * 4, 64, 64),
     ([1000, 1, 0, 500], 226, 64), ([128, 129], 64, 5), ([17, 300, 3], 333, 517), ([200, 0, 56], 512, 256), ([0, 0], 8, 8),
-    ([2500], 130, 40), ([1] * 70, 20, 24), ([700, 900], 128, 136), ([1, 2, 1, 0, 3], 1024, 520)]
+    ([2500], 130, 40), ([1] * 70, 20, 24), ([700, 900], 128, 136), ([1, 2, 1, 0, 3], 1024, 520),
+    ([900, 0, 1300, 760], 512, 2048), ([4100, 5001], 2048, 264), ([3000, 2200], 130, 2050), ([1500] * 6, 1032, 1024)]
 
 
 @pytest.mark.gpu

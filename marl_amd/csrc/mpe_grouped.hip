@@ -13,6 +13,9 @@ using namespace mpe;
 #define SKC 8
 #define SST 2
 #endif
+#ifndef MASKSH
+#define MASKSH 18
+#endif
 #ifndef LBN
 #define LBN 256
 #define LWM 2
@@ -123,17 +126,15 @@ int launch_dw(GroupedArgs a, const mpe_grouped_desc *d, bool fast, hipStream_t s
   a.splits = dw_splits(d);
   const int rc = launch<T, GROUPED_DW>(a, fast, tile, dw_tiles(d, tile) * a.splits * a.groups, s);
   if (rc || a.splits == 1) return rc;
-  const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = (int64_t)a.groups * a.n;
-  hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024)), dim3(256), 0, s, a.part, (T *)a.out, cw, a.splits);
-  if (a.dbias)
-    hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cb + 1023) / 1024)), dim3(256), 0, s, a.part_bias, (T *)a.dbias, cb, a.splits);
+  const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = a.dbias ? (int64_t)a.groups * a.n : 0;
+  hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024 + (cb + 1023) / 1024)), dim3(256), 0, s, a.part,
+                     (T *)a.out, cw, a.part_bias, (T *)a.dbias, cb, a.splits);
   return (int)hipGetLastError();
 }
 
-// An array whose rows are whole aligned 16-byte chunks, and a tile of which (256 lines) spans less than kGroupedSpan
-bool chunked(const void *p, int64_t ld, int64_t cols, int size) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * size % 16 == 0 && cols * size % 16 == 0 &&
-         ld < (int64_t)kGroupedSpan / (256 * size);
+// An array that tiles may be copied from: dwords stay dwords from row to row, a tile (256 lines) spans less than kGroupedSpan
+bool copyable(const void *p, int64_t ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * size % 4 == 0 && ld < (int64_t)kGroupedSpan / (256 * size) - 16;
 }
 
 template <int MODE>
@@ -165,11 +166,19 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
   a.ld_out = ld_y;
   a.relu = relu;
   a.zero_tail = zero_tail;
-  const bool fast = chunked(x, ld_x, d->k, size) && chunked(weight, d->k, d->k, size);
+  const bool fast = copyable(x, ld_x, size) && copyable(weight, d->k, size);
   return launch_type<GROUPED_FWD>(a, d->dtype, fast, d->n, (hipStream_t)stream);
 }
 
 namespace {
+
+// A masked gradient is written once (in rows of whole chunks) and read by plain copies where there is enough of it; otherwise
+// each product masks what it loads.
+bool mask_first(const mpe_grouped_desc *d) { return d->rows * d->n >= (int64_t)1 << MASKSH; }
+int64_t masked_ld(const mpe_grouped_desc *d) {
+  const int chunk = 16 / dtype_size(d->dtype);
+  return (d->n + chunk - 1) / chunk * chunk;
+}
 
 // Scratch of a backward pass: the masked gradient, the partial sums of dweight and of dbias.
 struct Scratch { int64_t masked, part, part_bias, total; };
@@ -177,22 +186,17 @@ Scratch scratch_of(const mpe_grouped_desc *d, bool masked, bool want_dw) {
   const int splits = dw_splits(d);
   const auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
   Scratch s{};
-  s.part = masked ? up(d->rows * d->n * dtype_size(d->dtype)) : 0;
+  s.part = masked ? up(d->rows * masked_ld(d) * dtype_size(d->dtype)) : 0;
   const int64_t one = want_dw && splits > 1 ? (int64_t)splits * d->groups * d->n * 4 : 0;
   s.part_bias = s.part + up(one * d->k);
   s.total = s.part_bias + up(one);
   return s;
 }
 
-// A masked gradient is written once and read by plain copies where there is enough of it (rows of whole chunks); otherwise
-// each product masks what it loads.
-bool mask_first(const mpe_grouped_desc *d) {
-  return d->rows * d->n >= (int64_t)1 << 18 && (int64_t)d->n * dtype_size(d->dtype) % 16 == 0;
-}
-
 template <typename T>
 int launch_mask(const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, void *out, int64_t rows, int n, hipStream_t s) {
-  const int64_t grid = (rows * (n / (16 / (int)sizeof(T))) + 255) / 256;
+  constexpr int chunk = 16 / (int)sizeof(T);
+  const int64_t grid = (rows * ((n + chunk - 1) / chunk) + 255) / 256;
   if (grid > kMaxGrid) return MPE_ERR_ARG;
   hipLaunchKernelGGL(grouped_mask_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, (const T *)dy, ld_dy, (const T *)y, ld_y, (T *)out, rows, n);
   return (int)hipGetLastError();
@@ -223,17 +227,16 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   if (w.total > 0 && !workspace) return MPE_ERR_NULL;
   if (workspace_bytes < w.total) return MPE_ERR_SCRATCH;
   hipStream_t s = (hipStream_t)stream;
-  const bool fast_d = chunked(dy, ld_dy, d->n, size) && (!y || chunked(y, ld_y, d->n, size));
-  const bool fast_w = chunked(weight, d->k, d->k, size), fast_x = d->rows > 0 && chunked(x, ld_x, d->k, size);
-  if (masked && fast_d) {
+  if (masked) {
     const int rc = d->dtype == MPE_F32    ? launch_mask<float>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s)
                    : d->dtype == MPE_BF16 ? launch_mask<__bf16>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s)
                                           : launch_mask<_Float16>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s);
     if (rc) return rc;
     dy = workspace;
-    ld_dy = d->n;
+    ld_dy = masked_ld(d);
     y = nullptr;
   }
+  const bool fast_d = d->rows > 0 && copyable(dy, ld_dy, size);
   GroupedArgs a = base_args(d);
   a.a = dy;
   a.ld_a = ld_dy;
@@ -246,7 +249,7 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
     b.out = dx;
     b.ld_out = ld_dx;
     b.zero_tail = zero_tail;
-    if (const int rc = launch_type<GROUPED_DX>(b, d->dtype, fast_d && fast_w, d->k, s)) return rc;
+    if (const int rc = launch_type<GROUPED_DX>(b, d->dtype, fast_d && copyable(weight, d->k, size), d->k, s)) return rc;
   }
   if (!dweight) return MPE_OK;
   a.b = x;
@@ -255,7 +258,7 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   a.dbias = dbias;
   a.part = (float *)((char *)workspace + w.part);
   a.part_bias = (float *)((char *)workspace + w.part_bias);
-  return d->dtype == MPE_F32    ? launch_dw<float>(a, d, fast_d && fast_x, s)
-         : d->dtype == MPE_BF16 ? launch_dw<__bf16>(a, d, fast_d && fast_x, s)
-                                : launch_dw<_Float16>(a, d, fast_d && fast_x, s);
+  return d->dtype == MPE_F32    ? launch_dw<float>(a, d, fast_d && copyable(x, ld_x, size), s)
+         : d->dtype == MPE_BF16 ? launch_dw<__bf16>(a, d, fast_d && copyable(x, ld_x, size), s)
+                                : launch_dw<_Float16>(a, d, fast_d && copyable(x, ld_x, size), s);
 }

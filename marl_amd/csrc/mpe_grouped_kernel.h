@@ -135,9 +135,7 @@ __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int
   return false;
 }
 
-__device__ const uint4 kGroupedZero = {0, 0, 0, 0};  // what a chunk outside the arrays is read from
-
-constexpr uint32_t kGroupedSpan = 0x80000000u;  // bytes a tile's copies may reach (the host checks it)
+constexpr uint32_t kGroupedSpan = 0x7ffffff0u;  // bytes a tile's copies may reach (the host checks it); an offset outside
 
 // One operand's tile: ROWS of i (or j) by KC 16-byte chunks of c (KC = 4 or 8), in LDS.
 //   CONTIG (c contiguous in memory): [row][KC chunks], chunk q of row i at place q ^ swizzle(i): the 16 rows of a fragment
@@ -145,9 +143,10 @@ constexpr uint32_t kGroupedSpan = 0x80000000u;  // bytes a tile's copies may rea
 //   otherwise (row index contiguous in memory): [c][ROWS elements], the 16 elements of a fragment's row range (one unit) at
 //   place unit ^ swizzle(c), so that the c's which one read touches lie in different banks; a fragment is two transposing
 //   reads (16 bits) or four 4-byte reads (f32).
-// Two ways in.  FAST (bases and row strides multiples of 16 bytes, whole chunks: checked on the host): straight from memory
-// to LDS, or through registers where dy is masked; a chunk outside the tile's rows or columns is fetched from a zero.
-// Otherwise through registers, element by element at the edges.
+// Two ways in.  FAST (bases and row strides multiples of 4 bytes: checked on the host): straight from memory to LDS by buffer
+// loads, whose bounds (the array's end, checked dword by dword) and whose offset beyond every bound (rows and columns outside
+// the tile's) read as zeros; or through registers where dy is masked.  Otherwise through registers, element by element at
+// the edges.
 template <typename T, int ROWS, int KC, int NT, bool CONTIG, bool FAST>
 struct GroupedOperand {
   static constexpr int CE = 16 / sizeof(T), N = ROWS * KC / NT;
@@ -203,15 +202,9 @@ struct GroupedOperand {
     for (int u = 0; u < N; ++u) {
       const int id = t + u * NT, line = id / kLine, pos = (id % kLine) * CE;
       const int64_t valid = CONTIG ? (line < rows ? cs - pos : 0) : (line < cs ? rows - pos : 0);
-      if (FAST) {
-        const T *zero = reinterpret_cast<const T *>(&kGroupedZero);
-        r[u] = *reinterpret_cast<const uint4 *>(valid > 0 ? p + line * ld + pos : zero);
-        if (mask != nullptr) r[u] = keep(r[u], *reinterpret_cast<const uint4 *>(valid > 0 ? mask + line * ld_mask + pos : zero));
-      } else {
-        const int v = valid < 0 ? 0 : (valid < CE ? (int)valid : CE);
-        r[u] = v > 0 ? load(p, line * ld + pos, v) : uint4{0, 0, 0, 0};
-        if (mask != nullptr && v > 0) r[u] = keep(r[u], load(mask, line * ld_mask + pos, v));
-      }
+      const int v = valid < 0 ? 0 : (valid < CE ? (int)valid : CE);
+      r[u] = v > 0 ? load(p, line * ld + pos, v) : uint4{0, 0, 0, 0};
+      if (mask != nullptr && v > 0) r[u] = keep(r[u], load(mask, line * ld_mask + pos, v));
     }
   }
   __device__ __forceinline__ void put(uint4 *lds) const {
@@ -234,9 +227,11 @@ struct GroupedOperand {
       left[u] = (CONTIG ? line : pos) < rows ? (int)cs - (CONTIG ? pos : line) : 0;
     }
   }
-  __device__ __forceinline__ void copy(uint4 *lds, const T *p) {
+  // p: the tile at its next c; bytes: from there to the array's end
+  __device__ __forceinline__ void copy(uint4 *lds, const T *p, int64_t bytes) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, kGroupedSpan, 0x00027000);
+    const int records = (int)(bytes < 0 ? 0 : (bytes < (int64_t)kGroupedSpan ? bytes : (int64_t)kGroupedSpan));
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, records, 0x00027000);
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + u * NT + uniform((int)threadIdx.x & ~63)),
@@ -244,6 +239,21 @@ struct GroupedOperand {
       left[u] -= KC * CE;
     }
 #endif
+  }
+  // The last k-step of a c that ends inside a chunk: what the copies brought from behind it becomes zero (times the other
+  // operand's zeros it would still be NaN where it is not finite).  ago: copies since this stage's, itself included.
+  __device__ __forceinline__ void trim(uint4 *lds, int ago) {
+    if (!CONTIG) return;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int have = left[u] + ago * KC * CE;
+      if (have > 0 && have < CE) {
+        T *c = reinterpret_cast<T *>(lds + u * NT + threadIdx.x);
+#pragma unroll
+        for (int e = 1; e < CE; ++e)
+          if (e >= have) c[e] = T(0);
+      }
+    }
   }
   // lane l's share of k-step kk: row i0 + l % 16, c = kk * 4 CE + (l / 16) * CE .. + CE   (i0: a multiple of 16)
   static __device__ __forceinline__ uint4 frag(const uint4 *lds, int i0, int kk) {
@@ -348,7 +358,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     }
   }
   const bool tail = MODE != GROUPED_DW && c_end == 0;
-  if (MODE != GROUPED_DW) pb += (int64_t)g * a.n * a.k;
+  // bytes to the arrays' ends, whole dwords (their last 2-byte element may share one with nothing)
+  const auto end_of = [](int64_t lines, int64_t ld, int64_t cols) { return (((lines - 1) * ld + cols) * (int64_t)sizeof(T) + 3) & ~(int64_t)3; };
+  const int64_t end_a = end_of(a.rows, a.ld_a, MODE == GROUPED_FWD ? a.k : a.n);
+  const int64_t end_b = MODE == GROUPED_DW ? end_of(a.rows, a.ld_b, a.k) : end_of((int64_t)a.groups * a.n, a.k, a.k);
+  const int64_t b0 = MODE == GROUPED_DW ? 0 : (int64_t)g * a.n * a.k;
 
   // ---- the product: two stages, one barrier a k-step; the next stage is on its way while this one is multiplied ------------
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -363,16 +377,16 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   }
   auto fetch = [&](int64_t c, uint4 *la) {
     uint4 *lb = la + BM * KC;
-    const T *at = MODE == GROUPED_DW ? pa + c * a.ld_a + i0 : pa + i0 * a.ld_a + c;
-    const T *bt = MODE == GROUPED_FWD ? pb + j0 * a.ld_b + c : pb + c * a.ld_b + j0;
+    const int64_t at = MODE == GROUPED_DW ? c * a.ld_a + i0 : i0 * a.ld_a + c;
+    const int64_t bt = b0 + (MODE == GROUPED_FWD ? j0 * a.ld_b + c : c * a.ld_b + j0);
     if constexpr (regs_a) {
       const T *mt = pm == nullptr ? nullptr : MODE == GROUPED_DW ? pm + c * a.ld_mask + i0 : pm + i0 * a.ld_mask + c;
-      oa.fetch(at, a.ld_a, mt, a.ld_mask, i_end - i0, c_end - c);
+      oa.fetch(pa + at, a.ld_a, mt, a.ld_mask, i_end - i0, c_end - c);
     } else {
-      oa.copy(la, at);
+      oa.copy(la, pa + at, end_a - at * (int64_t)sizeof(T));
     }
-    if constexpr (FAST) ob.copy(lb, bt);
-    else ob.fetch(bt, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
+    if constexpr (FAST) ob.copy(lb, pb + bt, end_b - bt * (int64_t)sizeof(T));
+    else ob.fetch(pb + bt, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
   };
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
   constexpr int kAhead = (STAGES - 2) * (OpA::N + OpB::N);  // copies of later stages that may still be under way
@@ -381,7 +395,14 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     if constexpr (regs_a) oa.put(la);
     if constexpr (!FAST) ob.put(lb);
     // this wavefront's copies of this stage have landed, its reads and writes of LDS are done; then so are everybody's
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(FAST ? kAhead : 63) : "memory");
+    if constexpr (FAST) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
+      if (MODE != GROUPED_DW && c_end - c < KE && (c_end - c) % OpA::CE != 0) {
+        if constexpr (!regs_a) oa.trim(la, STAGES - 1);
+        ob.trim(lb, STAGES - 1);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     fetch(c + (STAGES - 1) * KE, next);  // past the end: zeros
@@ -491,33 +512,43 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   }
 }
 
-// d = dy where y is not <= 0, zero elsewhere: both products of a backward pass then load it like any other operand.
+// d = dy where y is not <= 0, zero elsewhere, in rows of whole chunks: both products of a backward pass then copy it.
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_mask_kernel(const T *dy, int64_t ld_dy, const T *y, int64_t ld_y, T *d, int64_t rows, int n) {
   constexpr int CE = 16 / sizeof(T);
-  const int chunks = n / CE;
+  using Op = GroupedOperand<T, 64, 8, 256, true, false>;
+  const int chunks = (n + CE - 1) / CE;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / chunks;
   if (row >= rows) return;
-  const int col = (int)(at % chunks) * CE;
-  using Op = GroupedOperand<T, 64, 8, 256, true, true>;
-  *reinterpret_cast<uint4 *>(d + row * n + col) = Op::keep(*reinterpret_cast<const uint4 *>(dy + row * ld_dy + col),
-                                                          *reinterpret_cast<const uint4 *>(y + row * ld_y + col));
+  const int col = (int)(at % chunks) * CE, valid = n - col < CE ? n - col : CE;
+  *reinterpret_cast<uint4 *>(d + at * CE) = Op::keep(Op::load(dy, row * ld_dy + col, valid), Op::load(y, row * ld_y + col, valid));
 }
 
-// dw over splits: the partial sums in split order, rounded once.
+// dw over splits: the partial sums of dweight (cw values) and dbias (cb) in split order, rounded once.
 template <typename T>
-__global__ __launch_bounds__(256) void grouped_join_kernel(const float *part, T *out, int64_t count, int splits) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256) void grouped_join_kernel(const float *part, T *out, int64_t cw, const float *part_bias, T *dbias,
+                                                           int64_t cb, int splits) {
+  const int64_t blocks = (cw + 1023) / 1024;
+  const bool bias = blockIdx.x >= blocks;
+  const int64_t count = bias ? cb : cw, i = (((int64_t)blockIdx.x - (bias ? blocks : 0)) * 256 + threadIdx.x) * 4;
   if (i >= count) return;
   const int valid = count - i >= 4 ? 4 : (int)(count - i);
+  const float *p = (bias ? part_bias : part) + i;
   f4v sum = {};
-  for (int s = 0; s < splits; ++s) {
-    const float *p = part + (int64_t)s * count + i;
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    f4v v[8] = {};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < valid) sum[e] += p[e];
+    for (int s = 0; s < 8; ++s) {
+      if (s0 + s >= splits) continue;
+      const float *q = p + (int64_t)(s0 + s) * count;
+      if (valid == 4) v[s] = __builtin_bit_cast(f4v, *reinterpret_cast<const Quad<float> *>(q));
+      else
+        for (int e = 0; e < valid; ++e) v[s][e] = q[e];
+    }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) sum += v[s];
   }
-  grouped_store4(out + i, sum, valid);
+  grouped_store4((bias ? dbias : out) + i, sum, valid);
 }
 
 }  // namespace mpe

@@ -264,6 +264,14 @@ def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(index, fn, *args):
+    """``fn(*args, stream)`` on the current stream of GPU ``index``, which is made current for the call."""
+    if torch.cuda.current_device() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with on_device(torch.device('cuda', index)):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 class on_device(object):
     """Makes ``device`` the current HIP device for the duration of a library call.  The C ABI launches on
     the current device (include/mpe_hip.h); a world / replay buffer / trainer created on ``cuda:1`` while

@@ -38,46 +38,63 @@ def group_ends(sizes, device='cuda'):
     return torch.tensor(ends, dtype=torch.int32, device=device)
 
 
-def _rows_of(t, name, shape=None, like=None):
-    """A 2-d tensor the kernels take: adjacent columns, rows that do not overlap (a copy if need be); its row stride."""
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError('%s: expected %s, got shape %s' % (name, 'a matrix' if shape is None else list(shape), list(t.shape)))
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError('%s is %s on %s, not %s on %s' % (name, t.dtype, t.device, like.dtype, like.device))
+def _rows_of(t):
+    """A matrix the kernels take -- adjacent columns, rows that do not overlap -- as it is or as a copy; its row stride."""
     rows, cols = t.shape
+    if t.is_contiguous():
+        return t, cols
     if not ((cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols)):
-        t = t.contiguous()
+        return t.contiguous(), cols
     return t, (cols if rows <= 1 else t.stride(0))
 
 
-def _check(x, weight, ends, bias=None):
-    if not (torch.is_tensor(x) and torch.is_tensor(weight) and torch.is_tensor(ends)):
-        raise TypeError('x, weight and ends are tensors')
+def _matrix(t, name, rows, cols, like):
+    """Checks an argument that belongs to ``like``'s rows."""
+    if not torch.is_tensor(t) or t.dtype is not like.dtype or t.get_device() != like.get_device():
+        raise ValueError('%s: expected %s on %s, got %s' % (name, like.dtype, like.device,
+                                                            '%s on %s' % (t.dtype, t.device) if torch.is_tensor(t) else type(t)))
+    if tuple(t.shape) != (rows, cols):
+        raise ValueError('%s: expected %s, got shape %s' % (name, [rows, cols], list(t.shape)))
+
+
+def _refuse(x, weight, ends, bias):
+    """Says what is wrong with arguments that ``_check`` does not take."""
+    if not (torch.is_tensor(x) and torch.is_tensor(weight) and torch.is_tensor(ends) and (bias is None or torch.is_tensor(bias))):
+        raise TypeError('x, weight, ends and bias are tensors')
     if x.device.type != 'cuda':
         raise RuntimeError('marl_amd.grouped works on GPU tensors (no CPU fallback)')
     if x.dtype not in _DTYPES:
         raise TypeError('marl_amd.grouped supports float32, bfloat16 and float16, got %r' % (x.dtype,))
     if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
         raise ValueError('x [rows, k] and weight [groups, n, k] do not fit: %s, %s' % (list(x.shape), list(weight.shape)))
-    g, n, k = weight.shape
     for t, name in ((weight, 'weight'), (bias, 'bias')):
         if t is not None and (t.dtype != x.dtype or t.device != x.device):
             raise ValueError('%s is %s on %s, not %s on %s' % (name, t.dtype, t.device, x.dtype, x.device))
+    g, n, k = weight.shape
     if bias is not None and tuple(bias.shape) != (g, n):
         raise ValueError('bias: expected %s, got shape %s' % ([g, n], list(bias.shape)))
     if not 1 <= g <= MAX_GROUPS or n < 1 or k < 1:
         raise ValueError('weight %s: 1 to %d groups of at least 1 x 1 are supported' % (list(weight.shape), MAX_GROUPS))
-    if x.shape[0] >= 1 << 31 or n * k >= 1 << 31:
-        raise ValueError('rows and n * k are below 2**31')
     if ends.dtype not in (torch.int32, torch.int64) or tuple(ends.shape) != (g,) or ends.device != x.device:
         raise ValueError('ends: expected int32 or int64 [%d] on %s, got %s %s on %s'
                          % (g, x.device, ends.dtype, list(ends.shape), ends.device))
+    raise ValueError('rows and n * k are below 2**31')
 
 
-def _desc(x, weight, ends):
-    g, n, k = weight.shape
-    return _hip.GroupedDesc(ends=ends.data_ptr(), rows=x.shape[0], groups=g, n=n, k=k, dtype=_DTYPES[x.dtype],
-                            ends64=ends.dtype == torch.int64)
+def _check(x, weight, ends, bias=None):
+    """The sizes' descriptor and the GPU's index; ``ends`` has to outlive the call."""
+    try:
+        (rows, k), (g, n, wk), (ge,) = x.shape, weight.shape, ends.shape
+        dtype, index, e64 = x.dtype, x.get_device(), ends.dtype is torch.int64
+        ok = (index >= 0 and dtype in _DTYPES and weight.dtype is dtype and weight.get_device() == index and wk == k and ge == g
+              and ends.get_device() == index and (e64 or ends.dtype is torch.int32) and 1 <= g <= MAX_GROUPS and n >= 1 and k >= 1
+              and rows < 1 << 31 and n * k < 1 << 31
+              and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == (g, n))))
+    except (ValueError, AttributeError, TypeError):
+        ok = False
+    if not ok:
+        _refuse(x, weight, ends, bias)
+    return _hip.GroupedDesc(ends.data_ptr(), rows, g, n, k, _DTYPES[dtype], e64, 0), index, rows, n, k
 
 
 def _overlap(a, b):
@@ -91,24 +108,26 @@ def _overlap(a, b):
 
 
 def _forward(x, weight, ends, bias, relu, out):
-    _check(x, weight, ends, bias)
-    x, ld_x = _rows_of(x, 'x')
-    weight, ends = weight.contiguous(), ends.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    rows, n = x.shape[0], weight.shape[1]
+    if torch.is_tensor(ends) and not ends.is_contiguous():
+        ends = ends.contiguous()
+    desc, index, rows, n, _ = _check(x, weight, ends, bias)
+    x, ld_x = _rows_of(x)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     own = out is None
     if own:
-        out, ld_y = torch.empty(rows, n, dtype=x.dtype, device=x.device), n
+        out, ld_y = x.new_empty((rows, n)), n
     else:
-        y, ld_y = _rows_of(out, 'out', (rows, n), x)
+        _matrix(out, 'out', rows, n, x)
+        y, ld_y = _rows_of(out)
         if y is not out:
             raise ValueError('out: its columns must be adjacent and its rows must not overlap')
         if any(_overlap(out, t) for t in (x, weight, bias, ends)):
             raise ValueError('out overlaps an input')
-    with _hip.on_device(x.device):
-        _hip.check(_hip.lib.mpe_grouped_linear(_desc(x, weight, ends), x.data_ptr(), ld_x, weight.data_ptr(), _hip.ptr(bias),
-                                               out.data_ptr(), ld_y, int(relu), int(own), _hip.stream_of(x.device)),
-                   'mpe_grouped_linear')
+    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear, desc, x.data_ptr(), ld_x, weight.data_ptr(),
+                           None if bias is None else bias.data_ptr(), out.data_ptr(), ld_y, relu, own), 'mpe_grouped_linear')
     return out
 
 
@@ -131,7 +150,7 @@ class _GroupedLinear(torch.autograd.Function):
 def grouped_linear(x, weight, ends, bias=None, relu=False, out=None):
     """``y[r] = act(x[r] @ weight[g].T + bias[g])`` for the rows ``r`` of every group ``g`` (module docstring).  Rows behind
     the last group: zeros, or with ``out`` (``[rows, n]``, adjacent columns, no overlap with an input) left as they were."""
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and any([torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias)]):
         if out is not None:
             raise RuntimeError('grouped_linear(out=...) does not support automatic differentiation')
         return _GroupedLinear.apply(x, weight, ends, bias, bool(relu))
@@ -143,28 +162,30 @@ def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dw
     """``(dx, dweight, dbias)`` of ``grouped_linear`` for the gradient ``grad`` ``[rows, n]`` of its result; ``y``: the
     result itself where it was made with ``relu=True`` (``grad`` counts where ``y`` is not <= 0).  An entry that is not needed
     is None.  ``dx`` is zero in rows of no group, ``dweight`` / ``dbias`` are zero for groups without rows."""
-    _check(x, weight, ends)
-    shape, want_dweight = (x.shape[0], weight.shape[1]), need_dweight
-    grad, ld_g = _rows_of(grad, 'grad', shape, x)
-    ld_y = 0
+    if torch.is_tensor(ends) and not ends.is_contiguous():
+        ends = ends.contiguous()
+    desc, index, rows, n, k = _check(x, weight, ends)
+    _matrix(grad, 'grad', rows, n, x)
+    grad, ld_g = _rows_of(grad)
+    ld_x = ld_y = 0
     if y is not None:
-        y, ld_y = _rows_of(y, 'y', shape, x)
-    ends = ends.contiguous()
-    need_dweight = need_dweight or need_dbias
-    desc, dx, dw, db = _desc(x, weight, ends), None, None, None
-    ld_x = 0
+        _matrix(y, 'y', rows, n, x)
+        y, ld_y = _rows_of(y)
+    both = need_dweight or need_dbias
+    dx = dw = db = ws = None
     if need_dx:
-        weight = weight.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if need_dweight:
-        x, ld_x = _rows_of(x, 'x')
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=x.device)
-        db = torch.empty(weight.shape[:2], dtype=x.dtype, device=x.device) if need_dbias else None
-    need = _hip.lib.mpe_grouped_backward_workspace(desc, y is not None, need_dweight)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        dx = x.new_empty((rows, k))
+    if both:
+        x, ld_x = _rows_of(x)
+        dw = x.new_empty(weight.shape)
+        db = x.new_empty(weight.shape[:2]) if need_dbias else None
+    need = _hip.lib.mpe_grouped_backward_workspace(desc, y is not None, both)
     _hip.check(min(need, 0), 'mpe_grouped_backward_workspace')
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with _hip.on_device(x.device):
-        _hip.check(_hip.lib.mpe_grouped_linear_backward(
-            desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, x.data_ptr(), ld_x, weight.data_ptr(), _hip.ptr(dx), x.shape[1], 1,
-            _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need, _hip.stream_of(x.device)), 'mpe_grouped_linear_backward')
-    return dx, dw if want_dweight else None, db
+    if need:
+        ws = x.new_empty((need + 3) // 4, dtype=torch.float32)
+    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear_backward, desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, x.data_ptr(),
+                           ld_x, weight.data_ptr(), _hip.ptr(dx), k, 1, _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need),
+               'mpe_grouped_linear_backward')
+    return dx, dw if need_dweight else None, db

@@ -36,9 +36,8 @@ def dequantize(codes, base, signed, dtype=torch.float32):
         raise TypeError('dequantize returns float32 or bfloat16, not %r' % (dtype,))
     codes, base = codes.contiguous(), base.contiguous()
     out = torch.empty(codes.numel(), dtype=dtype, device=codes.device)
-    with _hip.on_device(codes.device):
-        _hip.check(_hip.lib.mpe_adamw_moments(codes.data_ptr(), base.data_ptr(), out.data_ptr(), codes.numel(), int(signed),
-                                              _DTYPES[dtype], _hip.stream_of(codes.device)), 'mpe_adamw_moments')
+    _hip.check(_hip.launch(codes.get_device(), _hip.lib.mpe_adamw_moments, codes.data_ptr(), base.data_ptr(), out.data_ptr(),
+                           codes.numel(), int(signed), _DTYPES[dtype]), 'mpe_adamw_moments')
     return out
 
 
@@ -49,6 +48,7 @@ class _Plan(object):
         p0 = params[0]
         self.params, self.targets, self.bits = list(params), targets, state_bits
         self.device, self.dtype = p0.device, p0.dtype
+        self.written = self.params + (self.targets or [])
         self.counts = [p.numel() for p in self.params]
         self.first, total = [], 0
         for c in self.counts:                       # every variable starts at a multiple of BLOCK
@@ -78,8 +78,9 @@ class _Plan(object):
 
     def build(self):
         """The host table of pointers and its device plan."""
-        if not all(t.is_contiguous() for t in self.params + (self.targets or [])):
-            raise ValueError('AdamW: parameters and targets are contiguous')
+        for t in self.params + (self.targets or []):
+            if not t.is_contiguous() or t.dtype != self.dtype or t.device != self.device:
+                raise ValueError('AdamW: parameters and targets are contiguous and keep their type and device')
         n = len(self.params)
         self.table = (_hip.AdamTensor * n)()
         for j, p in enumerate(self.params):
@@ -93,13 +94,11 @@ class _Plan(object):
         blob = torch.empty(size, dtype=torch.uint8)
         _hip.check(min(_hip.lib.mpe_adamw_plan(n, self.table, code, self.bits, blob.data_ptr(), size), 0), 'mpe_adamw_plan')
         self.plan = blob.to(self.device)
+        self.plan_ptr = self.plan.data_ptr()
         self.ptrs = self.pointers()
 
     def pointers(self):
-        ptrs = [p.data_ptr() for p in self.params]
-        if self.targets is not None:
-            ptrs += [t.data_ptr() for t in self.targets]
-        return ptrs
+        return list(map(torch.Tensor.data_ptr, self.params if self.targets is None else self.params + self.targets))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -201,20 +200,19 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step ----------------------------------------------------------------------------------------------------------
     def _gradients(self, plan):
-        """Fills the plan's pointers; returns what must outlive the launch."""
-        keep, arr, dtype, device = [], plan.grads, plan.dtype, plan.device
-        for j, p in enumerate(plan.params):
-            g = p.grad
-            if g is None:
-                arr[j] = None
-                continue
-            if g.dtype != dtype or g.device != device or g.layout != torch.strided:
-                raise ValueError('AdamW: a gradient is %s on %s, its parameter %s on %s' % (g.dtype, g.device, dtype, device))
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            arr[j] = g.data_ptr()
-        return keep
+        """Fills the plan's pointers; returns what must outlive the launch.  (torch sees to it that a gradient has its
+        parameter's type, device and shape.)"""
+        grads = [p.grad for p in plan.params]
+        try:
+            plain = all(map(torch.Tensor.is_contiguous, grads))
+        except TypeError:                                         # a None
+            plain = False
+        if not plain:
+            grads = [None if g is None else g.contiguous() for g in grads]
+            plan.grads[:] = [None if g is None else g.data_ptr() for g in grads]
+        else:
+            plan.grads[:] = list(map(torch.Tensor.data_ptr, grads))
+        return grads
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -236,14 +234,13 @@ class AdamW(torch.optim.Optimizer):
                                  weight_decay=group['weight_decay'], max_norm=group['max_norm'] or 0.0, polyak=group['polyak'],
                                  step=group['step'] + 1, clock=_hip.ptr(clock), seed=self._seed, index0=index0,
                                  dtype=_DTYPES[plan.dtype], state_bits=self._bits)
-            with _hip.on_device(plan.device):
-                _hip.check(_hip.lib.mpe_adamw_step(args, len(plan.params), plan.table, plan.plan.data_ptr(), plan.grads,
-                                                   _hip.stream_of(plan.device)), 'mpe_adamw_step')
+            _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_step, args, len(plan.params), plan.table,
+                                   plan.plan_ptr, plan.grads), 'mpe_adamw_step')
             del keep
             if clock is None:
                 group['step'] += 1
             index0 += len(plan.params)
-            torch.autograd.graph.increment_version(plan.params + (plan.targets or []))
+            torch.autograd.graph.increment_version(plan.written)
         return loss
 
     # -- the moments -------------------------------------------------------------------------------------------------------

@@ -605,7 +605,8 @@ int mpe_grouped_linear_backward(const mpe_grouped_desc *desc, const void *dy, in
  *                    target moves).  step >= 1 counts this step, or clock (device, 32 bytes: int64 step, then 16 bytes that
  *                    the call writes) holds the steps taken so far and is moved on by one (for graph capture).
  *                    max_norm 0: no clip.  The plan holds the clip's scratch: steps on one plan must not overlap
- *   mpe_adamw_moments  byte codes of count (a multiple of 128) elements as the values they stand for (MPE_F32 / MPE_BF16)
+ *   mpe_adamw_moments  the byte codes of count (a multiple of 128) elements as the values they stand for (MPE_F32 / MPE_BF16);
+ *                    out NULL or out_sq NULL: not that one
  */
 typedef struct mpe_adamw_tensor {
   void *param, *target, *exp_avg, *exp_avg_base, *exp_avg_sq, *exp_avg_sq_base;
@@ -622,8 +623,8 @@ typedef struct mpe_adamw_args {
 int64_t mpe_adamw_plan(int n, const mpe_adamw_tensor *tensors, int dtype, int state_bits, void *blob, int64_t blob_bytes);
 int mpe_adamw_step(const mpe_adamw_args *args, int n, const mpe_adamw_tensor *tensors, const void *plan,
                    const void *const *grads, void *stream);
-int mpe_adamw_moments(const void *codes, const void *base, void *out, int64_t count, int is_signed, int dtype,
-                      void *stream);
+int mpe_adamw_moments(const void *exp_avg, const void *exp_avg_base, const void *exp_avg_sq, const void *exp_avg_sq_base,
+                      void *out, void *out_sq, int64_t count, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

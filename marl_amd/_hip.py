@@ -213,8 +213,8 @@ def _load():
     L.mpe_adamw_plan.argtypes = [ci, ap, ci, ci, vp, i64]
     L.mpe_adamw_step.restype = ci                 # args, n, tensors (host), plan (device), grads (host array), stream
     L.mpe_adamw_step.argtypes = [C.POINTER(AdamArgs), ci, ap, vp, C.POINTER(vp), vp]
-    L.mpe_adamw_moments.restype = ci              # codes, base, out, count, is_signed, dtype, stream
-    L.mpe_adamw_moments.argtypes = [vp, vp, vp, i64, ci, ci, vp]
+    L.mpe_adamw_moments.restype = ci              # exp_avg, its base, exp_avg_sq, its base, out, out_sq, count, dtype, stream
+    L.mpe_adamw_moments.argtypes = [vp, vp, vp, vp, vp, vp, i64, ci, vp]
     L.mpe_stats_rows.restype = i64
     L.mpe_stats_rows.argtypes = [dp, i64, ci, u32]
     L.mpe_stats_reduce.restype = ci

@@ -142,20 +142,24 @@ extern "C" int mpe_adamw_step(const mpe_adamw_args *h, int n, const mpe_adamw_te
   return MPE_OK;
 }
 
-extern "C" int mpe_adamw_moments(const void *codes, const void *base, void *out, int64_t count, int is_signed, int dtype,
-                                 void *stream) {
-  if (count < 0 || count % kAdamBlock != 0 || (is_signed != 0 && is_signed != 1)) return MPE_ERR_ARG;
+extern "C" int mpe_adamw_moments(const void *exp_avg, const void *exp_avg_base, const void *exp_avg_sq, const void *exp_avg_sq_base,
+                                 void *out, void *out_sq, int64_t count, int dtype, void *stream) {
+  if (count < 0 || count % kAdamBlock != 0) return MPE_ERR_ARG;
   if (dtype != MPE_F32 && dtype != MPE_BF16) return MPE_ERR_UNSUPPORTED;
   if (count == 0) return MPE_OK;
-  if (!codes || !base || !out) return MPE_ERR_NULL;
-  if (bad_align(codes, 8) || bad_align(base, 2) || bad_align(out, dtype == MPE_F32 ? 4 : 2)) return MPE_ERR_ALIGN;
+  if ((!out && !out_sq) || (out && (!exp_avg || !exp_avg_base)) || (out_sq && (!exp_avg_sq || !exp_avg_sq_base))) return MPE_ERR_NULL;
+  const int size = dtype == MPE_F32 ? 4 : 2;
+  if (bad_align(exp_avg, 8) || bad_align(exp_avg_sq, 8) || bad_align(exp_avg_base, 2) || bad_align(exp_avg_sq_base, 2) ||
+      bad_align(out, size) || bad_align(out_sq, size))
+    return MPE_ERR_ALIGN;
   const int64_t grid = (count / 8 + 255) / 256;
   if (grid > 0x7fffffff) return MPE_ERR_ARG;
+  const AdamMoments a = {{out ? (const uint8_t *)exp_avg : nullptr, out_sq ? (const uint8_t *)exp_avg_sq : nullptr},
+                         {(const int16_t *)exp_avg_base, (const int16_t *)exp_avg_sq_base},
+                         {out, out_sq}};
   if (dtype == MPE_F32)
-    hipLaunchKernelGGL(adamw_moments_kernel<float>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,
-                       (const uint8_t *)codes, (const int16_t *)base, (float *)out, count, is_signed);
+    hipLaunchKernelGGL(adamw_moments_kernel<float>, dim3((unsigned)grid, out_sq ? 2 : 1), dim3(256), 0, (hipStream_t)stream, a, count);
   else
-    hipLaunchKernelGGL(adamw_moments_kernel<__bf16>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream,
-                       (const uint8_t *)codes, (const int16_t *)base, (__bf16 *)out, count, is_signed);
+    hipLaunchKernelGGL(adamw_moments_kernel<__bf16>, dim3((unsigned)grid, out_sq ? 2 : 1), dim3(256), 0, (hipStream_t)stream, a, count);
   return (int)hipGetLastError();
 }

@@ -23,7 +23,7 @@ namespace mpe {
 constexpr int kAdamBlock = 128;    // elements that share a base
 constexpr int kAdamItem = 8192;    // elements of a work item (one workgroup)
 constexpr int kAdamThreads = 256;
-constexpr int kAdamMaxGrads = 256; // gradients (pointers in the kernel's arguments) per launch
+constexpr int kAdamMaxGrads = 448; // gradients (pointers in the kernel's arguments, which end at 4 KiB) per launch
 
 struct AdamTensor {
   void *param, *target, *exp_avg, *exp_avg_base, *exp_avg_sq, *exp_avg_sq_base;
@@ -44,6 +44,7 @@ struct AdamArgs {
   uint32_t index0;                    // the first tensor's number in the random streams
   const void *grads[kAdamMaxGrads];
 };
+static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; };
@@ -131,15 +132,21 @@ __device__ __forceinline__ double adam_block_sum(double s) {
   return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+// Sum of squares of [begin, end), at most an item, over the workgroup's threads: every load first, then the sums.
 template <typename T>
 __device__ __forceinline__ double adam_squares(const T *g, int64_t begin, int64_t end) {
-  double s = 0.0;
-  for (int64_t i = begin + 8 * threadIdx.x; i < end; i += 8 * kAdamThreads) {
-    float x[8];
-    adam_load8(g + i, end - i < 8 ? (int)(end - i) : 8, x);
+  constexpr int kRounds = kAdamItem / (8 * kAdamThreads);
+  float x[kRounds][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = __builtin_fma((double)x[e], (double)x[e], s);
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = begin + 8 * (threadIdx.x + r * kAdamThreads);
+    adam_load8(g + i, end - i >= 8 ? 8 : (end > i ? (int)(end - i) : 0), x[r]);
   }
+  double s = 0.0;
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fma((double)x[r][e], (double)x[r][e], s);
   return s;
 }
 
@@ -204,7 +211,11 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamArgs a) {
         const float gc = CLIP ? d[e] * scale : d[e];
         m[e] = m[e] * a.beta1 + gc * a.beta1c;
         v[e] = v[e] * a.beta2 + (gc * gc) * a.beta2c;
-        x[e] = x[e] * s.decay - (m[e] / (sqrtf(v[e]) * s.root + a.eps)) * s.step_size;
+        // 8 bits: 10 bytes a value leave ~90 vector instructions at the memory's rate, and correctly rounded roots and
+        // quotients take 20 of them: the 1-ulp instructions there (302 M values bf16: 723 -> 600 us)
+        const float q = EIGHT ? m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.root + a.eps)
+                              : m[e] / (sqrtf(v[e]) * s.root + a.eps);
+        x[e] = x[e] * s.decay - q * s.step_size;
         held[e] = (T)x[e];
         if (e >= valid) m[e] = v[e] = 0.0f;  // nothing behind the variable's end reaches its block
       }
@@ -252,22 +263,24 @@ __global__ void adamw_clock_kernel(AdamClock *c, double lr, double beta1, double
   c->s.key = adam_step_key(seed, t);
 }
 
-// 8-bit moments as the values they stand for (four significant bits: exact in T = f32 or bf16)
+// 8-bit moments as the values they stand for (four significant bits: exact in T = f32 or bf16); blockIdx.y: first, second
+struct AdamMoments { const uint8_t *codes[2]; const int16_t *base[2]; void *out[2]; };
 template <typename T>
-__global__ __launch_bounds__(256) void adamw_moments_kernel(const uint8_t *codes, const int16_t *base, T *out, int64_t count,
-                                                            int is_signed) {
+__global__ __launch_bounds__(256) void adamw_moments_kernel(AdamMoments a, int64_t count) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= count) return;
+  const bool first = blockIdx.y == 0;
+  const uint8_t *codes = first ? a.codes[0] : a.codes[1];
+  if (i >= count || codes == nullptr) return;
   const uint2 c = *reinterpret_cast<const uint2 *>(codes + i);
-  const uint32_t b = (uint16_t)base[i / kAdamBlock];
+  const uint32_t b = (uint16_t)(first ? a.base[0] : a.base[1])[i / kAdamBlock];
   T v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const uint32_t w = ((e < 4 ? c.x : c.y) >> (8 * (e & 3))) & 255u;
-    const float x = is_signed ? __uint_as_float(__float_as_uint(adam_decode(w & 127u, b)) | (w >> 7) << 31) : adam_decode(w, b);
+    const float x = first ? __uint_as_float(__float_as_uint(adam_decode(w & 127u, b)) | (w >> 7) << 31) : adam_decode(w, b);
     v[e] = (T)x;
   }
-  adam_store8(out + i, 8, v);
+  adam_store8(static_cast<T *>(first ? a.out[0] : a.out[1]) + i, 8, v);
 }
 
 }  // namespace mpe

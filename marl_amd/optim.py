@@ -36,8 +36,10 @@ def dequantize(codes, base, signed, dtype=torch.float32):
         raise TypeError('dequantize returns float32 or bfloat16, not %r' % (dtype,))
     codes, base = codes.contiguous(), base.contiguous()
     out = torch.empty(codes.numel(), dtype=dtype, device=codes.device)
-    _hip.check(_hip.launch(codes.get_device(), _hip.lib.mpe_adamw_moments, codes.data_ptr(), base.data_ptr(), out.data_ptr(),
-                           codes.numel(), int(signed), _DTYPES[dtype]), 'mpe_adamw_moments')
+    pair, none = (codes.data_ptr(), base.data_ptr()), (None, None)
+    _hip.check(_hip.launch(codes.get_device(), _hip.lib.mpe_adamw_moments, *(pair + none if signed else none + pair),
+                           *((out.data_ptr(), None) if signed else (None, out.data_ptr())), codes.numel(), _DTYPES[dtype]),
+               'mpe_adamw_moments')
     return out
 
 
@@ -256,8 +258,17 @@ class AdamW(torch.optim.Optimizer):
             if dtype != torch.float32:
                 raise TypeError('32-bit moments are float32')
             return [(plan.flat['exp_avg'], plan.flat['exp_avg_sq']) for plan in self._plans]
-        return [(dequantize(plan.flat['exp_avg'], plan.flat['exp_avg_base'], True, dtype),
-                 dequantize(plan.flat['exp_avg_sq'], plan.flat['exp_avg_sq_base'], False, dtype)) for plan in self._plans]
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError('8-bit moments are given in float32 or bfloat16, not %r' % (dtype,))
+        out = []
+        for plan in self._plans:
+            f = plan.flat
+            m, v = torch.empty_like(f['exp_avg'], dtype=dtype), torch.empty_like(f['exp_avg_sq'], dtype=dtype)
+            _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_moments, f['exp_avg'].data_ptr(),
+                                   f['exp_avg_base'].data_ptr(), f['exp_avg_sq'].data_ptr(), f['exp_avg_sq_base'].data_ptr(),
+                                   m.data_ptr(), v.data_ptr(), m.numel(), _DTYPES[dtype]), 'mpe_adamw_moments')
+            out.append((m, v))
+        return out
 
     def state_dict(self):
         for i in range(len(self._plans)):

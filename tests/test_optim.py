@@ -66,11 +66,13 @@ def test_c_abi_refuses_bad_arguments():
     blob = torch.empty(need, dtype=torch.uint8)
     assert need > 0 and L.mpe_adamw_plan(1, _table(), _hip.F32, 32, blob.data_ptr(), need) == need
     assert L.mpe_adamw_plan(1, _table(), _hip.F32, 32, blob.data_ptr(), need - 1) == -7
-    for bad in ((p, p, p, 100, 1, 0), (p, p, p, 128, 2, 0), (p, p, p, -128, 1, 0)):
-        assert L.mpe_adamw_moments(*bad, None) == -6
-    assert L.mpe_adamw_moments(p, p, p, 128, 1, 2, None) == -5
-    assert L.mpe_adamw_moments(None, p, p, 128, 1, 0, None) == -1
-    assert L.mpe_adamw_moments(p + 4, p, p, 128, 1, 0, None) == -4
+    for count in (100, -128):
+        assert L.mpe_adamw_moments(p, p, p, p, p, p, count, 0, None) == -6
+    assert L.mpe_adamw_moments(p, p, p, p, p, p, 128, 2, None) == -5
+    for bad in ((None, p, p, p, p, p), (p, None, p, p, p, p), (p, p, None, p, p, p), (p, p, p, None, p, p), (p, p, p, p, None, None)):
+        assert L.mpe_adamw_moments(*bad, 128, 0, None) == -1
+    for bad in ((p + 4, p, p, p, p, p), (p, p + 1, p, p, p, p), (p, p, p + 4, p, p, p), (p, p, p, p, p + 2, p), (p, p, p, p, p, p + 1)):
+        assert L.mpe_adamw_moments(*bad, 128, 0, None) == -4
     assert C.sizeof(_hip.AdamTensor) == 56 and C.sizeof(_hip.AdamArgs) == 96
 
 
@@ -239,8 +241,8 @@ def test_one_step_matches_torch_adam_at_zero_decay():
 
 @pytest.mark.gpu
 def test_more_tensors_than_one_launch_holds_and_missing_gradients():
-    """600 variables (three launches), every third without a gradient: value and moments stay, the target still follows."""
-    sizes = [(1 + (i * 37) % 300,) for i in range(599)] + [(20000,)]
+    """1 000 variables (three launches), every third without a gradient: value and moments stay, the target still follows."""
+    sizes = [(1 + (i * 37) % 300,) for i in range(999)] + [(20000,)]
     ps, ts = _tensors(sizes, torch.float32, 1), _tensors(sizes, torch.float32, 2)
     gs = _tensors(sizes, torch.float32, 3)
     p0, t0 = [p.clone() for p in ps], [t.clone() for t in ts]
@@ -279,6 +281,9 @@ def test_eight_bit_moments_are_right_on_average():
     assert abs(float((hm.double() - m).mean())) < 10 * 0.125 * float(m.abs().mean()) * math.sqrt(5.3) / 128
     assert float((hm.double() - m).abs().mean()) < 0.3 * float(m.abs().mean())
     assert torch.equal(opt.moments(torch.bfloat16)[0][0].float(), hm)     # bfloat16 holds the values
+    flat = opt.buffers()[0]
+    assert torch.equal(optim.dequantize(flat['exp_avg'], flat['exp_avg_base'], True), hm)
+    assert torch.equal(optim.dequantize(flat['exp_avg_sq'], flat['exp_avg_sq_base'], False, torch.bfloat16).float(), hv)
 
 
 @pytest.mark.gpu

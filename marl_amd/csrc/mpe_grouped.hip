@@ -5,32 +5,12 @@
 #include "mpe_grouped_kernel.h"
 
 using namespace mpe;
-#ifndef MKC
-#define MKC 4
-#define MST 4
-#endif
-#ifndef SKC
-#define SKC 8
-#define SST 2
-#endif
-#ifndef MASKSH
-#define MASKSH 18
-#endif
-#ifndef LBN
-#define LBN 256
-#define LWM 2
-#define LWN 4
-#define LKC 4
-#define LST 4
-#endif
-#ifndef LARGE_MEAN
-#define LARGE_MEAN 384
-#endif
 
 namespace {
 
-constexpr int kMaxGroups = 1024;
+constexpr int kMaxGroups = 1024, kMaxWidth = 1 << 20;
 constexpr int64_t kMaxGrid = 0x7fffffff;
+static_assert((int64_t)kMaxWidth * 4 * 256 < (int64_t)kGroupedSpan, "a tile of packed rows spans less than a copy may reach");
 
 int dtype_size(int dtype) { return dtype == MPE_F32 ? 4 : 2; }
 bool bad_align(const void *p, int size) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; }
@@ -39,39 +19,135 @@ int grouped_check(const mpe_grouped_desc *d) {
   if (!d || !d->ends) return MPE_ERR_NULL;
   if (d->dtype != MPE_F32 && d->dtype != MPE_BF16 && d->dtype != MPE_F16) return MPE_ERR_UNSUPPORTED;
   if (d->groups < 1 || d->groups > kMaxGroups || d->n < 1 || d->k < 1 || d->rows < 0 || d->rows > INT32_MAX) return MPE_ERR_ARG;
-  if ((int64_t)d->n * d->k > INT32_MAX) return MPE_ERR_ARG;
+  if (d->n > kMaxWidth || d->k > kMaxWidth || (int64_t)d->n * d->k > INT32_MAX) return MPE_ERR_ARG;
   if (d->ends64 != 0 && d->ends64 != 1) return MPE_ERR_ARG;
   if (bad_align(d->ends, d->ends64 ? 8 : 4)) return MPE_ERR_ALIGN;
   return MPE_OK;
 }
 
+// ---- what the tiles are copied from --------------------------------------------------------------------------------------
+// A matrix of the call, and whether it is packed into the workspace first: a tile (256 lines) of it would span too much, or it
+// is masked (written once, read by both products: 4 096 x 64 f32 backward
+// 17.1 -> 15.7 us, 16 384 x 512 238 -> 165 us against a mask in the tiles' loads).
+struct Matrix {
+  const void *p, *mask;
+  int64_t ld, ld_mask, lines, at;  // at: offset in the workspace, or -1
+  int cols;
+};
+
+struct Workspace {
+  int size;  // of an element
+  int64_t total = 0;
+  GroupedPacks packs{};
+  int jobs = 0;
+  int64_t blocks = 0;
+
+  int chunk() const { return 16 / size; }
+  int64_t packed_ld(const Matrix &m) const { return (m.cols + chunk() - 1) / chunk() * chunk(); }
+  bool copyable(const Matrix &m) const {
+    return m.ld < (int64_t)kGroupedSpan / (256 * size) - 16;
+  }
+  int64_t take(int64_t bytes) {
+    const int64_t at = total;
+    total += (bytes + 15) / 16 * 16;
+    return at;
+  }
+  void plan(Matrix &m) { m.at = m.lines > 0 && (m.mask || !copyable(m)) ? take(m.lines * packed_ld(m) * size) : -1; }
+  // after the plan: the matrix as the kernels read it
+  void place(Matrix &m, void *base) {
+    if (m.at < 0) return;
+    GroupedPack &j = packs.job[jobs++];
+    const int64_t chunks = packed_ld(m) / chunk();  // of a line; workgroups as grouped_pack_kernel counts them
+    const int64_t many = chunks <= 256 ? (m.lines + 256 / chunks - 1) / (256 / chunks) : m.lines * ((chunks + 255) / 256);
+    j = GroupedPack{m.p, m.mask, (char *)base + m.at, m.ld, m.ld_mask, m.lines, m.cols, (int)(many < kMaxGrid ? many : kMaxGrid)};
+    blocks += many;
+    m.p = j.dst;
+    m.ld = packed_ld(m);
+  }
+  int run(int dtype, hipStream_t s) {
+    if (jobs == 0) return MPE_OK;
+    if (blocks > kMaxGrid) return MPE_ERR_ARG;
+    const dim3 grid((unsigned)blocks), block(256);
+    if (dtype == MPE_F32) hipLaunchKernelGGL(grouped_pack_kernel<float>, grid, block, 0, s, packs);
+    else if (dtype == MPE_BF16) hipLaunchKernelGGL(grouped_pack_kernel<__bf16>, grid, block, 0, s, packs);
+    else hipLaunchKernelGGL(grouped_pack_kernel<_Float16>, grid, block, 0, s, packs);
+    return (int)hipGetLastError();
+  }
+};
+
+// ---- tiles ---------------------------------------------------------------------------------------------------------------
 // Tiles (rows x columns of the output, wavefronts): small 64 x 64 (2 x 2), middle 128 x 128 (2 x 2), large 256 x 256 (2 x 4).
 enum Tile { SMALL = 0, MIDDLE = 1, LARGE = 2 };
-constexpr int kTile[3] = {64, 128, 256}, kTileJ[3] = {64, 128, LBN};
+constexpr int kTile[3] = {64, 128, 256};
 
-// A 16-bit product is bound by what the tile reads from LDS per matrix instruction: the largest tile that still leaves every
-// CU a workgroup and does not mostly overhang its group's rows.  f32 matrix instructions are 16 times slower: small tiles.
-Tile pick_tile(int dtype, bool fast, int64_t mean_rows, int64_t cols, int64_t groups_rows, int64_t others) {
-  if (dtype == MPE_F32) return SMALL;
-  const auto tiles = [&](int64_t t) { return (groups_rows + t - 1) / t * ((cols + t - 1) / t) * others; };
-  if (fast && mean_rows >= LARGE_MEAN && cols >= 256 && tiles(256) >= 256) return LARGE;
+// A 16-bit product is bound by what the tiles read per matrix instruction: the largest tile that still leaves every CU a
+// workgroup and does not mostly overhang its group's rows.  f32 matrix instructions are 16 times slower: small tiles.
+// mean_rows: of a group; rows: of all; others: independent products.  The large tile has no registers for n or k that end
+// inside a chunk (with them 32 768 rows 4 096 -> 2 048 take 679 us instead of 510).
+Tile pick_tile(const mpe_grouped_desc *d, int64_t mean_rows, int64_t cols, int64_t rows, int64_t others) {
+  if (d->dtype == MPE_F32) return SMALL;
+  const auto tiles = [&](int64_t t) { return (rows + t - 1) / t * ((cols + t - 1) / t) * others; };
+  if (mean_rows >= 384 && cols >= 256 && tiles(256) >= 256 && d->n % 8 == 0 && d->k % 8 == 0) return LARGE;
   if (mean_rows >= 96 && cols >= 96 && tiles(128) >= 256) return MIDDLE;
   return SMALL;
 }
 
 // dweight: rows and columns of the output are n and k, the contraction runs over the group's rows.
-Tile dw_tile(const mpe_grouped_desc *d, bool fast) { return pick_tile(d->dtype, fast, d->n, d->k, d->n, d->groups); }
-int64_t dw_tiles(const mpe_grouped_desc *d, Tile t) {
-  return (int64_t)((d->n + kTile[t] - 1) / kTile[t]) * ((d->k + kTileJ[t] - 1) / kTileJ[t]);
+Tile dw_tile(const mpe_grouped_desc *d) { return pick_tile(d, d->n, d->k, d->n, d->groups); }
+int64_t dw_tiles(const mpe_grouped_desc *d) {
+  const int t = kTile[dw_tile(d)];
+  return (int64_t)((d->n + t - 1) / t) * ((d->k + t - 1) / t) * d->groups;
 }
-// Where the outputs are too few tiles to fill the chip, each group's rows are split; goes by sizes alone (the workspace is
-// made before the call).  Enough tiles for the large one are enough not to split.
+// Where the outputs are too few tiles to fill the chip (two workgroups a CU; of large tiles, which one fills, they are
+// enough by pick_tile's rule), each group's rows are split.
 int dw_splits(const mpe_grouped_desc *d) {
-  const int64_t tiles = dw_tiles(d, dw_tile(d, false)) * d->groups, mean = d->rows / d->groups;
+  const int64_t tiles = dw_tiles(d), mean = d->rows / d->groups;
   int s = 1;
-  while (s < 64 && tiles * s < 512 && mean / (s * 2) >= 64) s *= 2;
+  if (dw_tile(d) != LARGE)
+    while (s < 64 && tiles * s < 512 && mean / (s * 2) >= 64) s *= 2;
   return s;
 }
+
+// ---- launches ------------------------------------------------------------------------------------------------------------
+template <typename T, int MODE>
+int launch(const GroupedArgs &a, Tile tile, int64_t grid, hipStream_t s) {
+  if (grid > kMaxGrid) return MPE_ERR_ARG;
+  const dim3 blocks((unsigned)grid);
+  if (sizeof(T) == 2 && tile == LARGE) {
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, MODE, 256, 256, 2, 4, 4, 4>), blocks, dim3(512), 0, s, a);
+  } else if (sizeof(T) == 2 && tile == MIDDLE) {
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, MODE, 128, 128, 2, 2, 4, 4>), blocks, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((grouped_kernel<T, MODE, 64, 64, 2, 2, 8, 2>), blocks, dim3(256), 0, s, a);
+  }
+  return (int)hipGetLastError();
+}
+
+template <typename T, int MODE>
+int launch_rows(GroupedArgs a, const mpe_grouped_desc *d, hipStream_t s) {
+  const int64_t cols = MODE == GROUPED_FWD ? d->n : d->k;
+  const Tile tile = pick_tile(d, d->rows / d->groups, cols, d->rows, 1);
+  a.tiles_j = (int)((cols + kTile[tile] - 1) / kTile[tile]);
+  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;  // groups (and the tail) with rows: each may add a partial tile
+  return launch<T, MODE>(a, tile, (a.rows / kTile[tile] + most) * a.tiles_j, s);
+}
+
+template <typename T>
+int launch_dw(GroupedArgs a, const mpe_grouped_desc *d, hipStream_t s) {
+  const Tile tile = dw_tile(d);
+  a.tiles_i = (d->n + kTile[tile] - 1) / kTile[tile];
+  a.tiles_j = (d->k + kTile[tile] - 1) / kTile[tile];
+  a.splits = dw_splits(d);
+  const int rc = launch<T, GROUPED_DW>(a, tile, dw_tiles(d) * a.splits, s);
+  if (rc || a.splits == 1) return rc;
+  const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = a.dbias ? (int64_t)a.groups * a.n : 0;
+  hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024 + (cb + 1023) / 1024)), dim3(256), 0, s, a.part,
+                     (T *)a.out, cw, a.part_bias, (T *)a.dbias, cb, a.splits);
+  return (int)hipGetLastError();
+}
+
+#define GROUPED_BY_TYPE(dtype, F, ...) \
+  ((dtype) == MPE_F32 ? F<float __VA_ARGS__ : (dtype) == MPE_BF16 ? F<__bf16 __VA_ARGS__ : F<_Float16 __VA_ARGS__)
 
 GroupedArgs base_args(const mpe_grouped_desc *d) {
   GroupedArgs a{};
@@ -85,69 +161,51 @@ GroupedArgs base_args(const mpe_grouped_desc *d) {
   return a;
 }
 
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int PATH, int KC, int STAGES>
-int launch_tile(const GroupedArgs &a, int64_t grid, hipStream_t s) {
-  if (grid > kMaxGrid) return MPE_ERR_ARG;
-  hipLaunchKernelGGL((grouped_kernel<T, MODE, BM, BN, WM, WN, PATH, KC, STAGES>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, a);
-  return (int)hipGetLastError();
-}
+Matrix rows_of(const mpe_grouped_desc *d, const void *p, int64_t ld, int cols) { return Matrix{p, nullptr, ld, 0, d->rows, -1, cols}; }
+Matrix weight_of(const mpe_grouped_desc *d, const void *p) { return Matrix{p, nullptr, d->k, 0, (int64_t)d->groups * d->n, -1, d->k}; }
 
-template <typename T, int MODE, int PATH>
-int launch_as(const GroupedArgs &a, Tile tile, int64_t grid, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (PATH == GROUPED_FAST)
-      if (tile == LARGE) return launch_tile<T, MODE, 256, LBN, LWM, LWN, PATH, LKC, LST>(a, grid, s);
-    if (tile != SMALL) return launch_tile<T, MODE, 128, 128, 2, 2, PATH, PATH == GROUPED_FAST ? MKC : 8, PATH == GROUPED_FAST ? MST : 2>(a, grid, s);
+struct Forward {
+  Matrix x, w;
+  Workspace ws;
+  Forward(const mpe_grouped_desc *d, const void *px, int64_t ld_x, const void *pw)
+      : x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)} {
+    ws.plan(x);
+    ws.plan(w);
   }
-  return launch_tile<T, MODE, 64, 64, 2, 2, PATH, PATH == GROUPED_FAST ? SKC : 8, PATH == GROUPED_FAST ? SST : 2>(a, grid, s);
-}
+};
 
-template <typename T, int MODE>
-int launch(const GroupedArgs &a, bool fast, Tile tile, int64_t grid, hipStream_t s) {
-  if (!fast) return launch_as<T, MODE, GROUPED_ANY>(a, tile, grid, s);
-  if constexpr (MODE != GROUPED_FWD)
-    if (a.mask) return launch_as<T, MODE, GROUPED_FAST_MASK>(a, tile, grid, s);
-  return launch_as<T, MODE, GROUPED_FAST>(a, tile, grid, s);
-}
-
-template <typename T, int MODE>
-int launch_rows(GroupedArgs a, bool fast, int dtype, int cols, hipStream_t s) {
-  const Tile tile = pick_tile(dtype, fast && !a.mask, a.rows / a.groups, cols, a.rows, 1);
-  a.tiles_j = (cols + kTileJ[tile] - 1) / kTileJ[tile];
-  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;  // groups (and the tail) with rows: each may add a partial tile
-  return launch<T, MODE>(a, fast, tile, (a.rows / kTile[tile] + most) * a.tiles_j, s);
-}
-
-template <typename T>
-int launch_dw(GroupedArgs a, const mpe_grouped_desc *d, bool fast, hipStream_t s) {
-  const Tile tile = dw_tile(d, fast && !a.mask);
-  a.tiles_i = (d->n + kTile[tile] - 1) / kTile[tile];
-  a.tiles_j = (d->k + kTileJ[tile] - 1) / kTileJ[tile];
-  a.splits = dw_splits(d);
-  const int rc = launch<T, GROUPED_DW>(a, fast, tile, dw_tiles(d, tile) * a.splits * a.groups, s);
-  if (rc || a.splits == 1) return rc;
-  const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = a.dbias ? (int64_t)a.groups * a.n : 0;
-  hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024 + (cb + 1023) / 1024)), dim3(256), 0, s, a.part,
-                     (T *)a.out, cw, a.part_bias, (T *)a.dbias, cb, a.splits);
-  return (int)hipGetLastError();
-}
-
-// An array that tiles may be copied from: dwords stay dwords from row to row, a tile (256 lines) spans less than kGroupedSpan
-bool copyable(const void *p, int64_t ld, int size) {
-  return (reinterpret_cast<uintptr_t>(p) & 3) == 0 && ld * size % 4 == 0 && ld < (int64_t)kGroupedSpan / (256 * size) - 16;
-}
-
-template <int MODE>
-int launch_type(const GroupedArgs &a, int dtype, bool fast, int cols, hipStream_t s) {
-  return dtype == MPE_F32    ? launch_rows<float, MODE>(a, fast, dtype, cols, s)
-         : dtype == MPE_BF16 ? launch_rows<__bf16, MODE>(a, fast, dtype, cols, s)
-                             : launch_rows<_Float16, MODE>(a, fast, dtype, cols, s);
-}
+// The gradient of the result, the operands that are wanted, and the partial sums of dweight and dbias.
+struct Backward {
+  Matrix d_, x, w;
+  Workspace ws;
+  int64_t part = 0, part_bias = 0;
+  Backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, const void *px, int64_t ld_x,
+           const void *pw, bool dx, bool dw)
+      : d_(rows_of(d, dy, ld_dy, d->n)), x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)} {
+    d_.mask = y;
+    d_.ld_mask = ld_y;
+    if (dx || dw) ws.plan(d_);
+    if (dw) ws.plan(x);
+    if (dx) ws.plan(w);
+    const int splits = dw_splits(d);
+    if (dw && splits > 1) {
+      const int64_t one = (int64_t)splits * d->groups * d->n * 4;
+      part = ws.take(one * d->k);
+      part_bias = ws.take(one);
+    }
+  }
+};
 
 }  // namespace
 
+extern "C" int64_t mpe_grouped_linear_workspace(const mpe_grouped_desc *d, const void *x, int64_t ld_x, const void *weight) {
+  if (const int rc = grouped_check(d)) return rc;
+  return Forward(d, x, ld_x, weight).ws.total;
+}
+
 extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int64_t ld_x, const void *weight, const void *bias,
-                                  void *y, int64_t ld_y, int relu, int zero_tail, void *stream) {
+                                  void *y, int64_t ld_y, int relu, int zero_tail, void *workspace, int64_t workspace_bytes,
+                                  void *stream) {
   if (const int rc = grouped_check(d)) return rc;
   if (relu != 0 && relu != 1) return MPE_ERR_ARG;
   if (zero_tail != 0 && zero_tail != 1) return MPE_ERR_ARG;
@@ -155,59 +213,34 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
   if (!x || !weight || !y) return MPE_ERR_NULL;
   if (ld_x < d->k || ld_y < d->n) return MPE_ERR_ARG;
   const int size = dtype_size(d->dtype);
-  if (bad_align(x, size) || bad_align(weight, size) || bad_align(bias, size) || bad_align(y, size)) return MPE_ERR_ALIGN;
+  for (const void *p : {x, weight, bias, (const void *)y})
+    if (bad_align(p, size)) return MPE_ERR_ALIGN;
+  if (bad_align(workspace, 16)) return MPE_ERR_ALIGN;
+  Forward f(d, x, ld_x, weight);
+  if (f.ws.total > 0 && !workspace) return MPE_ERR_NULL;
+  if (workspace_bytes < f.ws.total) return MPE_ERR_SCRATCH;
+  hipStream_t s = (hipStream_t)stream;
+  f.ws.place(f.x, workspace);
+  f.ws.place(f.w, workspace);
+  if (const int rc = f.ws.run(d->dtype, s)) return rc;
   GroupedArgs a = base_args(d);
-  a.a = x;
-  a.ld_a = ld_x;
-  a.b = weight;
-  a.ld_b = d->k;
+  a.a = f.x.p;
+  a.ld_a = f.x.ld;
+  a.b = f.w.p;
+  a.ld_b = f.w.ld;
   a.bias = bias;
   a.out = y;
   a.ld_out = ld_y;
   a.relu = relu;
   a.zero_tail = zero_tail;
-  const bool fast = copyable(x, ld_x, size) && copyable(weight, d->k, size);
-  return launch_type<GROUPED_FWD>(a, d->dtype, fast, d->n, (hipStream_t)stream);
+  return GROUPED_BY_TYPE(d->dtype, launch_rows, , GROUPED_FWD>(a, d, s));
 }
 
-namespace {
-
-// A masked gradient is written once (in rows of whole chunks) and read by plain copies where there is enough of it; otherwise
-// each product masks what it loads.
-bool mask_first(const mpe_grouped_desc *d) { return d->rows * d->n >= (int64_t)1 << MASKSH; }
-int64_t masked_ld(const mpe_grouped_desc *d) {
-  const int chunk = 16 / dtype_size(d->dtype);
-  return (d->n + chunk - 1) / chunk * chunk;
-}
-
-// Scratch of a backward pass: the masked gradient, the partial sums of dweight and of dbias.
-struct Scratch { int64_t masked, part, part_bias, total; };
-Scratch scratch_of(const mpe_grouped_desc *d, bool masked, bool want_dw) {
-  const int splits = dw_splits(d);
-  const auto up = [](int64_t b) { return (b + 15) / 16 * 16; };
-  Scratch s{};
-  s.part = masked ? up(d->rows * masked_ld(d) * dtype_size(d->dtype)) : 0;
-  const int64_t one = want_dw && splits > 1 ? (int64_t)splits * d->groups * d->n * 4 : 0;
-  s.part_bias = s.part + up(one * d->k);
-  s.total = s.part_bias + up(one);
-  return s;
-}
-
-template <typename T>
-int launch_mask(const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, void *out, int64_t rows, int n, hipStream_t s) {
-  constexpr int chunk = 16 / (int)sizeof(T);
-  const int64_t grid = (rows * ((n + chunk - 1) / chunk) + 255) / 256;
-  if (grid > kMaxGrid) return MPE_ERR_ARG;
-  hipLaunchKernelGGL(grouped_mask_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, (const T *)dy, ld_dy, (const T *)y, ld_y, (T *)out, rows, n);
-  return (int)hipGetLastError();
-}
-
-}  // namespace
-
-extern "C" int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *d, int with_y, int with_dweight) {
+extern "C" int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, const void *x,
+                                                  int64_t ld_x, const void *weight, int with_dx, int with_dweight) {
   if (const int rc = grouped_check(d)) return rc;
-  if (with_y < 0 || with_y > 1 || with_dweight < 0 || with_dweight > 1) return MPE_ERR_ARG;
-  return scratch_of(d, with_y && mask_first(d), with_dweight).total;
+  if (with_dx < 0 || with_dx > 1 || with_dweight < 0 || with_dweight > 1) return MPE_ERR_ARG;
+  return Backward(d, dy, ld_dy, y, 0, x, ld_x, weight, with_dx, with_dweight).ws.total;
 }
 
 extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
@@ -222,43 +255,31 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   for (const void *p : {dy, y, x, weight, (const void *)dx, (const void *)dweight, (const void *)dbias})
     if (bad_align(p, size)) return MPE_ERR_ALIGN;
   if (bad_align(workspace, 16)) return MPE_ERR_ALIGN;
-  const bool masked = y && mask_first(d);
-  const Scratch w = scratch_of(d, masked, dweight != nullptr);
-  if (w.total > 0 && !workspace) return MPE_ERR_NULL;
-  if (workspace_bytes < w.total) return MPE_ERR_SCRATCH;
+  Backward b(d, dy, ld_dy, y, ld_y, x, ld_x, weight, dx != nullptr, dweight != nullptr);
+  if (b.ws.total > 0 && !workspace) return MPE_ERR_NULL;
+  if (workspace_bytes < b.ws.total) return MPE_ERR_SCRATCH;
   hipStream_t s = (hipStream_t)stream;
-  if (masked) {
-    const int rc = d->dtype == MPE_F32    ? launch_mask<float>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s)
-                   : d->dtype == MPE_BF16 ? launch_mask<__bf16>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s)
-                                          : launch_mask<_Float16>(dy, ld_dy, y, ld_y, workspace, d->rows, d->n, s);
-    if (rc) return rc;
-    dy = workspace;
-    ld_dy = masked_ld(d);
-    y = nullptr;
-  }
-  const bool fast_d = d->rows > 0 && copyable(dy, ld_dy, size);
+  b.ws.place(b.d_, workspace);
+  b.ws.place(b.x, workspace);
+  b.ws.place(b.w, workspace);
+  if (const int rc = b.ws.run(d->dtype, s)) return rc;
   GroupedArgs a = base_args(d);
-  a.a = dy;
-  a.ld_a = ld_dy;
-  a.mask = y;
-  a.ld_mask = ld_y;
+  a.a = b.d_.p;
+  a.ld_a = b.d_.ld;
   if (dx && d->rows > 0) {
-    GroupedArgs b = a;
-    b.b = weight;
-    b.ld_b = d->k;
-    b.out = dx;
-    b.ld_out = ld_dx;
-    b.zero_tail = zero_tail;
-    if (const int rc = launch_type<GROUPED_DX>(b, d->dtype, fast_d && copyable(weight, d->k, size), d->k, s)) return rc;
+    a.b = b.w.p;
+    a.ld_b = b.w.ld;
+    a.out = dx;
+    a.ld_out = ld_dx;
+    a.zero_tail = zero_tail;
+    if (const int rc = GROUPED_BY_TYPE(d->dtype, launch_rows, , GROUPED_DX>(a, d, s))) return rc;
   }
   if (!dweight) return MPE_OK;
-  a.b = x;
-  a.ld_b = ld_x;
+  a.b = b.x.p;
+  a.ld_b = b.x.ld;
   a.out = dweight;
   a.dbias = dbias;
-  a.part = (float *)((char *)workspace + w.part);
-  a.part_bias = (float *)((char *)workspace + w.part_bias);
-  return d->dtype == MPE_F32    ? launch_dw<float>(a, d, fast_d && copyable(x, ld_x, size), s)
-         : d->dtype == MPE_BF16 ? launch_dw<__bf16>(a, d, fast_d && copyable(x, ld_x, size), s)
-                                : launch_dw<_Float16>(a, d, fast_d && copyable(x, ld_x, size), s);
+  a.part = (float *)((char *)workspace + b.part);
+  a.part_bias = (float *)((char *)workspace + b.part_bias);
+  return GROUPED_BY_TYPE(d->dtype, launch_dw, >(a, d, s));
 }

@@ -21,14 +21,13 @@ namespace mpe {
 enum GroupedMode { GROUPED_FWD = 0, GROUPED_DX = 1, GROUPED_DW = 2 };
 
 struct GroupedArgs {
-  const void *a, *b;        // forward: x, weight; dx: dy, weight; dw: dy, x
-  const void *mask;         // dx, dw: y (same layout as dy up to ld_mask), or NULL
+  const void *a, *b;        // forward: x, weight; dx: d, weight; dw: d, x
   const void *bias;         // forward: [G][N] or NULL
   void *out;                // forward: y; dx: dx; dw: dweight
   void *dbias;              // dw: [G][N] or NULL
   float *part, *part_bias;  // dw over splits: [S][G][N][K] and [S][G][N] partial sums
   const void *ends;
-  int64_t rows, ld_a, ld_b, ld_mask, ld_out;
+  int64_t rows, ld_a, ld_b, ld_out;
   int32_t groups, n, k, ends64, relu, zero_tail;
   int32_t tiles_i, tiles_j, splits;  // dw: tiles over n, over k, over rows; forward / dx: tiles_j only
 };
@@ -40,12 +39,9 @@ typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
 // 16 bytes with the alignment of one element (gfx950 loads and stores multi-dword data at any byte address)
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Chunk16 { T v[16 / sizeof(T)]; };
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Quad { T v[4]; };
 
 template <typename T> struct GroupedType;
 template <> struct GroupedType<float> {
-  static constexpr int kSteps = 4;  // matrix instructions per 16-byte chunk: 16x16x4 takes one f32 a lane
   static __device__ __forceinline__ f4v mma(const uint4 &p, const uint4 &q, f4v c) {
     const float *a = reinterpret_cast<const float *>(&p), *b = reinterpret_cast<const float *>(&q);
 #pragma unroll
@@ -137,86 +133,31 @@ __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int
 
 constexpr uint32_t kGroupedSpan = 0x7ffffff0u;  // bytes a tile's copies may reach (the host checks it); an offset outside
 
-// One operand's tile: ROWS of i (or j) by KC 16-byte chunks of c (KC = 4 or 8), in LDS.
-//   CONTIG (c contiguous in memory): [row][KC chunks], chunk q of row i at place q ^ swizzle(i): the 16 rows of a fragment
-//   are spread over the banks; a fragment is one 16-byte read.
-//   otherwise (row index contiguous in memory): [c][ROWS elements], the 16 elements of a fragment's row range (one unit) at
-//   place unit ^ swizzle(c), so that the c's which one read touches lie in different banks; a fragment is two transposing
-//   reads (16 bits) or four 4-byte reads (f32).
-// Two ways in.  FAST (bases and row strides multiples of 4 bytes: checked on the host): straight from memory to LDS by buffer
-// loads, whose bounds (the array's end, checked dword by dword) and whose offset beyond every bound (rows and columns outside
-// the tile's) read as zeros; or through registers where dy is masked.  Otherwise through registers, element by element at
-// the edges.
-template <typename T, int ROWS, int KC, int NT, bool CONTIG, bool FAST>
+// One operand's tile: ROWS of i (or j) by KC 16-byte chunks of c (KC = 4 or 8), copied from memory straight to LDS.
+//   CONTIG (c contiguous in memory): [row][KC chunks], chunk q of row i at place q ^ swizzle(i); a fragment is one 16-byte read.
+//   otherwise (row index contiguous): [c][ROWS elements], in units of 16 elements, unit u of line c at place u ^ swizzle(c); a
+//   fragment is two transposing reads (16 bits) or four 4-byte reads (f32).
+// The swizzles spread what one read touches over the LDS banks.
+// The copies are buffer loads: the buffer ends where the array does (checked dword by dword, reads as zeros), rows and columns
+// outside the tile's are given an offset outside every buffer.
+template <typename T, int ROWS, int KC, int NT, bool CONTIG>
 struct GroupedOperand {
   static constexpr int CE = 16 / sizeof(T), N = ROWS * KC / NT;
   static constexpr int kLine = CONTIG ? KC : ROWS / CE;  // chunks of a line (a row, or a c)
   static constexpr int kUnit = 16 / CE;                 // chunks of 16 elements
   static_assert(ROWS * KC % NT == 0, "whole chunks per thread");
-  uint4 r[N];
 
   static __device__ __forceinline__ int swizzle(int line) {  // on chunks for CONTIG, on units otherwise
-    if (CONTIG) return KC == 8 ? line & 7 : (line >> 1) & 3;  // 8 lanes' chunks in one pass of 128 bytes: 8 places
-    if (sizeof(T) == 4) return (line >> 2) & 3;               // 32 lanes on two c's four apart
+    if (CONTIG) return KC == 8 ? line & 7 : (line >> 1) & 3;            // 8 lanes' chunks in one pass of 128 bytes: 8 places
+    if (sizeof(T) == 4) return (line >> 2) & 3;                         // 32 lanes on two c's four apart
     if (ROWS == 64) return ((line >> 1) & 1) | ((line >> 3) & 1) << 1;  // 32 lanes on eight c's: 256 bytes
     return (line & 3) | ((line >> 3) & 1) << 2;
   }
   static __device__ __forceinline__ int place(int line, int pos) {  // of chunk pos of a line; its own inverse in pos
     return CONTIG ? pos ^ swizzle(line) : (((pos / kUnit) ^ swizzle(line)) * kUnit + pos % kUnit);
   }
-  static __device__ __forceinline__ uint4 load(const T *p, int64_t off, int valid) {
-    if (valid >= CE) return __builtin_bit_cast(uint4, *reinterpret_cast<const Chunk16<T> *>(p + off));
-    Chunk16<T> c;
-#pragma unroll
-    for (int e = 0; e < CE; ++e) c.v[e] = e < valid ? p[off + e] : T(0);
-    return __builtin_bit_cast(uint4, c);
-  }
-  // keeps the elements of v whose saved output is > 0 or NaN (relu's derivative: zero where y <= 0)
-  static __device__ __forceinline__ uint4 keep(uint4 v, uint4 y) {
-    if constexpr (sizeof(T) == 4) {
-      Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, v), m = __builtin_bit_cast(Chunk16<T>, y);
-#pragma unroll
-      for (int e = 0; e < CE; ++e) c.v[e] = m.v[e] <= 0.0f ? 0.0f : c.v[e];
-      return __builtin_bit_cast(uint4, c);
-    } else {
-    // two elements an instruction: positive bits stay, of the others only what lies above -infinity (NaN); times 0 or 1
-    typedef unsigned short u2 __attribute__((ext_vector_type(2)));
-    typedef short i2 __attribute__((ext_vector_type(2)));
-    const unsigned short ninf = __builtin_bit_cast(unsigned short, (T)(-__builtin_inff()));
-    uint32_t *c = reinterpret_cast<uint32_t *>(&v);
-    const uint32_t *m = reinterpret_cast<const uint32_t *>(&y);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const u2 b = __builtin_bit_cast(u2, m[e]);
-      const u2 nan = __builtin_elementwise_sub_sat(b, u2{ninf, ninf});
-      const u2 pos = __builtin_bit_cast(u2, __builtin_elementwise_max(__builtin_bit_cast(i2, b), i2{0, 0}));
-      c[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(u2, c[e]) * __builtin_elementwise_min(nan | pos, u2{1, 1}));
-    }
-    return v;
-    }
-  }
-  // p: element (row 0, c 0) of the tile column; rows / cs: how many of them from there exist
-  __device__ __forceinline__ void fetch(const T *p, int64_t ld, const T *mask, int64_t ld_mask, int64_t rows, int64_t cs) {
-    const int t = threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int id = t + u * NT, line = id / kLine, pos = (id % kLine) * CE;
-      const int64_t valid = CONTIG ? (line < rows ? cs - pos : 0) : (line < cs ? rows - pos : 0);
-      const int v = valid < 0 ? 0 : (valid < CE ? (int)valid : CE);
-      r[u] = v > 0 ? load(p, line * ld + pos, v) : uint4{0, 0, 0, 0};
-      if (mask != nullptr && v > 0) r[u] = keep(r[u], load(mask, line * ld_mask + pos, v));
-    }
-  }
-  __device__ __forceinline__ void put(uint4 *lds) const {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int id = threadIdx.x + u * NT, line = id / kLine;
-      lds[line * kLine + place(line, id % kLine)] = r[u];
-    }
-  }
-  // Without registers: a wavefront's 64 chunks land side by side in LDS, so each lane fetches what belongs at its place.
+  // A wavefront's 64 chunks land side by side in LDS, so each lane fetches what belongs at its place.
   // at: the chunks' byte offsets in the tile; left: how many c's exist from there on (none for a chunk outside the rows).
-  // A chunk with nothing left is given an offset outside the buffer, which reads as zeros.
   uint32_t at[N];
   int left[N];
   __device__ __forceinline__ void aim(int64_t ld, int64_t rows, int64_t cs) {
@@ -255,18 +196,19 @@ struct GroupedOperand {
       }
     }
   }
-  // lane l's share of k-step kk: row i0 + l % 16, c = kk * 4 CE + (l / 16) * CE .. + CE   (i0: a multiple of 16)
+  // lane l's share of the fragment of rows i0 .. i0 + 15 (i0: a multiple of 16), k-step kk: row l % 16, c = kk * 4 CE +
+  // (l / 16) * CE .. + CE
   static __device__ __forceinline__ uint4 frag(const uint4 *lds, int i0, int kk) {
     const int lane = threadIdx.x & 63, t = lane & 15, q = lane >> 4;
     if (CONTIG) return lds[(i0 + t) * KC + ((kk * 4 + q) ^ swizzle(t))];
     if constexpr (sizeof(T) == 4) {
       const float *s = reinterpret_cast<const float *>(lds);
-      float4 f;
-      float *v = reinterpret_cast<float *>(&f);
+      float4 out;
+      float *v = reinterpret_cast<float *>(&out);
       const int at = q * 4 * ROWS + ((i0 / 16) ^ swizzle(q * 4)) * 16 + t;  // swizzle: the same for every kk and e
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = s[(kk * 16 + e) * ROWS + at];
-      return __builtin_bit_cast(uint4, f);
+      return __builtin_bit_cast(uint4, out);
     } else {
       // 16 lanes read 4 c's of 16 elements, 8 bytes a lane; each lane gets its element of the four
       typedef short s4 __attribute__((ext_vector_type(4)));
@@ -283,6 +225,9 @@ struct GroupedOperand {
   }
 };
 
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Quad { T v[4]; };
+// four neighbours of an output row, valid of them inside it
 template <typename T>
 __device__ __forceinline__ void grouped_store4(T *p, f4v v, int valid) {
   if (valid >= 4) {
@@ -307,21 +252,19 @@ __device__ __forceinline__ int grouped_block() {
   return at / kRun * (8 * kRun) + b % 8 * kRun + at % kRun;
 }
 
-enum GroupedPath { GROUPED_ANY = 0, GROUPED_FAST = 1, GROUPED_FAST_MASK = 2 };  // how tiles are loaded; FAST_MASK: A times its mask
-
 // STAGES buffers of KC chunks a row: while one is multiplied, STAGES - 1 are on their way.
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int PATH, int KC, int STAGES>
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int KC, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_kernel(GroupedArgs a) {
-  constexpr bool FAST = PATH != GROUPED_ANY, regs_a = PATH != GROUPED_FAST;
   constexpr int NT = 64 * WM * WN, KE = KC * 16 / (int)sizeof(T);
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
-  using OpA = GroupedOperand<T, BM, KC, NT, MODE != GROUPED_DW, FAST>;
-  using OpB = GroupedOperand<T, BN, KC, NT, MODE == GROUPED_FWD, FAST>;
-  static_assert(PATH == GROUPED_FAST || STAGES == 2, "what passes through registers is one stage ahead");
+  constexpr bool EDGES = BM < 256;  // the large tile, short of registers, takes whole chunks only (n and k multiples of 8)
+  using OpA = GroupedOperand<T, BM, KC, NT, MODE != GROUPED_DW>;
+  using OpB = GroupedOperand<T, BN, KC, NT, MODE == GROUPED_FWD>;
   // separate arrays: the compiler then knows that a read of one does not wait for copies into another
   constexpr int kStage = (BM + BN) * KC;  // A's chunks, then B's
-  __shared__ uint4 s0[kStage], s1[kStage], s2[STAGES > 2 ? kStage : 1], s3[STAGES > 3 ? kStage : 1];
-  const T *pa = static_cast<const T *>(a.a), *pb = static_cast<const T *>(a.b), *pm = static_cast<const T *>(a.mask);
+  static_assert(STAGES == 2 || STAGES == 4, "the loop below");
+  __shared__ uint4 s0[kStage], s1[kStage], s2[STAGES == 4 ? kStage : 1], s3[STAGES == 4 ? kStage : 1];
+  const T *pa = static_cast<const T *>(a.a), *pb = static_cast<const T *>(a.b);
 
   // ---- which tile ------------------------------------------------------------------------------------------------------
   const int block = grouped_block();
@@ -358,11 +301,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     }
   }
   const bool tail = MODE != GROUPED_DW && c_end == 0;
-  // bytes to the arrays' ends, whole dwords (their last 2-byte element may share one with nothing)
-  const auto end_of = [](int64_t lines, int64_t ld, int64_t cols) { return (((lines - 1) * ld + cols) * (int64_t)sizeof(T) + 3) & ~(int64_t)3; };
-  const int64_t end_a = end_of(a.rows, a.ld_a, MODE == GROUPED_FWD ? a.k : a.n);
-  const int64_t end_b = MODE == GROUPED_DW ? end_of(a.rows, a.ld_b, a.k) : end_of((int64_t)a.groups * a.n, a.k, a.k);
-  const int64_t b0 = MODE == GROUPED_DW ? 0 : (int64_t)g * a.n * a.k;
+  // the arrays: lines, columns, elements to their ends
+  const int64_t lines_b = MODE == GROUPED_DW ? a.rows : (int64_t)a.groups * a.n;
+  const int cols_a = MODE == GROUPED_FWD ? a.k : a.n, cols_b = a.k;
+  const int64_t end_a = (a.rows - 1) * a.ld_a + cols_a, end_b = (lines_b - 1) * a.ld_b + cols_b;
+  const int64_t b0 = MODE == GROUPED_DW ? 0 : (int64_t)g * a.n * a.ld_b;
 
   // ---- the product: two stages, one barrier a k-step; the next stage is on its way while this one is multiplied ------------
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -371,36 +314,23 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   float sum[MI] = {};  // dbias: this lane's share of its rows' (n's) sums
   OpA oa;
   OpB ob;
-  if constexpr (FAST) {
-    if constexpr (!regs_a) oa.aim(a.ld_a, i_end - i0, c_end - c0);
-    ob.aim(a.ld_b, j_end - j0, c_end - c0);
-  }
+  oa.aim(a.ld_a, i_end - i0, c_end - c0);
+  ob.aim(a.ld_b, j_end - j0, c_end - c0);
   auto fetch = [&](int64_t c, uint4 *la) {
-    uint4 *lb = la + BM * KC;
     const int64_t at = MODE == GROUPED_DW ? c * a.ld_a + i0 : i0 * a.ld_a + c;
     const int64_t bt = b0 + (MODE == GROUPED_FWD ? j0 * a.ld_b + c : c * a.ld_b + j0);
-    if constexpr (regs_a) {
-      const T *mt = pm == nullptr ? nullptr : MODE == GROUPED_DW ? pm + c * a.ld_mask + i0 : pm + i0 * a.ld_mask + c;
-      oa.fetch(pa + at, a.ld_a, mt, a.ld_mask, i_end - i0, c_end - c);
-    } else {
-      oa.copy(la, pa + at, end_a - at * (int64_t)sizeof(T));
-    }
-    if constexpr (FAST) ob.copy(lb, pb + bt, end_b - bt * (int64_t)sizeof(T));
-    else ob.fetch(pb + bt, a.ld_b, nullptr, 0, j_end - j0, c_end - c);
+    oa.copy(la, pa + at, (end_a - at) * (int64_t)sizeof(T));
+    ob.copy(la + BM * KC, pb + bt, (end_b - bt) * (int64_t)sizeof(T));
   };
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
   constexpr int kAhead = (STAGES - 2) * (OpA::N + OpB::N);  // copies of later stages that may still be under way
   auto step = [&](int64_t c, uint4 *la, uint4 *next) {
     uint4 *lb = la + BM * KC;
-    if constexpr (regs_a) oa.put(la);
-    if constexpr (!FAST) ob.put(lb);
-    // this wavefront's copies of this stage have landed, its reads and writes of LDS are done; then so are everybody's
-    if constexpr (FAST) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
-      if (MODE != GROUPED_DW && c_end - c < KE && (c_end - c) % OpA::CE != 0) {
-        if constexpr (!regs_a) oa.trim(la, STAGES - 1);
-        ob.trim(lb, STAGES - 1);
-      }
+    // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
+    if (EDGES && MODE != GROUPED_DW && c_end - c < KE && (c_end - c) % OpA::CE != 0) {
+      oa.trim(la, STAGES - 1);
+      ob.trim(lb, STAGES - 1);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -430,16 +360,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   };
   if (c0 < c_end) {
     fetch(c0, s0);
-    if constexpr (STAGES > 2) fetch(c0 + KE, s1);
-    if constexpr (STAGES > 3) fetch(c0 + 2 * KE, s2);
+    if constexpr (STAGES == 4) fetch(c0 + KE, s1), fetch(c0 + 2 * KE, s2);
     for (int64_t c = c0; c < c_end; c += STAGES * KE) {  // steps past the end multiply zeros
       if constexpr (STAGES == 2) {
         step(c, s0, s1);
         step(c + KE, s1, s0);
-      } else if constexpr (STAGES == 3) {
-        step(c, s0, s2);
-        step(c + KE, s1, s0);
-        step(c + 2 * KE, s2, s1);
       } else {
         step(c, s0, s3);
         step(c + KE, s1, s0);
@@ -451,6 +376,32 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
 
   // ---- epilogue: lane holds output row i0 + wi + 16 m + lane % 16, columns j0 + wj + 16 n + 4 (lane / 16) .. + 4 ----------
   const int64_t j_lane = j0 + wj + 4 * (lane >> 4);
+  if (EDGES && sizeof(T) == 2 && c0 < c_end && ((cols_a | cols_b) & 1)) {
+    // 2-byte elements in lines of odd width: an array's last element is half of a dword that the buffer's bounds cut off, and
+    // was multiplied as zero.  What it should have added: A(i, ca) B(j, ca) for A's, A(i, cb) B(j, cb) for B's.
+    const int64_t last_b = lines_b - 1 - (MODE == GROUPED_DW ? 0 : (int64_t)g * a.n);  // B's last line: a c, or forward a j
+    const int64_t ia = MODE == GROUPED_DW ? cols_a - 1 : a.rows - 1, ca = MODE == GROUPED_DW ? a.rows - 1 : cols_a - 1;
+    const int64_t jb = MODE == GROUPED_FWD ? last_b : cols_b - 1, cb = MODE == GROUPED_FWD ? cols_b - 1 : last_b;
+    const bool cut_a = (cols_a & 1) && ia >= i0 && ia < i0 + BM && ia < i_end && ca >= c0 && ca < c_end;
+    const bool cut_b = (cols_b & 1) && jb >= j0 && jb < j0 + BN && jb < j_end && cb >= c0 && cb < c_end;
+    const auto elem_a = [&](int64_t i, int64_t c) { return (float)pa[MODE == GROUPED_DW ? c * a.ld_a + i : i * a.ld_a + c]; };
+    const auto elem_b = [&](int64_t j, int64_t c) { return (float)pb[b0 + (MODE == GROUPED_FWD ? j * a.ld_b + c : c * a.ld_b + j)]; };
+    if (cut_a || cut_b) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int64_t i = i0 + wi + m * 16 + (lane & 15);
+        if (cut_a && i == ia && with_bias && lane < 16) sum[m] += elem_a(ia, ca);
+#pragma unroll
+        for (int n = 0; n < NJ; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int64_t j = j_lane + n * 16 + e;
+            if (cut_a && i == ia && j < j_end) acc[m][n][e] += elem_a(ia, ca) * elem_b(j, ca);
+            if (cut_b && j == jb && i < i_end && !(cut_a && i == ia && ca == cb)) acc[m][n][e] += elem_a(i, cb) * elem_b(jb, cb);
+          }
+      }
+    }
+  }
   const auto valid_of = [&](int n) { return j_end - j_lane - n * 16 >= 4 ? 4 : (int)(j_end - j_lane - n * 16); };
   if constexpr (MODE == GROUPED_FWD) {
     if (a.bias != nullptr && !tail) {  // all of it first: one wait
@@ -477,19 +428,13 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     }
   }
   const auto store = [&](auto *out, int64_t ld) {  // out: the array's row 0
-    auto *p = out + (i0 + wi + (lane & 15)) * ld + j_lane;
-    if (i0 + BM <= i_end && j0 + BN <= j_end) {  // the whole tile: no tests
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) grouped_store4(p + m * 16 * ld + n * 16, acc[m][n], 4);
-      return;
-    }
+    auto *at = out + (i0 + wi + (lane & 15)) * ld + j_lane;
+    const bool whole = i0 + BM <= i_end && j0 + BN <= j_end;  // no tests
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      if (i0 + wi + m * 16 + (lane & 15) >= i_end) continue;
+      if (!whole && i0 + wi + m * 16 + (lane & 15) >= i_end) continue;
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) grouped_store4(p + m * 16 * ld + n * 16, acc[m][n], valid_of(n));
+      for (int n = 0; n < NJ; ++n) grouped_store4(at + m * 16 * ld + n * 16, acc[m][n], whole ? 4 : valid_of(n));
     }
   };
   if constexpr (MODE == GROUPED_DW) {
@@ -512,16 +457,60 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   }
 }
 
-// d = dy where y is not <= 0, zero elsewhere, in rows of whole chunks: both products of a backward pass then copy it.
+// Copies matrices into rows of whole chunks where their stride is too large for a tile's copies, and applies relu's mask to dy
+// on the way: d = dy where y is not <= 0, zero elsewhere.
+struct GroupedPack { const void *src, *mask; void *dst; int64_t ld, ld_mask, lines; int32_t cols, blocks; };
+struct GroupedPacks { GroupedPack job[3]; };
+
+// keeps the elements of v whose saved output is > 0 or NaN (relu's derivative: zero where y <= 0)
 template <typename T>
-__global__ __launch_bounds__(256) void grouped_mask_kernel(const T *dy, int64_t ld_dy, const T *y, int64_t ld_y, T *d, int64_t rows, int n) {
+__device__ __forceinline__ Chunk16<T> grouped_keep(Chunk16<T> v, const Chunk16<T> &y) {
+#pragma unroll
+  for (int e = 0; e < 16 / (int)sizeof(T); ++e) v.v[e] = (float)y.v[e] <= 0.0f ? T(0) : v.v[e];
+  return v;
+}
+// the chunk at element off, valid of it kept; end: elements of the whole matrix (a chunk may reach into the next line)
+template <typename T>
+__device__ __forceinline__ Chunk16<T> grouped_chunk(const T *p, int64_t off, int valid, int64_t end) {
   constexpr int CE = 16 / sizeof(T);
-  using Op = GroupedOperand<T, 64, 8, 256, true, false>;
-  const int chunks = (n + CE - 1) / CE;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / chunks;
-  if (row >= rows) return;
-  const int col = (int)(at % chunks) * CE, valid = n - col < CE ? n - col : CE;
-  *reinterpret_cast<uint4 *>(d + at * CE) = Op::keep(Op::load(dy, row * ld_dy + col, valid), Op::load(y, row * ld_y + col, valid));
+  Chunk16<T> c;
+  if (valid > 0 && off + CE <= end) {
+    c = *reinterpret_cast<const Chunk16<T> *>(p + off);
+#pragma unroll
+    for (int e = 1; e < CE; ++e) c.v[e] = e < valid ? c.v[e] : T(0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < CE; ++e) c.v[e] = e < valid ? p[off + e] : T(0);
+  }
+  return c;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_pack_kernel(GroupedPacks a) {
+  constexpr int CE = 16 / sizeof(T);
+  uint32_t b = blockIdx.x, k = 0;
+  while (k < 2 && b >= (uint32_t)a.job[k].blocks) b -= a.job[k++].blocks;
+  const GroupedPack &j = a.job[k];
+  // a workgroup: some whole lines of up to 256 chunks, or up to 256 chunks of one line; one chunk a thread
+  const uint32_t chunks = (uint32_t)((j.cols + CE - 1) / CE), t = threadIdx.x;
+  int64_t line;
+  uint32_t at;
+  if (chunks <= 256) {
+    const uint32_t lines = 256 / chunks, sub = t / chunks;
+    line = (int64_t)b * lines + sub;
+    at = t - sub * chunks;
+    if (sub >= lines) return;
+  } else {
+    const uint32_t per = (chunks + 255) / 256, q = b / per;
+    line = q;
+    at = (b - q * per) * 256 + t;
+    if (at >= chunks) return;
+  }
+  if (line >= j.lines) return;
+  const int col = (int)at * CE, valid = j.cols - col < CE ? j.cols - col : CE;
+  Chunk16<T> c = grouped_chunk(static_cast<const T *>(j.src), line * j.ld + col, valid, (j.lines - 1) * j.ld + j.cols);
+  if (j.mask)
+    c = grouped_keep(c, grouped_chunk(static_cast<const T *>(j.mask), line * j.ld_mask + col, valid, (j.lines - 1) * j.ld_mask + j.cols));
+  *reinterpret_cast<uint4 *>(static_cast<T *>(j.dst) + (line * chunks + at) * CE) = __builtin_bit_cast(uint4, c);
 }
 
 // dw over splits: the partial sums of dweight (cw values) and dbias (cb) in split order, rounded once.

@@ -9,7 +9,8 @@ learners evaluate one network at a time, maddpg/maddpg/trainer/maddpg.py:161-196
 (``group_ends(sizes, device)`` makes it from row counts).  The kernels read ``ends`` from device memory, so a captured
 launch follows what the tensor holds at replay and nothing is copied to the host; whatever it holds, it is read as its
 running maximum clamped to ``[0, rows]``.  Groups may be empty.  float32, bfloat16 and float16, all arrays alike;
-sums are in 32 bits, each result is rounded once.  1 <= groups <= 1024; rows and n * k below 2**31.
+sums are in 32 bits, each result is rounded once.  1 <= groups <= 1024; n and k up to 2**20, rows and n * k
+below 2**31.
 
 Rows of ``x`` may have any stride; an ``x`` whose columns are not adjacent is copied first (also a ``weight`` or ``bias``
 that is not contiguous).  ``grouped_linear`` is differentiable (once) in ``x``, ``weight`` and ``bias``;
@@ -78,7 +79,7 @@ def _refuse(x, weight, ends, bias):
     if ends.dtype not in (torch.int32, torch.int64) or tuple(ends.shape) != (g,) or ends.device != x.device:
         raise ValueError('ends: expected int32 or int64 [%d] on %s, got %s %s on %s'
                          % (g, x.device, ends.dtype, list(ends.shape), ends.device))
-    raise ValueError('rows and n * k are below 2**31')
+    raise ValueError('n and k are up to 2**20, rows and n * k below 2**31')
 
 
 def _check(x, weight, ends, bias=None):
@@ -88,7 +89,7 @@ def _check(x, weight, ends, bias=None):
         dtype, index, e64 = x.dtype, x.get_device(), ends.dtype is torch.int64
         ok = (index >= 0 and dtype in _DTYPES and weight.dtype is dtype and weight.get_device() == index and wk == k and ge == g
               and ends.get_device() == index and (e64 or ends.dtype is torch.int32) and 1 <= g <= MAX_GROUPS and n >= 1 and k >= 1
-              and rows < 1 << 31 and n * k < 1 << 31
+              and rows < 1 << 31 and n * k < 1 << 31 and n <= 1 << 20 and k <= 1 << 20
               and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == (g, n))))
     except (ValueError, AttributeError, TypeError):
         ok = False
@@ -105,6 +106,12 @@ def _overlap(a, b):
         return False
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
+
+
+def _scratch(x, need):
+    """``need`` bytes of this call's own (from torch's allocator, so on this stream or of this recording)."""
+    _hip.check(min(need, 0), 'workspace')
+    return x.new_empty((need + 3) // 4, dtype=torch.float32)
 
 
 def _forward(x, weight, ends, bias, relu, out):
@@ -126,8 +133,12 @@ def _forward(x, weight, ends, bias, relu, out):
             raise ValueError('out: its columns must be adjacent and its rows must not overlap')
         if any(_overlap(out, t) for t in (x, weight, bias, ends)):
             raise ValueError('out overlaps an input')
-    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear, desc, x.data_ptr(), ld_x, weight.data_ptr(),
-                           None if bias is None else bias.data_ptr(), out.data_ptr(), ld_y, relu, own), 'mpe_grouped_linear')
+    px, pw, ws = x.data_ptr(), weight.data_ptr(), None
+    need = _hip.lib.mpe_grouped_linear_workspace(desc, px, ld_x, pw)
+    if need:
+        ws = _scratch(x, need)
+    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear, desc, px, ld_x, pw, None if bias is None else bias.data_ptr(),
+                           out.data_ptr(), ld_y, relu, own, _hip.ptr(ws), need), 'mpe_grouped_linear')
     return out
 
 
@@ -181,11 +192,10 @@ def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dw
         x, ld_x = _rows_of(x)
         dw = x.new_empty(weight.shape)
         db = x.new_empty(weight.shape[:2]) if need_dbias else None
-    need = _hip.lib.mpe_grouped_backward_workspace(desc, y is not None, both)
-    _hip.check(min(need, 0), 'mpe_grouped_backward_workspace')
+    pg, py, px, pw = grad.data_ptr(), _hip.ptr(y), x.data_ptr(), weight.data_ptr()
+    need = _hip.lib.mpe_grouped_backward_workspace(desc, pg, ld_g, py, px, ld_x, pw, need_dx, both)
     if need:
-        ws = x.new_empty((need + 3) // 4, dtype=torch.float32)
-    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear_backward, desc, grad.data_ptr(), ld_g, _hip.ptr(y), ld_y, x.data_ptr(),
-                           ld_x, weight.data_ptr(), _hip.ptr(dx), k, 1, _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need),
+        ws = _scratch(x, need)
+    _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear_backward, desc, pg, ld_g, py, ld_y, px, ld_x, pw, _hip.ptr(dx), k, 1, _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need),
                'mpe_grouped_linear_backward')
     return dx, dw if need_dweight else None, db

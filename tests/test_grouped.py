@@ -33,26 +33,27 @@ def _desc(**kw):
 
 @pytest.mark.parametrize('change,code', [
     (dict(ends=None), -1), (dict(dtype=3), -5), (dict(groups=0), -6), (dict(groups=1025), -6), (dict(n=0), -6), (dict(k=0), -6),
-    (dict(rows=-1), -6), (dict(rows=1 << 31), -6), (dict(n=1 << 16, k=1 << 15), -6), (dict(ends=4098), -4),
+    (dict(rows=-1), -6), (dict(rows=1 << 31), -6), (dict(n=1 << 16, k=1 << 15), -6), (dict(n=(1 << 20) + 1), -6), (dict(k=(1 << 20) + 1), -6), (dict(ends=4098), -4),
     (dict(ends=4100, ends64=1), -4), (dict(ends64=2), -6)])
 def test_c_abi_refuses_bad_descriptors(change, code):
     """Nothing is launched: the pointers are never read."""
     d, p = _desc(**change), 1 << 20
-    assert _hip.lib.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 0, None) == code
-    assert _hip.lib.mpe_grouped_backward_workspace(d, 0, 1) == code
+    assert _hip.lib.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 0, None, 0, None) == code
+    assert _hip.lib.mpe_grouped_linear_workspace(d, p, 3, p) == code
+    assert _hip.lib.mpe_grouped_backward_workspace(d, p, 5, None, p, 3, p, 1, 1) == code
     assert _hip.lib.mpe_grouped_linear_backward(d, p, 5, None, 0, p, 3, p, p, 3, 0, p, p, None, 0, None) == code
 
 
 def test_c_abi_refuses_bad_arrays():
     L, d, p = _hip.lib, _desc(), 1 << 20
-    assert L.mpe_grouped_linear(None, p, 3, p, None, p, 5, 0, 0, None) == -1
-    assert L.mpe_grouped_linear(d, None, 3, p, None, p, 5, 0, 0, None) == -1
-    assert L.mpe_grouped_linear(d, p, 2, p, None, p, 5, 0, 0, None) == -6
-    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 4, 0, 0, None) == -6
-    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 2, 0, None) == -6
-    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 2, None) == -6
-    assert L.mpe_grouped_linear(d, p + 2, 3, p, None, p, 5, 0, 0, None) == -4
-    assert L.mpe_grouped_linear(d, p, 3, p, p + 1, p, 5, 0, 0, None) == -4
+    assert L.mpe_grouped_linear(None, p, 3, p, None, p, 5, 0, 0, None, 0, None) == -1
+    assert L.mpe_grouped_linear(d, None, 3, p, None, p, 5, 0, 0, None, 0, None) == -1
+    assert L.mpe_grouped_linear(d, p, 2, p, None, p, 5, 0, 0, None, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 4, 0, 0, None, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 2, 0, None, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 2, None, 0, None) == -6
+    assert L.mpe_grouped_linear(d, p + 2, 3, p, None, p, 5, 0, 0, None, 0, None) == -4
+    assert L.mpe_grouped_linear(d, p, 3, p, p + 1, p, 5, 0, 0, None, 0, None) == -4
     ok = dict(dy=p, ld_dy=5, y=None, ld_y=0, x=p, ld_x=3, w=p, dx=p, ld_dx=3, zero=0, dw=p, db=p, ws=None, size=0)
 
     def back(desc=d, **kw):
@@ -62,13 +63,20 @@ def test_c_abi_refuses_bad_arrays():
                      (dict(y=p + 2, ld_y=5), -4), (dict(x=p + 2), -4), (dict(w=p + 2), -4), (dict(dx=p + 2), -4), (dict(dw=p + 2), -4),
                      (dict(db=p + 2), -4), (dict(ws=p + 8), -4)):
         assert back(**kw) == code, kw
-    assert L.mpe_grouped_backward_workspace(d, 2, 1) == -6 and L.mpe_grouped_backward_workspace(d, 0, -1) == -6
-    assert L.mpe_grouped_backward_workspace(d, 0, 1) == 0
+    def size(desc=d, y=None, dx=1, dw=1):
+        return L.mpe_grouped_backward_workspace(desc, p, 5, y, p, 3, p, dx, dw)
+    assert size(dx=2) == -6 and size(dw=-1) == -6 and size() == 0 and size(y=p) == 4 * 8 * 4   # y: dy masked, in whole chunks
     big = _desc(rows=1 << 20)                                     # rows split over workgroups: partial sums need an array
-    need = L.mpe_grouped_backward_workspace(big, 0, 1)
-    assert need > 0 and L.mpe_grouped_backward_workspace(big, 0, 0) == 0
+    need = size(big)
+    assert need > 0 and size(big, dw=0) == 0
     assert back(big, ws=None, size=need) == -1
     assert back(big, ws=p, size=need - 1) == -7
+    far = 1 << 24                                                 # rows so far apart that they are packed into scratch first
+    need = L.mpe_grouped_linear_workspace(d, p, far, p)
+    assert need == 4 * 4 * 4 and L.mpe_grouped_linear_workspace(d, p, 3, p) == 0
+    assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, None, need, None) == -1
+    assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, p, need - 1, None) == -7
+    assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, p + 8, need, None) == -4
     assert C.sizeof(_hip.GroupedDesc) == 40
 
 
@@ -299,6 +307,48 @@ def test_arguments_are_checked():
     assert dx.shape == (0, 6) and not dw.any() and not db.any()
     dx, dw, db = grouped.grouped_linear_backward(grad, x, w, ends, need_dx=False, need_dbias=False)
     assert dx is None and db is None and dw.shape == w.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('at', [0, 1, 2, 3])
+def test_every_alignment_of_odd_widths_and_the_arrays_last_elements(dtype, at):
+    """Odd and even widths at every 2-byte place; the arrays end where their memory's used part does (NaN behind and before),
+    and the last element of each counts."""
+    for sizes, k, n in (([7, 66], 9, 11), ([130, 1], 65, 67), ([5, 60], 71, 130), ([3], 1, 1), ([64, 3], 130, 5), ([300, 2], 129, 131)):
+        x, w, b, grad, ends = _case(sizes, k, n, dtype, seed=at)
+
+        def place(t):
+            flat = torch.full((t.numel() + at + 64,), float('nan'), dtype=dtype, device='cuda')
+            return flat[at:at + t.numel()].view(t.shape).copy_(t)
+        x, w, b, grad = (place(t) for t in (x, w, b, grad))
+        for t in (x, w, grad):
+            t.view(-1)[-1] = 30.0
+        y = grouped.grouped_linear(x, w, ends, bias=b)
+        got = (y,) + grouped.grouped_linear_backward(grad, x, w, ends)
+        want, terms = _reference(x, w, b, grad, sizes, False)
+        most = max(sizes)
+        for o, ref, ab, count, what in zip(got, want, terms, (k + 1, n, most, most), ('y', 'dx', 'dw', 'db')):
+            _close(o, ref, ab, count, dtype, (what, sizes, k, n))
+        relu = place(torch.randn(grad.shape, device='cuda').to(dtype))
+        got = grouped.grouped_linear_backward(grad, x, w, ends, y=relu)
+        want, terms = _reference(x, w, b, grad, sizes, False, relu)
+        for o, ref, ab, count, what in zip(got, want[1:], terms[1:], (n, most, most), ('dx', 'dw', 'db')):
+            _close(o, ref, ab, count, dtype, (what, sizes, k, n, 'masked'))
+
+
+@pytest.mark.gpu
+def test_rows_that_lie_far_apart_are_packed_first():
+    """A row stride beyond what a tile's copies reach (2^23 bytes): the same result as from adjacent rows."""
+    sizes, k, n = [3, 4], 70, 40
+    x, w, b, grad, ends = _case(sizes, k, n, torch.float32)
+    far = torch.zeros(7 << 21, device='cuda').view(7, 1 << 21)
+    xs, gs = far[:, 5:5 + k], far[:, 1000:1000 + n]
+    xs.copy_(x)
+    gs.copy_(grad)
+    assert torch.equal(grouped.grouped_linear(xs, w, ends, bias=b), grouped.grouped_linear(x, w, ends, bias=b))
+    for got, want in zip(grouped.grouped_linear_backward(gs, xs, w, ends), grouped.grouped_linear_backward(grad, x, w, ends)):
+        assert torch.equal(got, want)
 
 
 @pytest.mark.gpu

@@ -572,8 +572,8 @@ int mpe_env_step_stats_static(const mpe_scenario_desc *desc, int64_t B, int64_t 
  * stride 1, any alignment of an element.  dtype is of all float arrays.  1 <= groups <= 1024; n and k up to 2^20, rows and n * k below 2^31.
  * mpe_grouped_linear_workspace / mpe_grouped_backward_workspace: bytes that a call with these arrays needs (>= 0, or
  * MPE_ERR_*; no memory is read); the array is scratch of that call, 16-byte aligned; calls that may overlap (other streams,
- * concurrent graph replays) need one each.  What needs scratch: y, rows that lie 2^20 elements or more apart, and dweight
- * where its sums are split over the rows.
+ * concurrent graph replays) need one each.  What needs scratch: y beside large products, rows that lie 2^20 elements or more
+ * apart, and dweight where its sums are split over the rows.
  */
 #define MPE_F32 0
 #define MPE_BF16 1
@@ -586,7 +586,7 @@ typedef struct mpe_grouped_desc {
 int mpe_grouped_linear(const mpe_grouped_desc *desc, const void *x, int64_t ld_x, const void *weight, const void *bias,
                        void *y, int64_t ld_y, int relu, int zero_tail, void *workspace, int64_t workspace_bytes, void *stream);
 int64_t mpe_grouped_linear_workspace(const mpe_grouped_desc *desc, const void *x, int64_t ld_x, const void *weight);
-int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y,
+int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
                                        const void *x, int64_t ld_x, const void *weight, int with_dx, int with_dweight);
 int mpe_grouped_linear_backward(const mpe_grouped_desc *desc, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
                                 const void *x, int64_t ld_x, const void *weight, void *dx, int64_t ld_dx, int zero_tail,

@@ -205,8 +205,8 @@ def _load():
     L.mpe_grouped_linear.argtypes = [gp, vp, i64, vp, vp, vp, i64, ci, ci, vp, i64, vp]
     L.mpe_grouped_linear_workspace.restype = i64  # desc, x, ld_x, weight
     L.mpe_grouped_linear_workspace.argtypes = [gp, vp, i64, vp]
-    L.mpe_grouped_backward_workspace.restype = i64  # desc, dy, ld_dy, y, x, ld_x, weight, with_dx, with_dweight
-    L.mpe_grouped_backward_workspace.argtypes = [gp, vp, i64, vp, vp, i64, vp, ci, ci]
+    L.mpe_grouped_backward_workspace.restype = i64  # desc, dy, ld_dy, y, ld_y, x, ld_x, weight, with_dx, with_dweight
+    L.mpe_grouped_backward_workspace.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, ci, ci]
     # desc, dy, ld_dy, y, ld_y, x, ld_x, weight, dx, ld_dx, zero_tail, dweight, dbias, workspace, workspace_bytes, stream
     L.mpe_grouped_linear_backward.restype = ci
     L.mpe_grouped_linear_backward.argtypes = [gp, vp, i64, vp, i64, vp, i64, vp, vp, i64, ci, vp, vp, vp, i64, vp]

@@ -27,8 +27,11 @@ int grouped_check(const mpe_grouped_desc *d) {
 
 // ---- what the tiles are copied from --------------------------------------------------------------------------------------
 // A matrix of the call, and whether it is packed into the workspace first: a tile (256 lines) of it would span too much, or it
-// is masked (written once, read by both products: 4 096 x 64 f32 backward
-// 17.1 -> 15.7 us, 16 384 x 512 238 -> 165 us against a mask in the tiles' loads).
+// is masked and its readers do not apply the mask.  The larger tiles have no room for it; the small ones load and apply it once
+// per 64 columns of x, which pays while those are few (rows x k x n in groups, us, mask in the tiles / masked first):
+// f32 4 096 x 64 x 64 in 4 10.0 / 11.7, 32 768 x 64 x 64 in 8 24.8 / 28.9, 4 096 x 256 x 256 in 8 24.0 / 27.7, 1 024 x 512 x 512
+// in 4 30.8 / 31.2, 1 024 x 1 024 x 1 024 in 4 54 / 51, 16 384 x 512 x 512 in 16 188 / 165; fp16 5 003 x 333 x 517 in 7 38 / 34.
+constexpr int kMaskCols = 256;
 struct Matrix {
   const void *p, *mask;
   int64_t ld, ld_mask, lines, at;  // at: offset in the workspace, or -1
@@ -44,15 +47,17 @@ struct Workspace {
 
   int chunk() const { return 16 / size; }
   int64_t packed_ld(const Matrix &m) const { return (m.cols + chunk() - 1) / chunk() * chunk(); }
-  bool copyable(const Matrix &m) const {
-    return m.ld < (int64_t)kGroupedSpan / (256 * size) - 16;
-  }
+  bool copyable(int64_t ld) const { return ld < (int64_t)kGroupedSpan / (256 * size) - 16; }
   int64_t take(int64_t bytes) {
     const int64_t at = total;
     total += (bytes + 15) / 16 * 16;
     return at;
   }
-  void plan(Matrix &m) { m.at = m.lines > 0 && (m.mask || !copyable(m)) ? take(m.lines * packed_ld(m) * size) : -1; }
+  // masks: the kernel that reads m applies its mask
+  void plan(Matrix &m, bool masks = false) {
+    const bool as_it_is = copyable(m.ld) && (!m.mask || (masks && copyable(m.ld_mask)));
+    m.at = m.lines > 0 && !as_it_is ? take(m.lines * packed_ld(m) * size) : -1;
+  }
   // after the plan: the matrix as the kernels read it
   void place(Matrix &m, void *base) {
     if (m.at < 0) return;
@@ -63,6 +68,7 @@ struct Workspace {
     blocks += many;
     m.p = j.dst;
     m.ld = packed_ld(m);
+    m.mask = nullptr;
   }
   int run(int dtype, hipStream_t s) {
     if (jobs == 0) return MPE_OK;
@@ -117,33 +123,66 @@ int launch(const GroupedArgs &a, Tile tile, int64_t grid, hipStream_t s) {
     if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, MODE, 256, 256, 2, 4, 4, 4>), blocks, dim3(512), 0, s, a);
   } else if (sizeof(T) == 2 && tile == MIDDLE) {
     if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, MODE, 128, 128, 2, 2, 4, 4>), blocks, dim3(256), 0, s, a);
-  } else {
+  } else if constexpr (sizeof(T) == 2 || MODE == GROUPED_FWD) {  // an f32 backward is grouped_both_kernel's
     hipLaunchKernelGGL((grouped_kernel<T, MODE, 64, 64, 2, 2, 8, 2>), blocks, dim3(256), 0, s, a);
   }
   return (int)hipGetLastError();
 }
 
+// tiles over a.rows (forward, dx): groups (and the tail) with rows may each add a partial tile
+int64_t rows_grid(GroupedArgs &a, Tile tile, int64_t cols) {
+  a.tiles_j = (int)((cols + kTile[tile] - 1) / kTile[tile]);
+  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;
+  return (a.rows / kTile[tile] + most) * a.tiles_j;
+}
+Tile rows_tile(const mpe_grouped_desc *d, int64_t cols) { return pick_tile(d, d->rows / d->groups, cols, d->rows, 1); }
+
 template <typename T, int MODE>
 int launch_rows(GroupedArgs a, const mpe_grouped_desc *d, hipStream_t s) {
   const int64_t cols = MODE == GROUPED_FWD ? d->n : d->k;
-  const Tile tile = pick_tile(d, d->rows / d->groups, cols, d->rows, 1);
-  a.tiles_j = (int)((cols + kTile[tile] - 1) / kTile[tile]);
-  const int64_t most = a.groups + 1 < a.rows ? a.groups + 1 : a.rows;  // groups (and the tail) with rows: each may add a partial tile
-  return launch<T, MODE>(a, tile, (a.rows / kTile[tile] + most) * a.tiles_j, s);
+  const Tile tile = rows_tile(d, cols);
+  const int64_t grid = rows_grid(a, tile, cols);
+  return launch<T, MODE>(a, tile, grid, s);
 }
 
 template <typename T>
-int launch_dw(GroupedArgs a, const mpe_grouped_desc *d, hipStream_t s) {
-  const Tile tile = dw_tile(d);
-  a.tiles_i = (d->n + kTile[tile] - 1) / kTile[tile];
-  a.tiles_j = (d->k + kTile[tile] - 1) / kTile[tile];
-  a.splits = dw_splits(d);
-  const int rc = launch<T, GROUPED_DW>(a, tile, dw_tiles(d) * a.splits, s);
-  if (rc || a.splits == 1) return rc;
+int launch_join(const GroupedArgs &a, hipStream_t s) {
+  if (a.splits == 1) return MPE_OK;
   const int64_t cw = (int64_t)a.groups * a.n * a.k, cb = a.dbias ? (int64_t)a.groups * a.n : 0;
   hipLaunchKernelGGL(grouped_join_kernel<T>, dim3((unsigned)((cw + 1023) / 1024 + (cb + 1023) / 1024)), dim3(256), 0, s, a.part,
                      (T *)a.out, cw, a.part_bias, (T *)a.dbias, cb, a.splits);
   return (int)hipGetLastError();
+}
+
+// dx and dw: w.tiles_* and w.splits are set
+template <typename T>
+int launch_backward(GroupedArgs x, const GroupedArgs &w, const mpe_grouped_desc *d, hipStream_t s) {
+  const Tile tx = rows_tile(d, d->k), tw = dw_tile(d);
+  const int64_t nx = x.out ? rows_grid(x, tx, d->k) : 0, nw = w.out ? dw_tiles(d) * w.splits : 0;
+  if (nx + nw + 7 > kMaxGrid) return MPE_ERR_ARG;
+  int rc = MPE_OK;
+  if (tx == tw || nx == 0 || nw == 0) {
+    if (nx + nw > 0) {
+      const dim3 grid((unsigned)(nx + (nw + 7) / 8 * 8));
+      const Tile tile = nw ? tw : tx;
+      if (sizeof(T) == 2 && tile == LARGE) {
+        if constexpr (sizeof(T) == 2)
+          hipLaunchKernelGGL((grouped_both_kernel<T, 256, 256, 2, 4, 4, 4, false>), grid, dim3(512), 0, s, x, w, (int)nw);
+      } else if (sizeof(T) == 2 && tile == MIDDLE) {
+        if constexpr (sizeof(T) == 2)
+          hipLaunchKernelGGL((grouped_both_kernel<T, 128, 128, 2, 2, 4, 4, false>), grid, dim3(256), 0, s, x, w, (int)nw);
+      } else if (x.mask) {
+        hipLaunchKernelGGL((grouped_both_kernel<T, 64, 64, 2, 2, 8, 2, true>), grid, dim3(256), 0, s, x, w, (int)nw);
+      } else {
+        hipLaunchKernelGGL((grouped_both_kernel<T, 64, 64, 2, 2, 8, 2, false>), grid, dim3(256), 0, s, x, w, (int)nw);
+      }
+      rc = (int)hipGetLastError();
+    }
+  } else {
+    rc = launch<T, GROUPED_DW>(w, tw, nw, s);
+    if (!rc) rc = launch<T, GROUPED_DX>(x, tx, nx, s);
+  }
+  return rc || !w.out ? rc : launch_join<T>(w, s);
 }
 
 #define GROUPED_BY_TYPE(dtype, F, ...) \
@@ -178,13 +217,15 @@ struct Forward {
 struct Backward {
   Matrix d_, x, w;
   Workspace ws;
+  bool small;  // all tiles: one launch, which applies the mask itself
   int64_t part = 0, part_bias = 0;
   Backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, const void *px, int64_t ld_x,
            const void *pw, bool dx, bool dw)
-      : d_(rows_of(d, dy, ld_dy, d->n)), x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)} {
+      : d_(rows_of(d, dy, ld_dy, d->n)), x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)},
+        small((!dx || rows_tile(d, d->k) == SMALL) && (!dw || dw_tile(d) == SMALL)) {
     d_.mask = y;
     d_.ld_mask = ld_y;
-    if (dx || dw) ws.plan(d_);
+    if (dx || dw) ws.plan(d_, small && d->k <= kMaskCols);
     if (dw) ws.plan(x);
     if (dx) ws.plan(w);
     const int splits = dw_splits(d);
@@ -236,11 +277,11 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
   return GROUPED_BY_TYPE(d->dtype, launch_rows, , GROUPED_FWD>(a, d, s));
 }
 
-extern "C" int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, const void *x,
-                                                  int64_t ld_x, const void *weight, int with_dx, int with_dweight) {
+extern "C" int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
+                                                  const void *x, int64_t ld_x, const void *weight, int with_dx, int with_dweight) {
   if (const int rc = grouped_check(d)) return rc;
   if (with_dx < 0 || with_dx > 1 || with_dweight < 0 || with_dweight > 1) return MPE_ERR_ARG;
-  return Backward(d, dy, ld_dy, y, 0, x, ld_x, weight, with_dx, with_dweight).ws.total;
+  return Backward(d, dy, ld_dy, y, ld_y, x, ld_x, weight, with_dx, with_dweight).ws.total;
 }
 
 extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
@@ -266,20 +307,27 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   GroupedArgs a = base_args(d);
   a.a = b.d_.p;
   a.ld_a = b.d_.ld;
+  a.mask = b.d_.mask;
+  a.ld_mask = b.d_.ld_mask;
+  GroupedArgs gx = a, gw = a;
   if (dx && d->rows > 0) {
-    a.b = b.w.p;
-    a.ld_b = b.w.ld;
-    a.out = dx;
-    a.ld_out = ld_dx;
-    a.zero_tail = zero_tail;
-    if (const int rc = GROUPED_BY_TYPE(d->dtype, launch_rows, , GROUPED_DX>(a, d, s))) return rc;
+    gx.b = b.w.p;
+    gx.ld_b = b.w.ld;
+    gx.out = dx;
+    gx.ld_out = ld_dx;
+    gx.zero_tail = zero_tail;
   }
-  if (!dweight) return MPE_OK;
-  a.b = b.x.p;
-  a.ld_b = b.x.ld;
-  a.out = dweight;
-  a.dbias = dbias;
-  a.part = (float *)((char *)workspace + b.part);
-  a.part_bias = (float *)((char *)workspace + b.part_bias);
-  return GROUPED_BY_TYPE(d->dtype, launch_dw, >(a, d, s));
+  if (dweight) {
+    gw.b = b.x.p;
+    gw.ld_b = b.x.ld;
+    gw.out = dweight;
+    gw.dbias = dbias;
+    gw.part = (float *)((char *)workspace + b.part);
+    gw.part_bias = (float *)((char *)workspace + b.part_bias);
+    const int t = kTile[dw_tile(d)];
+    gw.tiles_i = (d->n + t - 1) / t;
+    gw.tiles_j = (d->k + t - 1) / t;
+    gw.splits = dw_splits(d);
+  }
+  return GROUPED_BY_TYPE(d->dtype, launch_backward, >(gx, gw, d, s));
 }

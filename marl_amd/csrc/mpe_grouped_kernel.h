@@ -22,12 +22,13 @@ enum GroupedMode { GROUPED_FWD = 0, GROUPED_DX = 1, GROUPED_DW = 2 };
 
 struct GroupedArgs {
   const void *a, *b;        // forward: x, weight; dx: d, weight; dw: d, x
+  const void *mask;         // dx, dw of the small tile: y, where d is dy times relu's mask (else NULL)
   const void *bias;         // forward: [G][N] or NULL
   void *out;                // forward: y; dx: dx; dw: dweight
   void *dbias;              // dw: [G][N] or NULL
   float *part, *part_bias;  // dw over splits: [S][G][N][K] and [S][G][N] partial sums
   const void *ends;
-  int64_t rows, ld_a, ld_b, ld_out;
+  int64_t rows, ld_a, ld_b, ld_mask, ld_out;
   int32_t groups, n, k, ends64, relu, zero_tail;
   int32_t tiles_i, tiles_j, splits;  // dw: tiles over n, over k, over rows; forward / dx: tiles_j only
 };
@@ -235,6 +236,7 @@ __device__ __forceinline__ void grouped_store4(T *p, f4v v, int valid) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) q.v[e] = (T)v[e];
     *reinterpret_cast<Quad<T> *>(p) = q;
+    asm volatile("");  // or the compiler shares the last element's store with the other branch: three stores for one
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -244,30 +246,38 @@ __device__ __forceinline__ void grouped_store4(T *p, f4v v, int valid) {
 
 // Workgroups are handed to the eight dies in turn: runs of 32 consecutive tiles (which share a weight or its rows) go to one
 // die's L2.  Not longer runs: the grid has a few tiles too many at its end, which must not all fall to one die.
-__device__ __forceinline__ int grouped_block() {
+// b: the workgroup's number among n, whose first one's number is a multiple of 8.
+__device__ __forceinline__ int grouped_block(int b, int n) {
   constexpr int kRun = 32;
-  const int b = blockIdx.x, n = gridDim.x;
   if (b >= n / (8 * kRun) * (8 * kRun)) return b;
   const int at = b / 8;
   return at / kRun * (8 * kRun) + b % 8 * kRun + at % kRun;
 }
 
-// STAGES buffers of KC chunks a row: while one is multiplied, STAGES - 1 are on their way.
-template <typename T, int MODE, int BM, int BN, int WM, int WN, int KC, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_kernel(GroupedArgs a) {
+// keeps the elements of v whose saved output is > 0 or NaN (relu's derivative: zero where y <= 0)
+template <typename T>
+__device__ __forceinline__ Chunk16<T> grouped_keep(Chunk16<T> v, const Chunk16<T> &y) {
+#pragma unroll
+  for (int e = 0; e < 16 / (int)sizeof(T); ++e) v.v[e] = (float)y.v[e] <= 0.0f ? T(0) : v.v[e];
+  return v;
+}
+// The tile kernel's LDS: STAGES buffers of KC chunks a row; while one is multiplied, STAGES - 1 are on their way.  Separate
+// arrays: the compiler then knows that a read of one does not wait for copies into another.
+#define GROUPED_STAGES(chunks, STAGES) \
+  __shared__ uint4 s0[chunks], s1[chunks], s2[(STAGES) == 4 ? (chunks) : 1], s3[(STAGES) == 4 ? (chunks) : 1]
+
+// One output tile: number `block` of a.tiles_* (and splits).  MASK: A times relu's mask, on its fragments.
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int KC, int STAGES, bool MASK>
+__device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, uint4 *s0, uint4 *s1, uint4 *s2, uint4 *s3) {
   constexpr int NT = 64 * WM * WN, KE = KC * 16 / (int)sizeof(T);
   constexpr int MI = BM / WM / 16, NJ = BN / WN / 16;
   constexpr bool EDGES = BM < 256;  // the large tile, short of registers, takes whole chunks only (n and k multiples of 8)
   using OpA = GroupedOperand<T, BM, KC, NT, MODE != GROUPED_DW>;
   using OpB = GroupedOperand<T, BN, KC, NT, MODE == GROUPED_FWD>;
-  // separate arrays: the compiler then knows that a read of one does not wait for copies into another
-  constexpr int kStage = (BM + BN) * KC;  // A's chunks, then B's
   static_assert(STAGES == 2 || STAGES == 4, "the loop below");
-  __shared__ uint4 s0[kStage], s1[kStage], s2[STAGES == 4 ? kStage : 1], s3[STAGES == 4 ? kStage : 1];
-  const T *pa = static_cast<const T *>(a.a), *pb = static_cast<const T *>(a.b);
+  const T *pa = static_cast<const T *>(a.a), *pb = static_cast<const T *>(a.b), *pm = static_cast<const T *>(a.mask);
 
   // ---- which tile ------------------------------------------------------------------------------------------------------
-  const int block = grouped_block();
   int g, tj = 0, split = 0;
   int64_t i0, i_end, j0, j_end, c0, c_end;  // output rows, output columns, contraction
   if (MODE == GROUPED_DW) {
@@ -312,18 +322,23 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   f4v acc[MI][NJ] = {};
   float sum[MI] = {};  // dbias: this lane's share of its rows' (n's) sums
-  OpA oa;
+  OpA oa, om;
   OpB ob;
   oa.aim(a.ld_a, i_end - i0, c_end - c0);
   ob.aim(a.ld_b, j_end - j0, c_end - c0);
+  if constexpr (MASK) om.aim(a.ld_mask, i_end - i0, c_end - c0);
   auto fetch = [&](int64_t c, uint4 *la) {
     const int64_t at = MODE == GROUPED_DW ? c * a.ld_a + i0 : i0 * a.ld_a + c;
     const int64_t bt = b0 + (MODE == GROUPED_FWD ? j0 * a.ld_b + c : c * a.ld_b + j0);
     oa.copy(la, pa + at, (end_a - at) * (int64_t)sizeof(T));
     ob.copy(la + BM * KC, pb + bt, (end_b - bt) * (int64_t)sizeof(T));
+    if constexpr (MASK) {
+      const int64_t mt = MODE == GROUPED_DW ? c * a.ld_mask + i0 : i0 * a.ld_mask + c;
+      om.copy(la + (BM + BN) * KC, pm + mt, ((a.rows - 1) * a.ld_mask + cols_a - mt) * (int64_t)sizeof(T));
+    }
   };
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
-  constexpr int kAhead = (STAGES - 2) * (OpA::N + OpB::N);  // copies of later stages that may still be under way
+  constexpr int kAhead = (STAGES - 2) * ((MASK ? 2 : 1) * OpA::N + OpB::N);  // copies of later stages that may still be under way
   auto step = [&](int64_t c, uint4 *la, uint4 *next) {
     uint4 *lb = la + BM * KC;
     // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
@@ -340,7 +355,12 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     for (int kk = 0; kk < KC / 4; ++kk) {
       uint4 fa[MI], fb[NJ];
 #pragma unroll
-      for (int m = 0; m < MI; ++m) fa[m] = OpA::frag(la, wi + m * 16, kk);
+      for (int m = 0; m < MI; ++m) {
+        fa[m] = OpA::frag(la, wi + m * 16, kk);
+        if constexpr (MASK)
+          fa[m] = __builtin_bit_cast(uint4, grouped_keep(__builtin_bit_cast(Chunk16<T>, fa[m]),
+                                                         __builtin_bit_cast(Chunk16<T>, OpA::frag(la + (BM + BN) * KC, wi + m * 16, kk))));
+      }
 #pragma unroll
       for (int n = 0; n < NJ; ++n) fb[n] = OpB::frag(lb, wj + n * 16, kk);
       // operands swapped: the result's rows are j, so a lane holds four neighbours of one output row
@@ -384,7 +404,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
     const int64_t jb = MODE == GROUPED_FWD ? last_b : cols_b - 1, cb = MODE == GROUPED_FWD ? cols_b - 1 : last_b;
     const bool cut_a = (cols_a & 1) && ia >= i0 && ia < i0 + BM && ia < i_end && ca >= c0 && ca < c_end;
     const bool cut_b = (cols_b & 1) && jb >= j0 && jb < j0 + BN && jb < j_end && cb >= c0 && cb < c_end;
-    const auto elem_a = [&](int64_t i, int64_t c) { return (float)pa[MODE == GROUPED_DW ? c * a.ld_a + i : i * a.ld_a + c]; };
+    const auto elem_a = [&](int64_t i, int64_t c) {
+      if (MASK && (float)pm[MODE == GROUPED_DW ? c * a.ld_mask + i : i * a.ld_mask + c] <= 0.0f) return 0.0f;
+      return (float)pa[MODE == GROUPED_DW ? c * a.ld_a + i : i * a.ld_a + c];
+    };
     const auto elem_b = [&](int64_t j, int64_t c) { return (float)pb[b0 + (MODE == GROUPED_FWD ? j * a.ld_b + c : c * a.ld_b + j)]; };
     if (cut_a || cut_b) {
 #pragma unroll
@@ -402,6 +425,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
       }
     }
   }
+  const bool whole = j0 + BN <= j_end;  // all columns exist
   const auto valid_of = [&](int n) { return j_end - j_lane - n * 16 >= 4 ? 4 : (int)(j_end - j_lane - n * 16); };
   if constexpr (MODE == GROUPED_FWD) {
     if (a.bias != nullptr && !tail) {  // all of it first: one wait
@@ -410,8 +434,15 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
 #pragma unroll
       for (int n = 0; n < NJ; ++n) {
         const int valid = valid_of(n);
+        if (whole || !EDGES) {
+          Quad<T> q{};
+          if (whole || valid == 4) q = *reinterpret_cast<const Quad<T> *>(b + n * 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bias[n][e] = e < valid ? (float)b[n * 16 + e] : 0.0f;
+          for (int e = 0; e < 4; ++e) bias[n][e] = (float)q.v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bias[n][e] = e < valid ? (float)b[n * 16 + e] : 0.0f;
+        }
       }
 #pragma unroll
       for (int m = 0; m < MI; ++m)
@@ -429,12 +460,21 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
   }
   const auto store = [&](auto *out, int64_t ld) {  // out: the array's row 0
     auto *at = out + (i0 + wi + (lane & 15)) * ld + j_lane;
-    const bool whole = i0 + BM <= i_end && j0 + BN <= j_end;  // no tests
+    if (whole && i0 + BM <= i_end) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NJ; ++n) grouped_store4(at + m * 16 * ld + n * 16, acc[m][n], 4);
+      return;
+    }
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      if (!whole && i0 + wi + m * 16 + (lane & 15) >= i_end) continue;
+      if (i0 + wi + m * 16 + (lane & 15) >= i_end) continue;
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) grouped_store4(at + m * 16 * ld + n * 16, acc[m][n], whole ? 4 : valid_of(n));
+      for (int n = 0; n < NJ; ++n) {
+        if (EDGES) grouped_store4(at + m * 16 * ld + n * 16, acc[m][n], valid_of(n));
+        else if (valid_of(n) == 4) grouped_store4(at + m * 16 * ld + n * 16, acc[m][n], 4);
+      }
     }
   };
   if constexpr (MODE == GROUPED_DW) {
@@ -446,14 +486,36 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
         v += __shfl_xor(v, 32);
         const int64_t i = i0 + wi + m * 16 + lane;
         if (lane >= 16 || i >= i_end) continue;
-        if (a.splits > 1) a.part_bias[part + i] = v;
+        if (EDGES && a.splits > 1) a.part_bias[part + i] = v;
         else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)v;
       }
     }
-    if (a.splits > 1) store(a.part + part * a.k, a.k);
+    if (EDGES && a.splits > 1) store(a.part + part * a.k, a.k);  // the large tile's sums are never split
     else store(static_cast<T *>(a.out) + (int64_t)g * a.n * a.k, a.k);
   } else {
     store(static_cast<T *>(a.out), a.ld_out);
+  }
+}
+
+template <typename T, int MODE, int BM, int BN, int WM, int WN, int KC, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_kernel(GroupedArgs a) {
+  GROUPED_STAGES((BM + BN) * KC, STAGES);
+  grouped_body<T, MODE, BM, BN, WM, WN, KC, STAGES, false>(a, grouped_block(blockIdx.x, gridDim.x), s0, s1, s2, s3);
+}
+
+// A backward pass in one launch: the first dw_tiles workgroups make dw's tiles, those behind them dx's; with MASK both mask what
+// they load.  One launch also fills the chip where the first product's last tiles leave it empty, and dw's, which run longest,
+// come first: 65 536 x 226 x 64 f32 in 64 groups, masked: two products in two launches 85 us, dx first 92, dw first 70;
+// 4 096 x 64 x 64 in 4 groups: mask, dx, dw and join as four launches 16.7 us, this and the join 9.6;
+// 16 384 x 1 024 x 1 024 bf16 in 16 unlike groups, without the mask: 116 us as two launches, 101 as one.
+template <typename T, int BM, int BN, int WM, int WN, int KC, int STAGES, bool MASK>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_both_kernel(GroupedArgs dx, GroupedArgs dw, int dw_tiles) {
+  GROUPED_STAGES((BM + BN + (MASK ? BM : 0)) * KC, STAGES);
+  const int b = (int)blockIdx.x, first = (dw_tiles + 7) & ~7;
+  if (b >= first) {
+    grouped_body<T, GROUPED_DX, BM, BN, WM, WN, KC, STAGES, MASK>(dx, grouped_block(b - first, (int)gridDim.x - first), s0, s1, s2, s3);
+  } else if (b < dw_tiles) {
+    grouped_body<T, GROUPED_DW, BM, BN, WM, WN, KC, STAGES, MASK>(dw, grouped_block(b, dw_tiles), s0, s1, s2, s3);
   }
 }
 
@@ -462,13 +524,6 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_ke
 struct GroupedPack { const void *src, *mask; void *dst; int64_t ld, ld_mask, lines; int32_t cols, blocks; };
 struct GroupedPacks { GroupedPack job[3]; };
 
-// keeps the elements of v whose saved output is > 0 or NaN (relu's derivative: zero where y <= 0)
-template <typename T>
-__device__ __forceinline__ Chunk16<T> grouped_keep(Chunk16<T> v, const Chunk16<T> &y) {
-#pragma unroll
-  for (int e = 0; e < 16 / (int)sizeof(T); ++e) v.v[e] = (float)y.v[e] <= 0.0f ? T(0) : v.v[e];
-  return v;
-}
 // the chunk at element off, valid of it kept; end: elements of the whole matrix (a chunk may reach into the next line)
 template <typename T>
 __device__ __forceinline__ Chunk16<T> grouped_chunk(const T *p, int64_t off, int valid, int64_t end) {

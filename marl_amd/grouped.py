@@ -193,7 +193,7 @@ def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dw
         dw = x.new_empty(weight.shape)
         db = x.new_empty(weight.shape[:2]) if need_dbias else None
     pg, py, px, pw = grad.data_ptr(), _hip.ptr(y), x.data_ptr(), weight.data_ptr()
-    need = _hip.lib.mpe_grouped_backward_workspace(desc, pg, ld_g, py, px, ld_x, pw, need_dx, both)
+    need = _hip.lib.mpe_grouped_backward_workspace(desc, pg, ld_g, py, ld_y, px, ld_x, pw, need_dx, both)
     if need:
         ws = _scratch(x, need)
     _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear_backward, desc, pg, ld_g, py, ld_y, px, ld_x, pw, _hip.ptr(dx), k, 1, _hip.ptr(dw), _hip.ptr(db), _hip.ptr(ws), need),

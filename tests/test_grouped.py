@@ -40,7 +40,7 @@ def test_c_abi_refuses_bad_descriptors(change, code):
     d, p = _desc(**change), 1 << 20
     assert _hip.lib.mpe_grouped_linear(d, p, 3, p, None, p, 5, 0, 0, None, 0, None) == code
     assert _hip.lib.mpe_grouped_linear_workspace(d, p, 3, p) == code
-    assert _hip.lib.mpe_grouped_backward_workspace(d, p, 5, None, p, 3, p, 1, 1) == code
+    assert _hip.lib.mpe_grouped_backward_workspace(d, p, 5, None, 0, p, 3, p, 1, 1) == code
     assert _hip.lib.mpe_grouped_linear_backward(d, p, 5, None, 0, p, 3, p, p, 3, 0, p, p, None, 0, None) == code
 
 
@@ -64,8 +64,10 @@ def test_c_abi_refuses_bad_arrays():
                      (dict(db=p + 2), -4), (dict(ws=p + 8), -4)):
         assert back(**kw) == code, kw
     def size(desc=d, y=None, dx=1, dw=1):
-        return L.mpe_grouped_backward_workspace(desc, p, 5, y, p, 3, p, dx, dw)
-    assert size(dx=2) == -6 and size(dw=-1) == -6 and size() == 0 and size(y=p) == 4 * 8 * 4   # y: dy masked, in whole chunks
+        return L.mpe_grouped_backward_workspace(desc, p, 5, y, 5, p, 3, p, dx, dw)
+    assert size(dx=2) == -6 and size(dw=-1) == -6 and size() == 0 and size(y=p) == 0
+    wide = _desc(dtype=_hip.BF16, rows=1 << 14, n=1001, k=1024)    # y beside large products: dy masked, in rows of whole chunks
+    assert size(wide, y=p, dw=0) == (1 << 14) * 1008 * 2
     big = _desc(rows=1 << 20)                                     # rows split over workgroups: partial sums need an array
     need = size(big)
     assert need > 0 and size(big, dw=0) == 0
@@ -349,6 +351,14 @@ def test_rows_that_lie_far_apart_are_packed_first():
     assert torch.equal(grouped.grouped_linear(xs, w, ends, bias=b), grouped.grouped_linear(x, w, ends, bias=b))
     for got, want in zip(grouped.grouped_linear_backward(gs, xs, w, ends), grouped.grouped_linear_backward(grad, x, w, ends)):
         assert torch.equal(got, want)
+    y = torch.randn(7, n, device='cuda')
+    ys, near = far[:, 9000:9000 + n], torch.full((7, n + 5), float('nan'), device='cuda')[:, 2:2 + n]
+    ys.copy_(y)
+    near.copy_(y)
+    plain = grouped.grouped_linear_backward(grad, x, w, ends, y=y)      # masked as they are read: y with strides of its own
+    for gg, yy in ((grad, near), (grad, ys), (gs, y), (gs, ys)):
+        for got, want in zip(grouped.grouped_linear_backward(gg, xs, w, ends, y=yy), plain):
+            assert torch.equal(got, want)
 
 
 @pytest.mark.gpu

@@ -15,6 +15,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace mpe {
 
@@ -90,27 +91,36 @@ __device__ __forceinline__ void grouped_rows_of(const GroupedArgs &a, int g, int
   r1 = uniform(hi < a.rows ? hi : a.rows);
 }
 
+// Lane l's rows [s, e) of group base + l; `before`: the running maximum of the ends before this batch, updated.
+__device__ __forceinline__ void grouped_batch(const GroupedArgs &a, int base, int64_t &before, int64_t &s, int64_t &e) {
+  const int lane = threadIdx.x & 63, i = base + lane;
+  e = i < a.groups ? grouped_end(a, i) : a.rows;  // the last, pseudo, group ends with the rows
+  e = e < 0 ? 0 : (e < a.rows ? e : a.rows);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(e, d);
+    if (lane >= d && o > e) e = o;
+  }
+  e = e > before ? e : before;
+  s = __shfl_up(e, 1);
+  if (lane == 0) s = before;
+  before = __shfl(e, 63);
+}
+
 // The group of row tile `tile` (tiles of BM rows, counted group by group) and its rows [r0, r1); behind the last group's
 // tiles come those of the rows that belong to none (g == groups).  false: no such tile.
+// Large tiles are counted in three turns: those with all their rows, those with more than half, the others.  The last ones take
+// half as long and fill the chip's last round (dx of 16 384 x 1 024 x 1 024 bf16 in 16 unlike groups: 64 us in order, 55).
 template <int BM>
 __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int &g, int64_t &r0, int64_t &r1) {
+  constexpr bool kWholeFirst = BM == 256;
   const int lane = threadIdx.x & 63;
-  int64_t before = 0;   // running maximum of the ends before this batch of 64 groups
-  int tiles_before = 0;
+  int64_t before = 0, s, e;
+  int tiles_before = 0, more = 0, less = 0;
   for (int base = 0; base <= a.groups; base += 64) {
-    const int i = base + lane;
-    int64_t e = i < a.groups ? grouped_end(a, i) : a.rows;  // the last, pseudo, group ends with the rows
-    e = e < 0 ? 0 : (e < a.rows ? e : a.rows);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(e, d);
-      if (lane >= d && o > e) e = o;
-    }
-    e = e > before ? e : before;
-    int64_t s = __shfl_up(e, 1);
-    if (lane == 0) s = before;
-    int sum = (int)((e - s + BM - 1) / BM);
-    const int mine = sum;
+    grouped_batch(a, base, before, s, e);
+    const int mine = (int)((e - s + (kWholeFirst ? 0 : BM - 1)) / BM);
+    int sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(sum, d);
@@ -126,8 +136,32 @@ __device__ __forceinline__ bool grouped_tile(const GroupedArgs &a, int tile, int
       r1 = last < r0 + BM ? last : r0 + BM;
       return true;
     }
-    before = __shfl(e, 63);
     tiles_before = __shfl(sum, 63);
+    if (kWholeFirst) {
+      const int rest = (int)((e - s) % BM);
+      more += __popcll(__ballot(rest > BM / 2));
+      less += __popcll(__ballot(rest > 0 && rest <= BM / 2));
+    }
+  }
+  if (!kWholeFirst) return false;
+  int at = uniform(tile - tiles_before);
+  const bool half = at >= more;
+  if (half) at -= more;
+  if (half && at >= less) return false;
+  before = 0;
+  for (int base = 0; base <= a.groups; base += 64) {
+    grouped_batch(a, base, before, s, e);
+    const int rest = (int)((e - s) % BM);
+    const uint64_t any = __ballot(half ? rest > 0 && rest <= BM / 2 : rest > BM / 2);
+    const int below = __popcll(any & ((1ull << lane) - 1)), count = __popcll(any);
+    if (at < count) {
+      const int w = __ffsll((unsigned long long)__ballot((any >> lane & 1) && below == at)) - 1;
+      g = base + w;
+      r1 = uniform(__shfl(e, w));
+      r0 = r1 - uniform(__shfl(rest, w));
+      return true;
+    }
+    at -= count;
   }
   return false;
 }
@@ -339,49 +373,58 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
   };
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
   constexpr int kAhead = (STAGES - 2) * ((MASK ? 2 : 1) * OpA::N + OpB::N);  // copies of later stages that may still be under way
-  auto step = [&](int64_t c, uint4 *la, uint4 *next) {
-    uint4 *lb = la + BM * KC;
-    // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
+  // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
+  auto landed = [&](int64_t c, uint4 *la) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
     if (EDGES && MODE != GROUPED_DW && c_end - c < KE && (c_end - c) % OpA::CE != 0) {
       oa.trim(la, STAGES - 1);
-      ob.trim(lb, STAGES - 1);
+      ob.trim(la + BM * KC, STAGES - 1);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    fetch(c + (STAGES - 1) * KE, next);  // past the end: zeros
+  };
+  auto read = [&](uint4 *la, int kk, uint4 (&fa)[MI], uint4 (&fb)[NJ]) {
 #pragma unroll
-    for (int kk = 0; kk < KC / 4; ++kk) {
-      uint4 fa[MI], fb[NJ];
+    for (int m = 0; m < MI; ++m) {
+      fa[m] = OpA::frag(la, wi + m * 16, kk);
+      if constexpr (MASK)
+        fa[m] = __builtin_bit_cast(uint4, grouped_keep(__builtin_bit_cast(Chunk16<T>, fa[m]),
+                                                       __builtin_bit_cast(Chunk16<T>, OpA::frag(la + (BM + BN) * KC, wi + m * 16, kk))));
+    }
+#pragma unroll
+    for (int n = 0; n < NJ; ++n) fb[n] = OpB::frag(la + BM * KC, wj + n * 16, kk);
+  };
+  auto multiply = [&](const uint4 (&fa)[MI], const uint4 (&fb)[NJ]) {
+    // operands swapped: the result's rows are j, so a lane holds four neighbours of one output row
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+      for (int n = 0; n < NJ; ++n) acc[m][n] = GroupedType<T>::mma(fb[n], fa[m], acc[m][n]);
+    if (with_bias) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
-        fa[m] = OpA::frag(la, wi + m * 16, kk);
-        if constexpr (MASK)
-          fa[m] = __builtin_bit_cast(uint4, grouped_keep(__builtin_bit_cast(Chunk16<T>, fa[m]),
-                                                         __builtin_bit_cast(Chunk16<T>, OpA::frag(la + (BM + BN) * KC, wi + m * 16, kk))));
-      }
+        const Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, fa[m]);
 #pragma unroll
-      for (int n = 0; n < NJ; ++n) fb[n] = OpB::frag(lb, wj + n * 16, kk);
-      // operands swapped: the result's rows are j, so a lane holds four neighbours of one output row
-#pragma unroll
-      for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NJ; ++n) acc[m][n] = GroupedType<T>::mma(fb[n], fa[m], acc[m][n]);
-      if (with_bias) {
-#pragma unroll
-        for (int m = 0; m < MI; ++m) {
-          const Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, fa[m]);
-#pragma unroll
-          for (int e = 0; e < OpA::CE; ++e) sum[m] += (float)c.v[e];
-        }
+        for (int e = 0; e < OpA::CE; ++e) sum[m] += (float)c.v[e];
       }
     }
   };
-  if (c0 < c_end) {
-    fetch(c0, s0);
-    if constexpr (STAGES == 4) fetch(c0 + KE, s1), fetch(c0 + 2 * KE, s2);
-    for (int64_t c = c0; c < c_end; c += STAGES * KE) {  // steps past the end multiply zeros
+  // stages past the end are zeros: fetched and multiplied like the others
+  auto steps = [&](auto works) {
+    auto step = [&](int64_t c, uint4 *la, uint4 *next) {
+      landed(c, la);
+      fetch(c + (STAGES - 1) * KE, next);
+      if constexpr (decltype(works)::value) {
+#pragma unroll
+        for (int kk = 0; kk < KC / 4; ++kk) {
+          uint4 fa[MI], fb[NJ];
+          read(la, kk, fa, fb);
+          multiply(fa, fb);
+        }
+      }
+    };
+    for (int64_t c = c0; c < c_end; c += STAGES * KE) {
       if constexpr (STAGES == 2) {
         step(c, s0, s1);
         step(c + KE, s1, s0);
@@ -392,6 +435,14 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
         step(c + 3 * KE, s3, s2);
       }
     }
+  };
+  if (c0 < c_end) {
+    fetch(c0, s0);
+    if constexpr (STAGES == 4) fetch(c0 + KE, s1), fetch(c0 + 2 * KE, s2);
+    // a wavefront of a large tile whose rows or columns do not exist only copies: its neighbour on the matrix unit goes on alone
+    if (BM < 256 || (i0 + wi < i_end && j0 + wj < j_end)) steps(std::true_type());
+    else steps(std::false_type());
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the tile
   }
 
   // ---- epilogue: lane holds output row i0 + wi + 16 m + lane % 16, columns j0 + wj + 16 n + 4 (lane / 16) .. + 4 ----------

@@ -168,7 +168,6 @@ def grouped_linear(x, weight, ends, bias=None, relu=False, out=None):
     return _forward(x, weight, ends, bias, bool(relu), out)
 
 
-@torch.no_grad()
 def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dweight=True, need_dbias=True):
     """``(dx, dweight, dbias)`` of ``grouped_linear`` for the gradient ``grad`` ``[rows, n]`` of its result; ``y``: the
     result itself where it was made with ``relu=True`` (``grad`` counts where ``y`` is not <= 0).  An entry that is not needed

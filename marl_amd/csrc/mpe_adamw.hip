@@ -28,7 +28,7 @@ int tensors_check(int n, const mpe_adamw_tensor *t, int dtype, int state_bits, i
         bad_align(t[i].exp_avg_sq, 16) || bad_align(t[i].exp_avg_base, 2) || bad_align(t[i].exp_avg_sq_base, 2))
       return MPE_ERR_ALIGN;
     *items += items_of(t[i].count);
-    if (*items > 0x7fffffff) return MPE_ERR_ARG;
+    if (*items > 0xffffff) return MPE_ERR_ARG;  // a launch has less than 2^32 threads
   }
   return MPE_OK;
 }
@@ -153,7 +153,7 @@ extern "C" int mpe_adamw_moments(const void *exp_avg, const void *exp_avg_base, 
       bad_align(out, size) || bad_align(out_sq, size))
     return MPE_ERR_ALIGN;
   const int64_t grid = (count / 8 + 255) / 256;
-  if (grid > 0x7fffffff) return MPE_ERR_ARG;
+  if (grid > 0xffffff) return MPE_ERR_ARG;
   const AdamMoments a = {{out ? (const uint8_t *)exp_avg : nullptr, out_sq ? (const uint8_t *)exp_avg_sq : nullptr},
                          {(const int16_t *)exp_avg_base, (const int16_t *)exp_avg_sq_base},
                          {out, out_sq}};

@@ -84,6 +84,8 @@ class _Plan(object):
             if not t.is_contiguous() or t.dtype != self.dtype or t.device != self.device:
                 raise ValueError('AdamW: parameters and targets are contiguous and keep their type and device')
         n = len(self.params)
+        if any(t.numel() != self.counts[j % n] for j, t in enumerate(self.params + (self.targets or []))):
+            raise ValueError('AdamW: parameters and targets keep their size')
         self.table = (_hip.AdamTensor * n)()
         for j, p in enumerate(self.params):
             o = self.first[j]
@@ -203,7 +205,7 @@ class AdamW(torch.optim.Optimizer):
     # -- the step ----------------------------------------------------------------------------------------------------------
     def _gradients(self, plan):
         """Fills the plan's pointers; returns what must outlive the launch.  (torch sees to it that a gradient has its
-        parameter's type, device and shape.)"""
+        parameter's type, device and shape when it is set; the parameter may have shrunk before.)"""
         grads = [p.grad for p in plan.params]
         try:
             plain = all(map(torch.Tensor.is_contiguous, grads))
@@ -211,9 +213,13 @@ class AdamW(torch.optim.Optimizer):
             plain = False
         if not plain:
             grads = [None if g is None else g.contiguous() for g in grads]
-            plan.grads[:] = [None if g is None else g.data_ptr() for g in grads]
+            sizes = [c if g is None else g.numel() for g, c in zip(grads, plan.counts)]
+            pointers = [None if g is None else g.data_ptr() for g in grads]
         else:
-            plan.grads[:] = list(map(torch.Tensor.data_ptr, grads))
+            sizes, pointers = list(map(torch.Tensor.numel, grads)), list(map(torch.Tensor.data_ptr, grads))
+        if sizes != plan.counts:
+            raise ValueError('AdamW: a gradient is not of the size that its parameter had')
+        plan.grads[:] = pointers
         return grads
 
     @torch.no_grad()
@@ -223,6 +229,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if not self._capturable and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('AdamW: step() is recorded with capturable=True only (every replay is one more step)')
         index0 = 0
         for i, (group, plan) in enumerate(zip(self.param_groups, self._plans)):
             self._check_group(group)
@@ -232,10 +240,9 @@ class AdamW(torch.optim.Optimizer):
                 plan.build()
             keep = self._gradients(plan)
             clock = self._clocks[i]
-            args = _hip.AdamArgs(lr=group['lr'], beta1=group['betas'][0], beta2=group['betas'][1], eps=group['eps'],
-                                 weight_decay=group['weight_decay'], max_norm=group['max_norm'] or 0.0, polyak=group['polyak'],
-                                 step=group['step'] + 1, clock=_hip.ptr(clock), seed=self._seed, index0=index0,
-                                 dtype=_DTYPES[plan.dtype], state_bits=self._bits)
+            args = _hip.AdamArgs(group['lr'], *group['betas'], group['eps'], group['weight_decay'], group['max_norm'] or 0.0,
+                                 group['polyak'], group['step'] + 1, _hip.ptr(clock), self._seed, index0, _DTYPES[plan.dtype],
+                                 self._bits)
             _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_step, args, len(plan.params), plan.table,
                                    plan.plan_ptr, plan.grads), 'mpe_adamw_step')
             del keep
@@ -269,6 +276,9 @@ class AdamW(torch.optim.Optimizer):
                                    m.data_ptr(), v.data_ptr(), m.numel(), _DTYPES[dtype]), 'mpe_adamw_moments')
             out.append((m, v))
         return out
+
+    def __getstate__(self):
+        raise TypeError('AdamW is not copied or pickled: build another one and load this one\'s state_dict()')
 
     def state_dict(self):
         for i in range(len(self._plans)):

@@ -1,7 +1,9 @@
 """marl_amd.optim.AdamW: one step over many tensors against the formulas in 64 bits, and its 8-bit moments against a
 restatement in numpy's float32, bit for bit."""
+import copy
 import ctypes as C
 import math
+import pickle
 
 import numpy as np
 import pytest
@@ -43,6 +45,8 @@ def _table(**kw):
 def test_c_abi_refuses_bad_arguments():
     """Nothing is launched: the pointers are never read."""
     L, p, inf, nan = _hip.lib, 1 << 20, float('inf'), float('nan')
+    assert L.mpe_adamw_plan(1, _table(count=1 << 37), _hip.F32, 32, None, 0) == -6     # more work items than a launch may have
+    assert L.mpe_adamw_moments(p, p, p, p, p, p, 1 << 36, _hip.F32, None) == -6
     grads = (C.c_void_p * 1)(p)
     for change, code in ((dict(lr=-1.0), -6), (dict(lr=nan), -6), (dict(lr=inf), -6), (dict(beta1=1.0), -6), (dict(beta2=-0.1), -6),
                          (dict(eps=-1.0), -6), (dict(eps=nan), -6), (dict(weight_decay=-1.0), -6), (dict(polyak=1.1), -6),
@@ -433,6 +437,48 @@ def test_groups_streams_versions_and_moved_parameters():
     a.data = torch.ones(600, device='cuda')[::2]
     with pytest.raises(ValueError):
         opt.step()
+
+
+@pytest.mark.gpu
+def test_parameters_that_change_size_are_refused():
+    """Host checks: no kernel reads behind a parameter, gradient or target that is smaller than it was."""
+    def fresh():
+        p, t = torch.nn.Parameter(torch.ones(40, device='cuda')), torch.ones(40, device='cuda')
+        p.grad = torch.ones_like(p)
+        return p, t, optim.AdamW([p], targets=[t])
+    p, t, opt = fresh()
+    p.data = p.data[:10]                                               # the same address
+    with pytest.raises(RuntimeError):                                  # torch's own check
+        p.grad = torch.ones(40, device='cuda')
+    p.grad = torch.ones(10, device='cuda')
+    with pytest.raises(ValueError):
+        opt.step()
+    p, t, opt = fresh()
+    p.data = torch.ones(10, device='cuda')
+    with pytest.raises(ValueError):
+        opt.step()
+    p, t, opt = fresh()
+    t.data = torch.ones(10, device='cuda')
+    with pytest.raises(ValueError):
+        opt.step()
+    assert (p == 1).all() and opt.step_count == 0
+
+
+@pytest.mark.gpu
+def test_recording_without_capturable_and_copies_are_refused():
+    p = torch.nn.Parameter(torch.ones(40, device='cuda'))
+    p.grad = torch.ones_like(p)
+    opt = optim.AdamW([p])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode='thread_local'):
+        with pytest.raises(RuntimeError):
+            opt.step()
+        p.grad.mul_(1.0)
+    torch.cuda.synchronize()
+    assert (p == 1).all() and opt.step_count == 0
+    for copies in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError):
+            copies(opt)
 
 
 @pytest.mark.gpu

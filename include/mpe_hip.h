@@ -569,7 +569,8 @@ int mpe_env_step_stats_static(const mpe_scenario_desc *desc, int64_t B, int64_t 
  *                          same inputs give the same bits
  * ends is a device array of int32 (ends64 = 0) or int64 and is read by the kernel as its running maximum clamped to
  * [0, rows].  Rows behind the last group: untouched, or zeros with zero_tail = 1.  ld_* are row strides in elements, inner
- * stride 1, any alignment of an element.  dtype is of all float arrays.  1 <= groups <= 1024; n and k up to 2^20, rows and n * k below 2^31.
+ * stride 1, any alignment of an element.  dtype is of all float arrays.  1 <= groups <= 1024; n and k up to 2^20, rows and n * k below 2^31;
+ * a call whose results are more than 2^23 - 8 tiles (64 x 64 and larger, a group's last one may be partial) is refused.
  * mpe_grouped_linear_workspace / mpe_grouped_backward_workspace: bytes that a call with these arrays needs (>= 0, or
  * MPE_ERR_*; no memory is read); the array is scratch of that call, 16-byte aligned; calls that may overlap (other streams,
  * concurrent graph replays) need one each.  What needs scratch: y beside large products, rows that lie 2^20 elements or more

@@ -9,7 +9,7 @@ using namespace mpe;
 namespace {
 
 constexpr int kMaxGroups = 1024, kMaxWidth = 1 << 20;
-constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int64_t kMaxGrid = (1 << 23) - 1;  // workgroups: a launch has less than 2^32 threads, a workgroup up to 512
 static_assert((int64_t)kMaxWidth * 4 * 256 < (int64_t)kGroupedSpan, "a tile of packed rows spans less than a copy may reach");
 
 int dtype_size(int dtype) { return dtype == MPE_F32 ? 4 : 2; }

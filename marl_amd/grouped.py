@@ -10,7 +10,7 @@ learners evaluate one network at a time, maddpg/maddpg/trainer/maddpg.py:161-196
 launch follows what the tensor holds at replay and nothing is copied to the host; whatever it holds, it is read as its
 running maximum clamped to ``[0, rows]``.  Groups may be empty.  float32, bfloat16 and float16, all arrays alike;
 sums are in 32 bits, each result is rounded once.  1 <= groups <= 1024; n and k up to 2**20, rows and n * k
-below 2**31.
+below 2**31; more than 2**23 - 8 tiles of 64 x 64 results are refused.
 
 Rows of ``x`` may have any stride; an ``x`` whose columns are not adjacent is copied first (also a ``weight`` or ``bias``
 that is not contiguous).  ``grouped_linear`` is differentiable (once) in ``x``, ``weight`` and ``bias``;

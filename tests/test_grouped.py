@@ -79,6 +79,9 @@ def test_c_abi_refuses_bad_arrays():
     assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, None, need, None) == -1
     assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, p, need - 1, None) == -7
     assert L.mpe_grouped_linear(d, p, far, p, None, p, 5, 0, 0, p + 8, need, None) == -4
+    many = _desc(rows=(1 << 31) - 1, n=64, k=16)                  # more tiles than one launch may have
+    assert L.mpe_grouped_linear(many, p, 16, p, None, p, 64, 0, 0, None, 0, None) == -6
+    assert L.mpe_grouped_linear_backward(many, p, 64, None, 0, p, 16, p, p, 16, 0, None, None, None, 0, None) == -6
     assert C.sizeof(_hip.GroupedDesc) == 40
 
 

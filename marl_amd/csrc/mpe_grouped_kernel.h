@@ -355,7 +355,11 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   f4v acc[MI][NJ] = {};
-  float sum[MI] = {};  // dbias: this lane's share of its rows' (n's) sums
+  // dbias: this lane's share of its rows' (n's) sums; the wavefronts of the same rows take kSums of their MI tiles of 16 rows each
+  constexpr int kSums = MI / WN;
+  static_assert(MI % WN == 0, "");
+  float sum[kSums] = {};
+  const int wn = wave % WN;
   OpA oa, om;
   OpB ob;
   oa.aim(a.ld_a, i_end - i0, c_end - c0);
@@ -371,7 +375,7 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
       om.copy(la + (BM + BN) * KC, pm + mt, ((a.rows - 1) * a.ld_mask + cols_a - mt) * (int64_t)sizeof(T));
     }
   };
-  const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0 && wj == 0;
+  const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0;
   constexpr int kAhead = (STAGES - 2) * ((MASK ? 2 : 1) * OpA::N + OpB::N);  // copies of later stages that may still be under way
   // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
   auto landed = [&](int64_t c, uint4 *la) {
@@ -403,13 +407,23 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
       for (int n = 0; n < NJ; ++n) acc[m][n] = GroupedType<T>::mma(fb[n], fa[m], acc[m][n]);
     if (with_bias) {
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, fa[m]);
+      for (int m = 0; m < kSums; ++m) {
+        uint4 f = fa[m];
+#pragma unroll
+        for (int w = 1; w < WN; ++w) {  // selects: an index that is not constant would put the fragments into memory
+          const uint4 o = fa[w * kSums + m];
+          f = uint4{wn == w ? o.x : f.x, wn == w ? o.y : f.y, wn == w ? o.z : f.z, wn == w ? o.w : f.w};
+        }
+        const Chunk16<T> c = __builtin_bit_cast(Chunk16<T>, f);
 #pragma unroll
         for (int e = 0; e < OpA::CE; ++e) sum[m] += (float)c.v[e];
       }
     }
   };
+  // Two halves of the wavefronts, one of each on every matrix unit, half a step apart: while one half reads its fragments the other
+  // multiplies.  32 768 x 2 048 x 2 048 bf16 in 32 unlike groups: 327 us, all in step 338; dx 278 / 275, dweight 331 / 308 of
+  // 32 768 x 2 048 x 2 048 in 8 (their transposing reads need more registers): there in step.
+  constexpr bool HALVES = BM == 256 && MODE == GROUPED_FWD;
   // stages past the end are zeros: fetched and multiplied like the others
   auto steps = [&](auto works) {
     auto step = [&](int64_t c, uint4 *la, uint4 *next) {
@@ -424,15 +438,45 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
         }
       }
     };
-    for (int64_t c = c0; c < c_end; c += STAGES * KE) {
-      if constexpr (STAGES == 2) {
-        step(c, s0, s1);
-        step(c + KE, s1, s0);
-      } else {
-        step(c, s0, s3);
-        step(c + KE, s1, s0);
-        step(c + 2 * KE, s2, s1);
-        step(c + 3 * KE, s3, s2);
+    if constexpr (HALVES) {
+      static_assert(!HALVES || (STAGES == 4 && KC == 4 && WM * WN == 8), "one fragment a stage, two wavefronts a matrix unit");
+      const bool late = wave >= 4;
+      auto turn = [&](int64_t c, uint4 *la, uint4 *free) {
+        uint4 fa[MI], fb[NJ];
+        fetch(c + 3 * KE, free);  // its last reads ended before the last barrier
+        if constexpr (decltype(works)::value) read(la, 0, fa, fb);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kAhead) : "memory");  // the next stage has landed; the reads are done
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (decltype(works)::value) {
+          __builtin_amdgcn_s_setprio(1);
+          multiply(fa, fb);
+          __builtin_amdgcn_s_setprio(0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      };
+      landed(c0, s0);
+      if (late) __builtin_amdgcn_s_barrier();
+      for (int64_t c = c0; c < c_end; c += 4 * KE) {
+        turn(c, s0, s3);
+        turn(c + KE, s1, s0);
+        turn(c + 2 * KE, s2, s1);
+        turn(c + 3 * KE, s3, s2);
+      }
+      if (!late) __builtin_amdgcn_s_barrier();
+    } else {
+      for (int64_t c = c0; c < c_end; c += STAGES * KE) {
+        if constexpr (STAGES == 2) {
+          step(c, s0, s1);
+          step(c + KE, s1, s0);
+        } else {
+          step(c, s0, s3);
+          step(c + KE, s1, s0);
+          step(c + 2 * KE, s2, s1);
+          step(c + 3 * KE, s3, s2);
+        }
       }
     }
   };
@@ -464,7 +508,7 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
         const int64_t i = i0 + wi + m * 16 + (lane & 15);
-        if (cut_a && i == ia && with_bias && lane < 16) sum[m] += elem_a(ia, ca);
+        if (cut_a && i == ia && with_bias && m / kSums == wn && lane < 16) sum[m % kSums] += elem_a(ia, ca);
 #pragma unroll
         for (int n = 0; n < NJ; ++n)
 #pragma unroll
@@ -532,10 +576,10 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
     const int64_t part = ((int64_t)split * a.groups + g) * a.n;
     if (with_bias) {
 #pragma unroll
-      for (int m = 0; m < MI; ++m) {
+      for (int m = 0; m < kSums; ++m) {
         float v = sum[m] + __shfl_xor(sum[m], 16);  // lanes l, l + 16, .. hold the same row's other c's
         v += __shfl_xor(v, 32);
-        const int64_t i = i0 + wi + m * 16 + lane;
+        const int64_t i = i0 + wi + (wn * kSums + m) * 16 + lane;
         if (lane >= 16 || i >= i_end) continue;
         if (EDGES && a.splits > 1) a.part_bias[part + i] = v;
         else static_cast<T *>(a.dbias)[(int64_t)g * a.n + i] = (T)v;

@@ -88,8 +88,10 @@ constexpr int kTile[3] = {64, 128, 256};
 
 // A 16-bit product is bound by what the tiles read per matrix instruction: the largest tile that still leaves every CU a
 // workgroup and does not mostly overhang its group's rows.  f32 matrix instructions are 16 times slower: small tiles.
-// mean_rows: of a group; rows: of all; others: independent products.  The large tile has no registers for n or k that end
-// inside a chunk (with them 32 768 rows 4 096 -> 2 048 take 679 us instead of 510).
+// mean_rows: of a group; rows: of all; others: independent products.
+// bf16 forward, us (small / middle / large, rows x k x n in groups): 4 096 x 512 x 512 in 16 8.6 / 11.1 / 22, 8 192 x 1 024 x 1 024 in
+// 16 37 / 28 / 36, 16 384 x 512 x 512 in 16 22 / 18 / 26, 32 768 x 512 x 512 in 32 41 / 32 / 28; dweight: 8 192 x 1 024 x 1 024 in 16
+// 43 / 33 / 30, 32 768 x 512 x 512 in 32 34 / 27 / 42.  The large tile has no registers for n or k that end inside a chunk.
 Tile pick_tile(const mpe_grouped_desc *d, int64_t mean_rows, int64_t cols, int64_t rows, int64_t others) {
   if (d->dtype == MPE_F32) return SMALL;
   const auto tiles = [&](int64_t t) { return (rows + t - 1) / t * ((cols + t - 1) / t) * others; };
@@ -104,14 +106,27 @@ int64_t dw_tiles(const mpe_grouped_desc *d) {
   const int t = kTile[dw_tile(d)];
   return (int64_t)((d->n + t - 1) / t) * ((d->k + t - 1) / t) * d->groups;
 }
-// Where the outputs are too few tiles to fill the chip (two workgroups a CU; of large tiles, which one fills, they are
-// enough by pick_tile's rule), each group's rows are split.
+// Where the outputs are few tiles that each run over many rows, a group's rows are split over workgroups and the partial sums
+// joined.  The join is a launch (4 us) and 8 bytes a partial sum: the split with the least sum of both, from the rows a tile gets
+// through per us.  f32 65 536 x 64 x 64 in 64 groups 28 us as one, 15 in eight parts; bf16 4 096 x 256 x 256 in 8 7.2 as one, 12 in
+// four, 8 192 x 512 x 512 in 4 17 as one, 19 in two.  Large tiles are enough by pick_tile's rule.
 int dw_splits(const mpe_grouped_desc *d) {
+  const Tile tile = dw_tile(d);
+  if (tile == LARGE) return 1;
   const int64_t tiles = dw_tiles(d), mean = d->rows / d->groups;
-  int s = 1;
-  if (dw_tile(d) != LARGE)
-    while (s < 64 && tiles * s < 512 && mean / (s * 2) >= 64) s *= 2;
-  return s;
+  const double rate = d->dtype == MPE_F32 ? 44.0 : tile == SMALL ? 142.0 : 64.0;
+  const double sums = (double)d->groups * d->n * d->k;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && (s == 1 || mean / s >= 64); s *= 2) {
+    const int64_t rounds = (tiles * s + 511) / 512;  // two workgroups a CU at a time
+    const double us = (double)mean / s / rate * (double)rounds + (s > 1 ? 4.0 + s * sums * 8 / 4e6 : 0.0);
+    if (s == 1 || us < least) {
+      least = us;
+      best = s;
+    }
+  }
+  return best;
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------------------

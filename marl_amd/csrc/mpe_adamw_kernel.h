@@ -18,7 +18,8 @@
 // One pass: every value is read and written once (with a clip, gradients of more than one work item are read twice).  Work items
 // of 8 192 values: 8 values a thread a turn, 16-byte accesses, no tensor shares an item, so the smallest and the largest tensors
 // need one launch together.  Bound by memory: 62 M f32 values with clip and target (2.2 GB) 540 us = 4.2 TB/s, 302 M bf16
-// values with 8-bit moments (3.0 GB) 600 us = 5.0 TB/s; 48 variables of 4 learners 9 us, 25 from Python.
+// values with 8-bit moments (3.0 GB) 620 us = 4.9 TB/s, the vector units 91 % active; 48 variables of 4 learners 9 us, 26 from
+// Python.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamArgs a) {
         m[e] = m[e] * a.beta1 + gc * a.beta1c;
         v[e] = v[e] * a.beta2 + (gc * gc) * a.beta2c;
         // 8 bits: 10 bytes a value leave ~90 vector instructions at the memory's rate, and correctly rounded roots and
-        // quotients take 20 of them: the 1-ulp instructions there (302 M values bf16: 723 -> 600 us)
+        // quotients take 20 of them: the 1-ulp instructions there (302 M values bf16: 723 -> 620 us)
         const float q = EIGHT ? m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.root + a.eps)
                               : m[e] / (sqrtf(v[e]) * s.root + a.eps);
         x[e] = x[e] * s.decay - q * s.step_size;

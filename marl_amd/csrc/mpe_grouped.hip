@@ -29,8 +29,8 @@ int grouped_check(const mpe_grouped_desc *d) {
 // A matrix of the call, and whether it is packed into the workspace first: a tile (256 lines) of it would span too much, or it
 // is masked and its readers do not apply the mask.  The larger tiles have no room for it; the small ones load and apply it once
 // per 64 columns of x, which pays while those are few (rows x k x n in groups, us, mask in the tiles / masked first):
-// f32 4 096 x 64 x 64 in 4 10.0 / 11.7, 32 768 x 64 x 64 in 8 24.8 / 28.9, 4 096 x 256 x 256 in 8 24.0 / 27.7, 1 024 x 512 x 512
-// in 4 30.8 / 31.2, 1 024 x 1 024 x 1 024 in 4 54 / 51, 16 384 x 512 x 512 in 16 188 / 165; fp16 5 003 x 333 x 517 in 7 38 / 34.
+// f32 4 096 x 64 x 64 in 4 9.6 / 11.4, 32 768 x 64 x 64 in 8 17.9 / 24.2, 4 096 x 256 x 256 in 8 23.2 / 27.1, 1 024 x 512 x 512 in 4
+// 27.5 / 26.9, 16 384 x 512 x 512 in 16 180 / 163; fp16 5 003 x 333 x 517 in 7 33 / 27.
 constexpr int kMaskCols = 256;
 struct Matrix {
   const void *p, *mask;

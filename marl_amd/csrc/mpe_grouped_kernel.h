@@ -17,8 +17,8 @@
 //     small calls        launch and one trip to memory: 4 096 x 16 x 64 f32 6 us, 5 003 x 333 x 517 f16 in 7 groups 12
 //     few rows           the weights: 13 rows over 16 of 1 024 x 2 048 bf16, 55 MB, 13 us = 4.2 TB/s
 //     f32                the matrix units: 65 536 x 14 752 x 64 in 64 groups 1 100 us, 3.7 TB/s, matrix units busy 78 % of the time
-//     16-bit, many rows  32 768 x 2 048 x 2 048 bf16 in 32 unlike groups 331 us = 830 TFLOP/s (even groups 288, one group 256), matrix
-//                        units busy 36 %.  No faster: a second set of fragments read ahead (70 us a round of tiles instead of
+//     16-bit, many rows  32 768 x 2 048 x 2 048 bf16 in 32 unlike groups 333 us = 825 TFLOP/s (even groups 288, one group 256), matrix
+//                        units busy 38 %.  No faster: a second set of fragments read ahead (70 us a round of tiles instead of
 //                        65), 128 elements of c a stage (whole cache lines) with two stages (70); a wavefront on 128 x 128 spills
 #pragma once
 #include <hip/hip_runtime.h>

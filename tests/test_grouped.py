@@ -127,7 +127,9 @@ SHAPES = [
     ([1], 1, 1), ([5], 3, 2), ([0, 1, 0], 7, 9), ([3, 0, 64, 65, 1], 16, 64), ([63, 64, 65], 33, 65), ([256] * 4, 64, 64),
     ([1000, 1, 0, 500], 226, 64), ([128, 129], 64, 5), ([17, 300, 3], 333, 517), ([200, 0, 56], 512, 256), ([0, 0], 8, 8),
     ([2500], 130, 40), ([1] * 70, 20, 24), ([700, 900], 128, 136), ([1, 2, 1, 0, 3], 1024, 520),
-    ([900, 0, 1300, 760], 512, 2048), ([4100, 5001], 2048, 264), ([3000, 2200], 130, 2050), ([1500] * 6, 1032, 1024)]
+    ([900, 0, 1300, 760], 512, 2048), ([4100, 5001], 2048, 264), ([3000, 2200], 130, 2050), ([1500] * 6, 1032, 1024),
+    ([700, 0, 1300, 399, 1111, 2600, 520, 1501], 264, 2056), ([33, 0, 64, 1] * 4, 1000, 1032),
+    ([1024, 1500, 3, 900, 0, 2048, 1111, 130, 1793, 640, 1280, 385, 2200, 1029, 1337, 1020], 1032, 1024)]
 
 
 @pytest.mark.gpu
@@ -174,6 +176,25 @@ def test_strides_alignment_and_rows_of_no_group(dtype):
     assert grouped.grouped_linear(xs, ws, ends, bias=b, out=out[:, 2:2 + n]).data_ptr() == out[:, 2:].data_ptr()
     _close(out[:live, 2:2 + n], want[0][:live], terms[0][:live], k + 1, dtype, 'out')
     assert (out[live:] == 5).all() and (out[:, :2] == 5).all() and (out[:, 2 + n:] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('k,n', [(64, 768), (768, 64)])
+def test_more_groups_than_lanes_with_whole_and_partial_tiles_and_a_tail(k, n, dtype):
+    """70 groups of one to three whole tiles and a rest of any size, empty ones between, rows of no group behind them."""
+    sizes, tail = [0 if i % 17 == 5 else 256 * (1 + i % 3) + i * 29 % 256 for i in range(70)], 300
+    x, w, b, grad, ends = _case(sizes, k, n, dtype, tail=tail)
+    live = sum(sizes)
+    y = grouped.grouped_linear(x, w, ends, bias=b, relu=True)
+    got = (y,) + grouped.grouped_linear_backward(grad, x, w, ends, y=y)
+    want, terms = _reference(x, w, b, grad, sizes, True, y)
+    for o, ref, ab, count, what in zip(got, want, terms, (k + 1, n, max(sizes), max(sizes)), ('y', 'dx', 'dw', 'db')):
+        _close(o, ref, ab, count, dtype, what)
+    assert not y[live:].any() and not got[1][live:].any()
+    out = torch.full((live + tail, n), 5.0, dtype=dtype, device='cuda')
+    grouped.grouped_linear(x, w, ends, bias=b, relu=True, out=out)
+    assert torch.equal(out[:live], y[:live]) and (out[live:] == 5).all()
 
 
 @pytest.mark.gpu

@@ -359,7 +359,7 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
   const int64_t end_a = (a.rows - 1) * a.ld_a + cols_a, end_b = (lines_b - 1) * a.ld_b + cols_b;
   const int64_t b0 = MODE == GROUPED_DW ? 0 : (int64_t)g * a.n * a.ld_b;
 
-  // ---- the product: two stages, one barrier a k-step; the next stage is on its way while this one is multiplied ------------
+  // ---- the product: one barrier a stage; the next stages are on their way while this one is multiplied ---------------------
   const int wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wi = (wave / WN) * (BM / WM), wj = (wave % WN) * (BN / WN);
   f4v acc[MI][NJ] = {};
@@ -492,6 +492,7 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
     fetch(c0, s0);
     if constexpr (STAGES == 4) fetch(c0 + KE, s1), fetch(c0 + 2 * KE, s2);
     // a wavefront of a large tile whose rows or columns do not exist only copies: its neighbour on the matrix unit goes on alone
+    // (dweight's first column tile is whole, large tiles have 256 columns at least: every share of dbias is summed)
     if (BM < 256 || (i0 + wi < i_end && j0 + wj < j_end)) steps(std::true_type());
     else steps(std::false_type());
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the tile

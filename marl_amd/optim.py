@@ -9,13 +9,14 @@ variables' memory here:
     p  = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
     target = polyak target + (1 - polyak) p                                                 (targets given)
 
-Parameters are float32, bfloat16 or float16 (one type a group; their gradients and targets alike); the arithmetic is in
+Parameters are float32, bfloat16 or float16 (one type a group; targets and gradients alike, others are refused); the arithmetic is in
 32 bits, the norms in 64, and p is rounded once.  ``state_bits=32`` holds the moments in float32; ``state_bits=8`` in one byte
 each, plus one int16 for 128 of them: a logarithmic code (eighths of a binade; m 16 binades and a sign, v 32 binades) below
 the largest element of its block, rounded stochastically from (seed, step, tensor, element), so that a moment is right on
 average and a run repeats bit for bit.  A gradient that is not finite makes its element (32 bits) or its block of 128
 (8 bits) useless, as it does any Adam."""
 import ctypes as C
+from operator import attrgetter
 
 import torch
 
@@ -23,6 +24,7 @@ from . import _hip
 
 BLOCK = 128                       # elements that share the base of their 8-bit moments; every variable starts a new one
 _DTYPES = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
+_dtype = attrgetter('dtype')
 
 
 def dequantize(codes, base, signed, dtype=torch.float32):
@@ -50,6 +52,7 @@ class _Plan(object):
         p0 = params[0]
         self.params, self.targets, self.bits = list(params), targets, state_bits
         self.device, self.dtype = p0.device, p0.dtype
+        self.like = ({p0.dtype}, {p0.get_device()})           # of every gradient
         self.written = self.params + (self.targets or [])
         self.counts = [p.numel() for p in self.params]
         self.first, total = [], 0
@@ -204,19 +207,22 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step ----------------------------------------------------------------------------------------------------------
     def _gradients(self, plan):
-        """Fills the plan's pointers; returns what must outlive the launch.  (torch sees to it that a gradient has its
-        parameter's type, device and shape when it is set; the parameter may have shrunk before.)"""
-        grads = [p.grad for p in plan.params]
+        """Fills the plan's pointers; returns what must outlive the launch.  torch lets a gradient differ from its parameter in
+        type (``grad_dtype``) and, through ``.data``, in everything else: the kernels read it as the parameter's."""
+        grads = live = [p.grad for p in plan.params]
         try:
             plain = all(map(torch.Tensor.is_contiguous, grads))
         except TypeError:                                         # a None
             plain = False
         if not plain:
             grads = [None if g is None else g.contiguous() for g in grads]
+            live = [g for g in grads if g is not None]
             sizes = [c if g is None else g.numel() for g, c in zip(grads, plan.counts)]
             pointers = [None if g is None else g.data_ptr() for g in grads]
         else:
             sizes, pointers = list(map(torch.Tensor.numel, grads)), list(map(torch.Tensor.data_ptr, grads))
+        if live and (set(map(_dtype, live)), set(map(torch.Tensor.get_device, live))) != plan.like:
+            raise ValueError('AdamW: gradients are %s on %s, as their parameters are' % (plan.dtype, plan.device))
         if sizes != plan.counts:
             raise ValueError('AdamW: a gradient is not of the size that its parameter had')
         plan.grads[:] = pointers

@@ -532,3 +532,53 @@ def test_offsets_past_32_bits():
     assert not p[:first].any() and not st['exp_avg'][:lo].any()
     live = p.grad[first:].float().abs() > 1e-3
     assert torch.allclose(p[first:].float()[live], -0.5 * p.grad[first:].float().sign()[live], rtol=2.0 ** -7)
+
+
+# ---- gradients of another type or device ---------------------------------------------------------------------------------
+OTHER_TYPES = [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16), (torch.float32, torch.float64)]
+
+
+def _with_gradient(dtype, grad_dtype, device):
+    """Two parameters, the second with a gradient of another type: torch's own way, ``grad_dtype``."""
+    ps = [torch.nn.Parameter(torch.ones(300, dtype=dtype, device=device)) for _ in range(2)]
+    ps[0].grad = torch.ones(300, dtype=dtype, device=device)
+    ps[1].grad_dtype = grad_dtype
+    ps[1].grad = torch.ones(300, dtype=grad_dtype, device=device)
+    return ps
+
+
+@pytest.mark.parametrize('first', [True, False], ids=['all', 'one_missing'])
+@pytest.mark.parametrize('dtype,grad_dtype', OTHER_TYPES)
+def test_the_host_refuses_gradients_of_another_type(dtype, grad_dtype, first):
+    """The check itself, on the CPU: what it lets through is read as the parameter's type."""
+    ps = _with_gradient(dtype, grad_dtype, 'cpu')
+    plan = optim._Plan(ps, None, 32)
+    if not first:
+        ps[0].grad = None
+    with pytest.raises(ValueError):
+        optim.AdamW._gradients(None, plan)
+    ps[1].grad = None
+    ps[1].grad_dtype = dtype
+    ps[1].grad = torch.ones(300, dtype=dtype)
+    assert optim.AdamW._gradients(None, plan)[1] is ps[1].grad
+    plan.like = plan.like[0], {0}                                      # parameters on a GPU, gradients that are not
+    with pytest.raises(ValueError):
+        optim.AdamW._gradients(None, plan)
+    ps[0].grad = ps[1].grad = None
+    assert optim.AdamW._gradients(None, plan) == [None, None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype,grad_dtype', OTHER_TYPES)
+def test_a_step_with_gradients_of_another_type_is_refused(dtype, grad_dtype, bits):
+    ps = _with_gradient(dtype, grad_dtype, 'cuda')
+    opt = optim.AdamW(ps, lr=0.5, state_bits=bits)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert all((p == 1).all() for p in ps) and opt.step_count == 0 and not any(t.any() for t in opt.buffers()[0].values())
+    ps[1].grad = None
+    ps[1].grad_dtype = dtype
+    ps[1].grad = torch.ones(300, dtype=dtype, device='cuda')
+    opt.step()
+    assert opt.step_count == 1 and all((p < 1).all() for p in ps)

@@ -239,6 +239,11 @@ struct GroupedOperand {
       }
     }
   }
+  // the place in LDS, in elements, of column `pos` of line `line`, or -1 where another thread copies it
+  static __device__ __forceinline__ int mine(int line, int pos) {
+    const int id = line * kLine + place(line, pos / CE);
+    return (int)threadIdx.x == id % NT ? id * CE + pos % CE : -1;
+  }
   // lane l's share of the fragment of rows i0 .. i0 + 15 (i0: a multiple of 16), k-step kk: row l % 16, c = kk * 4 CE +
   // (l / 16) * CE .. + CE
   static __device__ __forceinline__ uint4 frag(const uint4 *lds, int i0, int kk) {
@@ -383,6 +388,26 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
       om.copy(la + (BM + BN) * KC, pm + mt, ((a.rows - 1) * a.ld_mask + cols_a - mt) * (int64_t)sizeof(T));
     }
   };
+  // 2-byte elements in lines of odd width: an array's last element is half of a dword that the buffer's bounds cut off, and its copy
+  // brings zero.  The thread of that copy puts it in place before its stage is multiplied (adding its product afterwards would not
+  // undo a zero times an infinity).  fill_*: how far from c0 the element is multiplied, or -1; put_*: its place in the stage.
+  constexpr bool CUTS = EDGES && sizeof(T) == 2;
+  int fill_a = -1, fill_b = -1, put_a = 0, put_b = 0;
+  if constexpr (CUTS) {
+    const int64_t last_b = lines_b - 1 - (MODE == GROUPED_DW ? 0 : (int64_t)g * a.n);  // B's last line: a c, or forward a j
+    const int64_t ia = MODE == GROUPED_DW ? cols_a - 1 : a.rows - 1, ca = MODE == GROUPED_DW ? a.rows - 1 : cols_a - 1;
+    const int64_t jb = MODE == GROUPED_FWD ? last_b : cols_b - 1, cb = MODE == GROUPED_FWD ? cols_b - 1 : last_b;
+    if ((cols_a & 1) && ia >= i0 && ia < i0 + BM && ia < i_end && ca >= c0 && ca < c_end) {
+      const int i = (int)(ia - i0), c = (int)(ca - c0);
+      put_a = MODE == GROUPED_DW ? OpA::mine(c % KE, i) : OpA::mine(i, c % KE);
+      fill_a = put_a < 0 ? -1 : c;
+    }
+    if ((cols_b & 1) && jb >= j0 && jb < j0 + BN && jb < j_end && cb >= c0 && cb < c_end) {
+      const int j = (int)(jb - j0), c = (int)(cb - c0);
+      put_b = MODE == GROUPED_FWD ? OpB::mine(j, c % KE) : OpB::mine(c % KE, j);
+      fill_b = put_b < 0 ? -1 : c;
+    }
+  }
   const bool with_bias = MODE == GROUPED_DW && a.dbias != nullptr && tj == 0;
   constexpr int kAhead = (STAGES - 2) * ((MASK ? 2 : 1) * OpA::N + OpB::N);  // copies of later stages that may still be under way
   // this wavefront's copies of this stage have landed, its reads of LDS are done; then so are everybody's
@@ -391,6 +416,14 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
     if (EDGES && MODE != GROUPED_DW && c_end - c < KE && (c_end - c) % OpA::CE != 0) {
       oa.trim(la, STAGES - 1);
       ob.trim(la + BM * KC, STAGES - 1);
+    }
+    if constexpr (CUTS) {
+      const int past = (int)(c - c0);
+      if ((uint32_t)(fill_a - past) < (uint32_t)KE) {
+        reinterpret_cast<T *>(la)[put_a] = pa[end_a - 1];
+        if constexpr (MASK) reinterpret_cast<T *>(la + (BM + BN) * KC)[put_a] = pm[(a.rows - 1) * a.ld_mask + cols_a - 1];
+      }
+      if ((uint32_t)(fill_b - past) < (uint32_t)KE) reinterpret_cast<T *>(la + BM * KC)[put_b] = pb[end_b - 1];
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -500,35 +533,6 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
 
   // ---- epilogue: lane holds output row i0 + wi + 16 m + lane % 16, columns j0 + wj + 16 n + 4 (lane / 16) .. + 4 ----------
   const int64_t j_lane = j0 + wj + 4 * (lane >> 4);
-  if (EDGES && sizeof(T) == 2 && c0 < c_end && ((cols_a | cols_b) & 1)) {
-    // 2-byte elements in lines of odd width: an array's last element is half of a dword that the buffer's bounds cut off, and
-    // was multiplied as zero.  What it should have added: A(i, ca) B(j, ca) for A's, A(i, cb) B(j, cb) for B's.
-    const int64_t last_b = lines_b - 1 - (MODE == GROUPED_DW ? 0 : (int64_t)g * a.n);  // B's last line: a c, or forward a j
-    const int64_t ia = MODE == GROUPED_DW ? cols_a - 1 : a.rows - 1, ca = MODE == GROUPED_DW ? a.rows - 1 : cols_a - 1;
-    const int64_t jb = MODE == GROUPED_FWD ? last_b : cols_b - 1, cb = MODE == GROUPED_FWD ? cols_b - 1 : last_b;
-    const bool cut_a = (cols_a & 1) && ia >= i0 && ia < i0 + BM && ia < i_end && ca >= c0 && ca < c_end;
-    const bool cut_b = (cols_b & 1) && jb >= j0 && jb < j0 + BN && jb < j_end && cb >= c0 && cb < c_end;
-    const auto elem_a = [&](int64_t i, int64_t c) {
-      if (MASK && (float)pm[MODE == GROUPED_DW ? c * a.ld_mask + i : i * a.ld_mask + c] <= 0.0f) return 0.0f;
-      return (float)pa[MODE == GROUPED_DW ? c * a.ld_a + i : i * a.ld_a + c];
-    };
-    const auto elem_b = [&](int64_t j, int64_t c) { return (float)pb[b0 + (MODE == GROUPED_FWD ? j * a.ld_b + c : c * a.ld_b + j)]; };
-    if (cut_a || cut_b) {
-#pragma unroll
-      for (int m = 0; m < MI; ++m) {
-        const int64_t i = i0 + wi + m * 16 + (lane & 15);
-        if (cut_a && i == ia && with_bias && m / kSums == wn && lane < 16) sum[m % kSums] += elem_a(ia, ca);
-#pragma unroll
-        for (int n = 0; n < NJ; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t j = j_lane + n * 16 + e;
-            if (cut_a && i == ia && j < j_end) acc[m][n][e] += elem_a(ia, ca) * elem_b(j, ca);
-            if (cut_b && j == jb && i < i_end && !(cut_a && i == ia && ca == cb)) acc[m][n][e] += elem_a(i, cb) * elem_b(jb, cb);
-          }
-      }
-    }
-  }
   const bool whole = j0 + BN <= j_end;  // all columns exist
   const auto valid_of = [&](int n) { return j_end - j_lane - n * 16 >= 4 ? 4 : (int)(j_end - j_lane - n * 16); };
   if constexpr (MODE == GROUPED_FWD) {

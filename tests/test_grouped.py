@@ -405,3 +405,54 @@ def test_offsets_past_32_bits():
     want, terms = _reference(x[-300:], w, torch.zeros(2, n, device='cuda'), grad[-300:], [100, 200], False)
     for got, ref, ab, what in ((dw, want[2], terms[2], 'dw'), (db, want[3], terms[3], 'db')):
         _close(got, ref, ab, 200, torch.bfloat16, what)
+
+
+def _same(got, want, terms, count, dtype, what):
+    """Where the definition in 64 bits gives an infinity or NaN the result is the same, elsewhere it is close."""
+    odd = ~torch.isfinite(want)
+    assert torch.equal(got.double()[odd].nan_to_num(0.5), want[odd].nan_to_num(0.5)), what
+    _close(torch.where(odd, 0, got), torch.where(odd, 0, want), torch.where(odd, 0, terms), count, dtype, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('sizes,k,n', [([40, 33], 71, 51), ([3], 1, 1), ([5, 60], 70, 131), ([64, 3], 131, 8), ([600, 505], 301, 67),
+                                       ([300, 200, 100, 500], 1025, 1025), ([4000, 4192], 131, 1025), ([2000, 2100], 1025, 131)])
+def test_infinities_opposite_an_arrays_last_element(sizes, k, n, dtype):
+    """Odd widths, every tile: an infinity that meets x's, dy's or weight's last element in forward, dx or dweight gives what
+    the sum gives, plus or minus infinity, and relu turns the latter into zero."""
+    t, last = sum(sizes), len(sizes) - 1
+    for case in range(5):
+        x, w, b, grad, ends = _case(sizes, k, n, dtype, seed=case)
+        if n > 1 or case == 2:
+            r = t - 1 - (case + 1) % min(3, sizes[-1])
+            if case == 0:
+                x[r, k - 1] = float('inf')                           # forward: opposite weight's last
+            elif case == 1:
+                w[last, n // 2, k - 1] = float('-inf')               # forward: opposite x's last (and of weight's last column)
+            elif case == 2:
+                w[last, n - 1, k // 2] = float('inf')                # dx: opposite dy's last
+            elif case == 3:
+                grad[r, n - 1] = float('-inf')                       # dx: opposite weight's last; dweight
+                grad[t - 1, 0] = float('inf')                        # dweight: opposite x's last
+            else:
+                x[t - 1, 0] = float('inf')                           # dweight: opposite dy's last
+        y_saved = torch.randn(t, n, generator=torch.Generator().manual_seed(case)).to(dtype).cuda()
+        for y in (None, y_saved):
+            got = (grouped.grouped_linear(x, w, ends, bias=b, relu=y is not None),) + grouped.grouped_linear_backward(grad, x, w, ends, y=y)
+            want, terms = _reference_with_infinities(x, w, b, grad, sizes, y)
+            most = max(sizes)
+            for o, ref, ab, count, what in zip(got, want, terms, (k + 1, n, most, most), ('y', 'dx', 'dw', 'db')):
+                _same(o, ref, ab, count, dtype, (what, case, y is None))
+
+
+def _reference_with_infinities(x, w, b, grad, sizes, y_saved):
+    """``_reference`` with a gradient that is selected, not multiplied, by the mask, and a relu that keeps NaN; products on the
+    CPU, plain sums of products."""
+    x, w, b, grad = (t.double().cpu() for t in (x, w, b, grad))
+    if y_saved is not None:
+        grad = torch.where(y_saved.cpu() <= 0, 0.0, grad)
+    (y, dx, dw, db), terms = _reference(x, w, b, grad, sizes, False)
+    if y_saved is not None:
+        y = torch.where(y < 0, 0.0, y)
+    return [t.cuda() for t in (y, dx, dw, db)], [t.cuda() for t in terms]

@@ -139,6 +139,8 @@ def _forward(x, weight, ends, bias, relu, out):
         ws = _scratch(x, need)
     _hip.check(_hip.launch(index, _hip.lib.mpe_grouped_linear, desc, px, ld_x, pw, None if bias is None else bias.data_ptr(),
                            out.data_ptr(), ld_y, relu, own, _hip.ptr(ws), need), 'mpe_grouped_linear')
+    if not own and not out.is_inference():
+        torch.autograd.graph.increment_version(out)          # what autograd saved of it before is no longer there
     return out
 
 
@@ -161,7 +163,7 @@ class _GroupedLinear(torch.autograd.Function):
 def grouped_linear(x, weight, ends, bias=None, relu=False, out=None):
     """``y[r] = act(x[r] @ weight[g].T + bias[g])`` for the rows ``r`` of every group ``g`` (module docstring).  Rows behind
     the last group: zeros, or with ``out`` (``[rows, n]``, adjacent columns, no overlap with an input) left as they were."""
-    if torch.is_grad_enabled() and any([torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias)]):
+    if torch.is_grad_enabled() and any([torch.is_tensor(t) and t.requires_grad for t in (x, weight, bias, out)]):
         if out is not None:
             raise RuntimeError('grouped_linear(out=...) does not support automatic differentiation')
         return _GroupedLinear.apply(x, weight, ends, bias, bool(relu))

@@ -456,3 +456,25 @@ def _reference_with_infinities(x, w, b, grad, sizes, y_saved):
     if y_saved is not None:
         y = torch.where(y < 0, 0.0, y)
     return [t.cuda() for t in (y, dx, dw, db)], [t.cuda() for t in terms]
+
+
+@pytest.mark.gpu
+def test_autograd_notices_a_write_to_out():
+    """A buffer that autograd saved and a later call overwrites raises in the backward pass; an ``out`` that requires grad is
+    refused, outside ``no_grad``."""
+    x, w, b, grad, ends = _case([3, 4], 6, 5, torch.float32)
+    out = torch.zeros(7, 5, device='cuda')
+    scale = torch.ones(7, 5, device='cuda', requires_grad=True)
+    loss = (out * scale).sum()                                      # saves out
+    assert grouped.grouped_linear(x, w, ends, bias=b, out=out) is out
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    grows = torch.zeros(7, 5, device='cuda', requires_grad=True)
+    with pytest.raises(RuntimeError, match='automatic differentiation'):
+        grouped.grouped_linear(x, w, ends, bias=b, out=grows)
+    assert not grows.any()
+    with torch.no_grad():
+        grouped.grouped_linear(x, w, ends, bias=b, out=grows)
+    with torch.inference_mode():
+        again = grouped.grouped_linear(x, w, ends, bias=b, out=torch.empty(7, 5, device='cuda'))
+    assert torch.equal(grows, out) and torch.equal(again, out)

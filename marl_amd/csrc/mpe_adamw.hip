@@ -37,20 +37,24 @@ int tensors_check(int n, const mpe_adamw_tensor *t, int dtype, int state_bits, i
 int64_t plan_items_at(int n) { return (int64_t)n * (int64_t)sizeof(AdamTensor); }
 int64_t plan_norms_at(int n, int64_t items) { return plan_items_at(n) + items * (int64_t)sizeof(AdamItem); }
 
-template <typename T, bool EIGHT>
+template <typename T, bool EIGHT, bool FAST>
 int launch(const AdamArgs &a, unsigned items, bool clip, bool norms, hipStream_t s) {
   if (clip) {
     if (norms) hipLaunchKernelGGL(adamw_norm_kernel<T>, dim3(items), dim3(kAdamThreads), 0, s, a);
-    hipLaunchKernelGGL((adamw_kernel<T, EIGHT, true>), dim3(items), dim3(kAdamThreads), 0, s, a);
+    hipLaunchKernelGGL((adamw_kernel<T, EIGHT, true, FAST>), dim3(items), dim3(kAdamThreads), 0, s, a);
   } else {
-    hipLaunchKernelGGL((adamw_kernel<T, EIGHT, false>), dim3(items), dim3(kAdamThreads), 0, s, a);
+    hipLaunchKernelGGL((adamw_kernel<T, EIGHT, false, FAST>), dim3(items), dim3(kAdamThreads), 0, s, a);
   }
   return (int)hipGetLastError();
 }
 
 template <typename T>
-int launch_bits(const AdamArgs &a, int bits, unsigned items, bool clip, bool norms, hipStream_t s) {
-  return bits == 8 ? launch<T, true>(a, items, clip, norms, s) : launch<T, false>(a, items, clip, norms, s);
+int launch_bits(const AdamArgs &a, int bits, bool fast, unsigned items, bool clip, bool norms, hipStream_t s) {
+  if (bits != 8) return launch<T, false, false>(a, items, clip, norms, s);
+  if constexpr (sizeof(T) == 2) {
+    if (fast) return launch<T, true, true>(a, items, clip, norms, s);
+  }
+  return launch<T, true, false>(a, items, clip, norms, s);
 }
 
 }  // namespace
@@ -117,6 +121,8 @@ extern "C" int mpe_adamw_step(const mpe_adamw_args *h, int n, const mpe_adamw_te
     a.s.decay = (float)(1.0 - h->lr * h->weight_decay);
     a.s.key = adam_step_key(h->seed, h->step);
   }
+  // a root that reads v < 2^-126 as zero is off by 2^-63 / sqrt(1 - b2^t) at most: no more than half a step of eps
+  const bool fast = h->eps * std::sqrt(1.0 - h->beta2) >= 0x1p-39;
   uint32_t first = 0;
   for (int i0 = 0; i0 < n; i0 += kAdamMaxGrads) {
     const int many = n - i0 < kAdamMaxGrads ? n - i0 : kAdamMaxGrads;
@@ -134,9 +140,9 @@ extern "C" int mpe_adamw_step(const mpe_adamw_args *h, int n, const mpe_adamw_te
     first += batch;
     if (batch == 0) continue;
     const bool clip = h->max_norm > 0;
-    const int rc = h->dtype == MPE_F32    ? launch_bits<float>(a, h->state_bits, batch, clip, norms, s)
-                   : h->dtype == MPE_BF16 ? launch_bits<__bf16>(a, h->state_bits, batch, clip, norms, s)
-                                          : launch_bits<_Float16>(a, h->state_bits, batch, clip, norms, s);
+    const int rc = h->dtype == MPE_F32    ? launch_bits<float>(a, h->state_bits, fast, batch, clip, norms, s)
+                   : h->dtype == MPE_BF16 ? launch_bits<__bf16>(a, h->state_bits, fast, batch, clip, norms, s)
+                                          : launch_bits<_Float16>(a, h->state_bits, fast, batch, clip, norms, s);
     if (rc) return rc;
   }
   return MPE_OK;

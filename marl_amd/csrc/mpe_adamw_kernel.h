@@ -168,7 +168,12 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_norm_kernel(const AdamArgs
   if (threadIdx.x == 0) a.norms[a.first_item + blockIdx.x] = s;
 }
 
-template <typename T, bool EIGHT, bool CLIP>
+// FAST: 16-bit parameters with 8-bit moments, 10 bytes a value, leave ~90 vector instructions at the memory's rate, and a correctly
+// rounded root and quotient take 20 of them (302 M values bf16: 725 us, 623 without): there the 1-ulp instructions, whose error is
+// 2^-12 (f16) or 2^-15 (bf16) of what rounding the parameter brings.  The root's instruction reads subnormal v as zero: the host
+// takes FAST only where eps drowns that.  f32 parameters have bytes enough to hide the rounded ones (62 M values: 207 us, 201
+// without; with targets 305, 304).
+template <typename T, bool EIGHT, bool CLIP, bool FAST>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamArgs a) {
   const AdamItem it = a.items[a.first_item + blockIdx.x];
   const AdamTensor t = a.tensors[it.tensor];
@@ -217,10 +222,8 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamArgs a) {
         const float gc = CLIP ? d[e] * scale : d[e];
         m[e] = m[e] * a.beta1 + gc * a.beta1c;
         v[e] = v[e] * a.beta2 + (gc * gc) * a.beta2c;
-        // 8 bits: 10 bytes a value leave ~90 vector instructions at the memory's rate, and correctly rounded roots and
-        // quotients take 20 of them: the 1-ulp instructions there (302 M values bf16: 723 -> 620 us)
-        const float q = EIGHT ? m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.root + a.eps)
-                              : m[e] / (sqrtf(v[e]) * s.root + a.eps);
+        const float q = FAST ? m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[e]) * s.root + a.eps)
+                             : m[e] / (sqrtf(v[e]) * s.root + a.eps);
         x[e] = x[e] * s.decay - q * s.step_size;
         held[e] = (T)x[e];
         if (e >= valid) m[e] = v[e] = 0.0f;  // nothing behind the variable's end reaches its block

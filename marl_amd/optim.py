@@ -10,7 +10,8 @@ variables' memory here:
     target = polyak target + (1 - polyak) p                                                 (targets given)
 
 Parameters are float32, bfloat16 or float16 (one type a group; targets and gradients alike, others are refused); the arithmetic is in
-32 bits, the norms in 64, and p is rounded once.  ``state_bits=32`` holds the moments in float32; ``state_bits=8`` in one byte
+32 bits, the norms in 64, and p is rounded once.  (Of 16-bit parameters with 8-bit moments the root and the quotient are to one last
+place of 32 bits, elsewhere correctly rounded.)  ``state_bits=32`` holds the moments in float32; ``state_bits=8`` in one byte
 each, plus one int16 for 128 of them: a logarithmic code (eighths of a binade; m 16 binades and a sign, v 32 binades) below
 the largest element of its block, rounded stochastically from (seed, step, tensor, element), so that a moment is right on
 average and a run repeats bit for bit.  A gradient that is not finite makes its element (32 bits) or its block of 128

@@ -582,3 +582,20 @@ def test_a_step_with_gradients_of_another_type_is_refused(dtype, grad_dtype, bit
     ps[1].grad = torch.ones(300, dtype=dtype, device='cuda')
     opt.step()
     assert opt.step_count == 1 and all((p < 1).all() for p in ps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('capturable', [False, True], ids=['host', 'device'])
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_subnormal_second_moments_without_eps(dtype, bits, capturable):
+    """eps = 0: the first step is lr sign(g) however small g is.  g = 2e-20: g^2 = 4e-40 and v = g^2 / 1000 are subnormal, v holds
+    285 of the smallest steps, so sqrt(v) is right to half of 1 / 285 / 2 (0.1 %); the parameter to its own rounding."""
+    g = torch.full((700,), 2e-20, dtype=dtype, device='cuda')
+    g[::2].neg_()
+    p = torch.zeros(700, dtype=dtype, device='cuda')
+    p.grad = g
+    opt = optim.AdamW([p], lr=0.5, eps=0.0, weight_decay=0.0, state_bits=bits, capturable=capturable)
+    opt.step()
+    assert torch.allclose(p.double(), -0.5 * g.double().sign(), rtol=2e-3 + HALF[dtype], atol=0)
+    assert (opt.moments()[0][1][:700] > 0).all()

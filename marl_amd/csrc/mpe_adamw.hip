@@ -1,4 +1,5 @@
 // C ABI of the AdamW step over many tensors (include/mpe_hip.h); kernels in mpe_adamw_kernel.h.
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 
@@ -93,7 +94,7 @@ extern "C" int mpe_adamw_step(const mpe_adamw_args *h, int n, const mpe_adamw_te
   if (bad_align(plan, 8) || bad_align(h->clock, 8)) return MPE_ERR_ALIGN;
   if (!(h->lr >= 0) || !(h->beta1 >= 0 && h->beta1 < 1) || !(h->beta2 >= 0 && h->beta2 < 1) || !(h->eps >= 0) ||
       !(h->weight_decay >= 0) || !(h->polyak >= 0 && h->polyak <= 1) || !(h->max_norm >= 0) || std::isinf(h->lr) ||
-      std::isinf(h->max_norm) || (!h->clock && h->step < 1))
+      (h->max_norm > 0 && !((float)h->max_norm >= FLT_MIN && (float)h->max_norm <= FLT_MAX)) || (!h->clock && h->step < 1))
     return MPE_ERR_ARG;
   AdamArgs a{};
   const char *at = static_cast<const char *>(plan);

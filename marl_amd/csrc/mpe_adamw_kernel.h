@@ -188,8 +188,10 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(const AdamArgs a) {
     if (t.items == 1) sum = adam_squares(g, begin, end);
     else
       for (uint32_t i = threadIdx.x; i < t.items; i += kAdamThreads) sum += a.norms[t.first_item + i];
-    const float norm = (float)sqrt(adam_block_sum(sum));
-    scale = a.max_norm / (norm < a.max_norm ? a.max_norm : norm);  // NaN stays NaN
+    const double root = sqrt(adam_block_sum(sum));
+    const float norm = (float)root;
+    scale = a.max_norm / (norm < a.max_norm ? a.max_norm : norm);        // NaN stays NaN
+    if (norm > 3.4e38f && root < 1e300) scale = (float)(a.max_norm / root);  // finite elements, a norm beyond 32 bits
   }
   const uint32_t key = EIGHT ? adam_mix(s.key + (a.index0 + it.tensor - a.first_tensor) * 0x85EBCA77u) : 0;
   // whole wavefronts run to the end of the last block of 128: its lanes exchange their largest element

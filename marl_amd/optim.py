@@ -26,6 +26,7 @@ from . import _hip
 BLOCK = 128                       # elements that share the base of their 8-bit moments; every variable starts a new one
 _DTYPES = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
 _dtype = attrgetter('dtype')
+_F32 = torch.finfo(torch.float32)
 
 
 def dequantize(codes, base, signed, dtype=torch.float32):
@@ -143,8 +144,8 @@ class AdamW(torch.optim.Optimizer):
                 or not g['weight_decay'] >= 0 or not 0 <= g['polyak'] <= 1:
             raise ValueError('AdamW: lr %r, betas %r, eps %r, weight_decay %r, polyak %r' % (
                 g['lr'], g['betas'], g['eps'], g['weight_decay'], g['polyak']))
-        if g['max_norm'] is not None and not 0 < g['max_norm'] < float('inf'):
-            raise ValueError('AdamW: max_norm is positive and finite, or None, got %r' % (g['max_norm'],))
+        if g['max_norm'] is not None and not _F32.tiny <= g['max_norm'] <= _F32.max:
+            raise ValueError('AdamW: max_norm is positive and finite (a normal float32), or None, got %r' % (g['max_norm'],))
 
     def add_param_group(self, group):
         group = dict(group)

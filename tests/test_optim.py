@@ -599,3 +599,31 @@ def test_subnormal_second_moments_without_eps(dtype, bits, capturable):
     opt.step()
     assert torch.allclose(p.double(), -0.5 * g.double().sign(), rtol=2e-3 + HALF[dtype], atol=0)
     assert (opt.moments()[0][1][:700] > 0).all()
+
+
+# ---- the clip at the ends of 32 bits -------------------------------------------------------------------------------------
+@pytest.mark.parametrize('max_norm', [1e39, 1e-39, 1e-50])
+def test_a_clip_that_float32_does_not_hold_is_refused(max_norm):
+    """As float32 these are infinity, subnormal and zero."""
+    p = 1 << 20
+    assert _hip.lib.mpe_adamw_step(_args(max_norm=max_norm), 1, _table(), p, (C.c_void_p * 1)(p), None) == -6
+    group = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, polyak=0.99, max_norm=max_norm)
+    with pytest.raises(ValueError):
+        optim.AdamW._check_group(group)
+    for good in (None, 2.0 ** -126, 3.4028234663852886e38):
+        optim.AdamW._check_group(dict(group, max_norm=good))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('count', [4, 8192, 20000])
+def test_a_norm_beyond_float32_is_clipped(count):
+    """Finite gradients whose norm is not a float32: g' = g max_norm / |g| (the factor, 1e-41 at least, has 12 bits)."""
+    g = torch.full((count,), 3e38, device='cuda')
+    g[::2].neg_()
+    p = torch.zeros(count, device='cuda')
+    p.grad = g
+    opt = optim.AdamW([p], lr=0.5, weight_decay=0.0, max_norm=0.5)
+    opt.step()
+    want = 0.1 * 0.5 * g.double() / g.double().norm()
+    assert torch.allclose(opt.moments()[0][0][:count].double(), want, rtol=2.0 ** -10, atol=0)
+    assert torch.allclose(p.double(), -0.5 * g.double().sign(), rtol=2.0 ** -10, atol=0)

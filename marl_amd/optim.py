@@ -55,7 +55,9 @@ class _Plan(object):
         self.params, self.targets, self.bits = list(params), targets, state_bits
         self.device, self.dtype = p0.device, p0.dtype
         self.like = ({p0.dtype}, {p0.get_device()})           # of every gradient
-        self.written = self.params + (self.targets or [])
+        self.tracked = [not p.is_inference() for p in self.params]     # tensors of inference mode have no version
+        self.moved = [t for t in self.targets or [] if not t.is_inference()]
+        self.written = [p for p, on in zip(self.params, self.tracked) if on] + self.moved
         self.counts = [p.numel() for p in self.params]
         self.first, total = [], 0
         for c in self.counts:                       # every variable starts at a multiple of BLOCK
@@ -209,7 +211,7 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step ----------------------------------------------------------------------------------------------------------
     def _gradients(self, plan):
-        """Fills the plan's pointers; returns what must outlive the launch.  torch lets a gradient differ from its parameter in
+        """Fills the plan's pointers; returns what must outlive the launch (``plan.whole``: no gradient is missing).  torch lets a gradient differ from its parameter in
         type (``grad_dtype``) and, through ``.data``, in everything else: the kernels read it as the parameter's."""
         grads = live = [p.grad for p in plan.params]
         try:
@@ -228,6 +230,7 @@ class AdamW(torch.optim.Optimizer):
         if sizes != plan.counts:
             raise ValueError('AdamW: a gradient is not of the size that its parameter had')
         plan.grads[:] = pointers
+        plan.whole = len(live) == len(grads)
         return grads
 
     @torch.no_grad()
@@ -253,11 +256,12 @@ class AdamW(torch.optim.Optimizer):
                                  self._bits)
             _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_step, args, len(plan.params), plan.table,
                                    plan.plan_ptr, plan.grads), 'mpe_adamw_step')
-            del keep
             if clock is None:
                 group['step'] += 1
             index0 += len(plan.params)
-            torch.autograd.graph.increment_version(plan.written)
+            torch.autograd.graph.increment_version(plan.written if plan.whole else plan.moved + [
+                p for p, g, on in zip(plan.params, keep, plan.tracked) if g is not None and on])
+            del keep
         return loss
 
     # -- the moments -------------------------------------------------------------------------------------------------------

@@ -627,3 +627,26 @@ def test_a_norm_beyond_float32_is_clipped(count):
     want = 0.1 * 0.5 * g.double() / g.double().norm()
     assert torch.allclose(opt.moments()[0][0][:count].double(), want, rtol=2.0 ** -10, atol=0)
     assert torch.allclose(p.double(), -0.5 * g.double().sign(), rtol=2.0 ** -10, atol=0)
+
+
+@pytest.mark.gpu
+def test_versions_move_where_something_is_written():
+    """A parameter without a gradient is not written: a graph that saved it still runs; its target is.  Parameters and targets
+    made in inference mode, which have no version, are stepped like others."""
+    a, b = (torch.nn.Parameter(torch.ones(30, device='cuda')) for _ in range(2))
+    ta, tb = torch.zeros(30, device='cuda'), torch.zeros(30, device='cuda')
+    opt = optim.AdamW([a, b], lr=0.5, weight_decay=0.0, targets=[ta, tb])
+    kept = (a * a).sum()
+    seen = [t._version for t in (a, b, ta, tb)]
+    b.grad = torch.ones(30, device='cuda')
+    opt.step()
+    assert [t._version - v for t, v in zip((a, b, ta, tb), seen)] == [0, 1, 1, 1]
+    kept.backward()
+    assert (a.grad == 2).all()
+    with torch.inference_mode():
+        p, t = torch.ones(30, device='cuda'), torch.zeros(30, device='cuda')
+        p.grad = torch.ones(30, device='cuda')
+        opt = optim.AdamW([p], lr=0.5, weight_decay=0.0, targets=[t])
+        opt.step()
+        opt.step()
+        assert opt.step_count == 2 and torch.allclose(p, torch.zeros(30, device='cuda'), atol=1e-6) and (t > 0).all()

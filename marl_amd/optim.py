@@ -73,6 +73,7 @@ class _Plan(object):
             self.flat = {'exp_avg': torch.zeros(total, dtype=torch.float32, device=dev),
                          'exp_avg_sq': torch.zeros(total, dtype=torch.float32, device=dev)}
         self.grads = (C.c_void_p * len(self.params))()
+        self.plan, self.streams = None, set()
         self.build()
 
     def views(self, j):
@@ -104,9 +105,17 @@ class _Plan(object):
         _hip.check(min(size, 0), 'mpe_adamw_plan')
         blob = torch.empty(size, dtype=torch.uint8)
         _hip.check(min(_hip.lib.mpe_adamw_plan(n, self.table, code, self.bits, blob.data_ptr(), size), 0), 'mpe_adamw_plan')
-        self.plan = blob.to(self.device)
-        self.plan_ptr = self.plan.data_ptr()
+        if self.plan is None:                       # written again in place: a recording keeps reading this array
+            self.plan = torch.empty(size, dtype=torch.uint8, device=self.device)
+            self.plan_ptr = self.plan.data_ptr()
+        self.plan.copy_(blob)
         self.ptrs = self.pointers()
+
+    def use_on(self, raw):
+        """Before the first eager step on a stream: what the plan owns is not handed to others until that stream is through."""
+        for t in [self.plan] + list(self.flat.values()):
+            t.record_stream(torch.cuda.current_stream(self.device))
+        self.streams.add(raw)
 
     def pointers(self):
         return list(map(torch.Tensor.data_ptr, self.params if self.targets is None else self.params + self.targets))
@@ -119,7 +128,7 @@ class AdamW(torch.optim.Optimizer):
     them by ``polyak``; ``max_norm``: clip of each variable's gradient on its own; ``seed``: of the 8-bit rounding.
     ``capturable=True`` keeps the step count on the device, so that ``step()`` can be recorded in a HIP graph: every replay
     is one more step, with the learning rate and the other settings of the recording.  Gradients are read where they lie:
-    a recording reads the same addresses again, so let them stay (``zero_grad(set_to_none=False)``).
+    a recording reads the same addresses again, so let them stay (``zero_grad(set_to_none=False)``), and keep the optimizer.
 
     A parameter without a gradient keeps its value and moments (its target still moves); the step count is the group's.
     ``state_dict`` / ``load_state_dict`` hold the moments as they are stored."""
@@ -251,6 +260,11 @@ class AdamW(torch.optim.Optimizer):
                 plan.build()
             keep = self._gradients(plan)
             clock = self._clocks[i]
+            raw = torch._C._cuda_getCurrentRawStream(plan.device.index)
+            if raw not in plan.streams and not torch.cuda.is_current_stream_capturing():
+                plan.use_on(raw)
+                if clock is not None:
+                    clock.record_stream(torch.cuda.current_stream(plan.device))
             args = _hip.AdamArgs(group['lr'], *group['betas'], group['eps'], group['weight_decay'], group['max_norm'] or 0.0,
                                  group['polyak'], group['step'] + 1, _hip.ptr(clock), self._seed, index0, _DTYPES[plan.dtype],
                                  self._bits)

@@ -650,3 +650,70 @@ def test_versions_move_where_something_is_written():
         opt.step()
         opt.step()
         assert opt.step_count == 2 and torch.allclose(p, torch.zeros(30, device='cuda'), atol=1e-6) and (t > 0).all()
+
+
+# ---- the plan's memory ---------------------------------------------------------------------------------------------------
+def test_the_plan_stays_where_it_is_when_parameters_move():
+    """On the CPU: what a recording or a step under way reads is not given back while the optimizer lives."""
+    p, t = torch.nn.Parameter(torch.ones(300)), torch.ones(300)
+    plan = optim._Plan([p], [t], 8)
+    at, held = plan.plan_ptr, plan.plan.clone()
+    hold = [p.data, t.data]
+    p.data, t.data = p.data.clone(), t.data.clone()
+    assert plan.pointers() != plan.ptrs
+    plan.build()
+    assert plan.plan_ptr == plan.plan.data_ptr() == at and not torch.equal(plan.plan, held) and plan.pointers() == plan.ptrs
+    del hold
+
+
+@pytest.mark.gpu
+def test_recordings_follow_parameters_that_moved():
+    """After an eager step that found the parameters elsewhere, replays step them there, like the eager run."""
+    def make():
+        p = torch.nn.Parameter(torch.full((9000,), 2.0, device='cuda'))
+        p.grad = torch.linspace(-1, 1, 9000, device='cuda')
+        return p, optim.AdamW([p], lr=0.1, max_norm=0.5, capturable=True)
+    (a, oa), (b, ob) = make(), make()
+    for _ in range(5):
+        oa.step()
+    ob.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode='thread_local'):
+        ob.step()
+    graph.replay()
+    old = b.data
+    b.data = b.data.clone()
+    ob.step()
+    left = old.clone()
+    junk = [torch.full_like(ob._plans[0].plan, 255) for _ in range(4)]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(old, left) and torch.equal(a, b) and oa.step_count == ob.step_count == 5
+    del junk
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('capturable', [False, True])
+def test_an_optimizer_that_goes_while_another_stream_steps(capturable):
+    """Steps queued on a side stream behind other work; the optimizer is dropped and its memory asked for and written on the
+    main stream at once: the steps still read their own."""
+    n = 1 << 20
+    p = torch.nn.Parameter(torch.zeros(n, device='cuda'))
+    p.grad = torch.ones(n, device='cuda')
+    opt = optim.AdamW([p], lr=0.125, weight_decay=0.0, capturable=capturable)
+    sizes = [(t.numel(), t.dtype) for t in list(opt.buffers()[0].values()) + [opt._plans[0].plan]]
+    busy = torch.randn(4096, 4096, device='cuda')
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy = busy @ busy * 1e-2
+        for _ in range(3):
+            opt.step()
+    del opt
+    junk = [torch.full((c,), 77, dtype=dt, device='cuda') for c, dt in sizes for _ in range(2)]
+    torch.cuda.synchronize()
+    assert torch.allclose(p, torch.full_like(p, -0.375), rtol=1e-5)
+    del junk

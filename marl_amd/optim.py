@@ -190,10 +190,11 @@ class AdamW(torch.optim.Optimizer):
         for key, value in self.defaults.items():
             group.setdefault(key, value)
         self._check_group(group)
+        plan = _Plan(params, targets, self._bits)       # may fail: before the group is there
+        clock = torch.zeros(4, dtype=torch.int64, device=plan.device) if self._capturable else None
         super().add_param_group(group)
-        plan = _Plan(params, targets, self._bits)
         self._plans.append(plan)
-        self._clocks.append(torch.zeros(4, dtype=torch.int64, device=plan.device) if self._capturable else None)
+        self._clocks.append(clock)
         for j, p in enumerate(params):
             self.state[p] = plan.views(j)
 

@@ -717,3 +717,21 @@ def test_an_optimizer_that_goes_while_another_stream_steps(capturable):
     torch.cuda.synchronize()
     assert torch.allclose(p, torch.full_like(p, -0.375), rtol=1e-5)
     del junk
+
+
+@pytest.mark.gpu
+def test_a_group_that_could_not_be_added_is_not_there(monkeypatch):
+    """A failure on the way (memory, say) leaves no group that later steps pass over in silence."""
+    a, b = (torch.nn.Parameter(torch.ones(30, device='cuda')) for _ in range(2))
+    opt = optim.AdamW([a], lr=0.5)
+    with monkeypatch.context() as m:
+        m.setattr(optim._Plan, 'build', lambda self: (_ for _ in ()).throw(MemoryError()))
+        with pytest.raises(MemoryError):
+            opt.add_param_group(dict(params=[b]))
+    assert len(opt.param_groups) == 1 and b not in opt.state
+    opt.add_param_group(dict(params=[b]))
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[b]))              # torch's own check: already in a group
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt.step()
+    assert (a < 1).all() and (b < 1).all() and len(opt.buffers()) == len(opt.param_groups) == 2

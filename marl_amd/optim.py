@@ -27,6 +27,7 @@ BLOCK = 128                       # elements that share the base of their 8-bit 
 _DTYPES = {torch.float32: _hip.F32, torch.bfloat16: _hip.BF16, torch.float16: _hip.F16}
 _dtype = attrgetter('dtype')
 _F32 = torch.finfo(torch.float32)
+_SEED = 0xFFFFFFFFFFFFFFFF
 
 
 def dequantize(codes, base, signed, dtype=torch.float32):
@@ -131,7 +132,8 @@ class AdamW(torch.optim.Optimizer):
     a recording reads the same addresses again, so let them stay (``zero_grad(set_to_none=False)``), and keep the optimizer.
 
     A parameter without a gradient keeps its value and moments (its target still moves); the step count is the group's.
-    ``state_dict`` / ``load_state_dict`` hold the moments as they are stored."""
+    ``state_dict`` / ``load_state_dict`` hold the moments as they are stored, the step counts and the seed: a run that is
+    resumed repeats bit for bit."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None,
                  targets=None, polyak=0.99, seed=0, capturable=False):
@@ -142,10 +144,10 @@ class AdamW(torch.optim.Optimizer):
             if params and isinstance(params[0], dict):
                 raise ValueError("targets: give each parameter group its own 'targets'")
             params = [dict(params=params, targets=list(targets))]
-        self._bits, self._seed, self._capturable = state_bits, int(seed) & 0xFFFFFFFFFFFFFFFF, bool(capturable)
+        self._bits, self._capturable = state_bits, bool(capturable)
         self._plans, self._clocks = [], []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm,
-                                      polyak=polyak, step=0))
+                                      polyak=polyak, step=0, seed=int(seed) & _SEED))
 
     # -- construction ------------------------------------------------------------------------------------------------------
     @staticmethod
@@ -267,7 +269,7 @@ class AdamW(torch.optim.Optimizer):
                 if clock is not None:
                     clock.record_stream(torch.cuda.current_stream(plan.device))
             args = _hip.AdamArgs(group['lr'], *group['betas'], group['eps'], group['weight_decay'], group['max_norm'] or 0.0,
-                                 group['polyak'], group['step'] + 1, _hip.ptr(clock), self._seed, index0, _DTYPES[plan.dtype],
+                                 group['polyak'], group['step'] + 1, _hip.ptr(clock), group['seed'] & _SEED, index0, _DTYPES[plan.dtype],
                                  self._bits)
             _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_step, args, len(plan.params), plan.table,
                                    plan.plan_ptr, plan.grads), 'mpe_adamw_step')

@@ -735,3 +735,28 @@ def test_a_group_that_could_not_be_added_is_not_there(monkeypatch):
     a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
     opt.step()
     assert (a < 1).all() and (b < 1).all() and len(opt.buffers()) == len(opt.param_groups) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('capturable', [False, True])
+def test_a_resumed_run_keeps_its_seed(capturable):
+    """8-bit moments: a run continued by an optimizer of another seed rounds as the first one would have."""
+    p, q = (torch.nn.Parameter(torch.ones(5000, device='cuda')) for _ in range(2))
+    a, b = optim.AdamW([p], state_bits=8, seed=(3 << 40) + 4), optim.AdamW([q], state_bits=8, seed=9, capturable=capturable)
+
+    def go(x, opt, k):
+        x.grad = torch.randn(5000, generator=torch.Generator(device='cuda').manual_seed(k), device='cuda')
+        opt.step()
+    for k in range(2):
+        go(p, a, k)
+    q.data.copy_(p.data)
+    b.load_state_dict(a.state_dict())
+    for k in range(2, 4):
+        go(p, a, k)
+        go(q, b, k)
+    assert all(torch.equal(x, b.buffers()[0][k]) for k, x in a.buffers()[0].items())
+    old = a.state_dict()
+    for g in old['param_groups']:
+        del g['seed']                                        # as before the seed was held
+    b.load_state_dict(old)
+    assert b.param_groups[0]['seed'] == (3 << 40) + 4

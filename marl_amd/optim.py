@@ -16,10 +16,12 @@ each, plus one int16 for 128 of them: a logarithmic code (eighths of a binade; m
 the largest element of its block, rounded stochastically from (seed, step, tensor, element), so that a moment is right on
 average and a run repeats bit for bit.  A gradient that is not finite makes its element (32 bits) or its block of 128
 (8 bits) useless, as it does any Adam."""
+import collections
 import ctypes as C
 from operator import attrgetter
 
 import torch
+from torch.utils.hooks import RemovableHandle
 
 from . import _hip
 
@@ -146,6 +148,7 @@ class AdamW(torch.optim.Optimizer):
             params = [dict(params=params, targets=list(targets))]
         self._bits, self._capturable = state_bits, bool(capturable)
         self._plans, self._clocks = [], []
+        self._before_load, self._after_load = collections.OrderedDict(), collections.OrderedDict()
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm,
                                       polyak=polyak, step=0, seed=int(seed) & _SEED))
 
@@ -317,6 +320,10 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """Settings, step counts and moments of an optimizer with the same groups, shapes and ``state_bits``; the moments are
         copied into this optimizer's arrays, which stay where they are."""
+        state_dict = dict(state_dict)
+        for hook in list(self._before_load.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         groups = state_dict['param_groups']
         if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
             raise ValueError('AdamW: the state dict has other parameter groups')
@@ -335,3 +342,21 @@ class AdamW(torch.optim.Optimizer):
         for i, (group, saved) in enumerate(zip(self.param_groups, groups)):
             group.update({k: v for k, v in saved.items() if k != 'params'})
             self._set_steps(i, saved['step'])
+        for hook in list(self._after_load.values()):
+            hook(self)
+
+    @staticmethod
+    def _add_hook(hooks, hook, prepend):
+        handle = RemovableHandle(hooks)
+        hooks[handle.id] = hook
+        if prepend:
+            hooks.move_to_end(handle.id, last=False)
+        return handle
+
+    def register_load_state_dict_pre_hook(self, hook, prepend=False):
+        """As ``torch.optim.Optimizer``'s: ``hook(optimizer, state_dict)`` before ``load_state_dict``, which takes what it returns."""
+        return self._add_hook(self._before_load, hook, prepend)
+
+    def register_load_state_dict_post_hook(self, hook, prepend=False):
+        """As ``torch.optim.Optimizer``'s: ``hook(optimizer)`` behind ``load_state_dict``."""
+        return self._add_hook(self._after_load, hook, prepend)

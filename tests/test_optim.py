@@ -760,3 +760,23 @@ def test_a_resumed_run_keeps_its_seed(capturable):
         del g['seed']                                        # as before the seed was held
     b.load_state_dict(old)
     assert b.param_groups[0]['seed'] == (3 << 40) + 4
+
+
+@pytest.mark.gpu
+def test_load_hooks_run():
+    p = torch.nn.Parameter(torch.ones(300, device='cuda'))
+    p.grad = torch.ones_like(p)
+    opt, seen = optim.AdamW([p], lr=0.5), []
+    opt.step()
+    saved = opt.state_dict()
+
+    def halve(o, d):
+        seen.append('halve')
+        return dict(d, param_groups=[dict(g, lr=g['lr'] / 2) for g in d['param_groups']])
+    opt.register_load_state_dict_pre_hook(halve)
+    opt.register_load_state_dict_pre_hook(lambda o, d: seen.append('first'), prepend=True)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append((o is opt, o.param_groups[0]['lr'])))
+    gone = opt.register_load_state_dict_post_hook(lambda o: seen.append('gone'))
+    gone.remove()
+    opt.load_state_dict(saved)
+    assert seen == ['first', 'halve', (True, 0.25)] and saved['param_groups'][0]['lr'] == 0.5

@@ -397,6 +397,7 @@ class CapturedLearners(object):
             tr.replay_sample_index = idx
 
     def replay(self):
+        self.learners.check()
         self._draw()
         self.graph.replay()
         return self.last

@@ -9,7 +9,8 @@ One difference from the loop over trainers: every learner's targets come from th
 update.  In the loop learner i already sees the target policies of learners < i moved by their polyak step of 1 %.
 
 The trainers' networks become views of the stacked arrays (weights of narrower agents are padded with zeros, which stay
-zero), so acting, ``act_all`` and the trainers' own methods go on as before; the step is AdamW with ``weight_decay`` 0 unless
+zero), so acting, ``act_all`` and the trainers' own methods go on as before (an update finds and refuses networks that were
+taken out of the stacks since, as a second ``Learners`` of the same trainers does); the step is AdamW with ``weight_decay`` 0 unless
 given, which is the trainers' Adam.  Moments live here, not in the trainers' ``p_opt`` / ``q_opt``: use one or the other."""
 import torch
 from torch import nn
@@ -17,6 +18,9 @@ from torch import nn
 from . import maddpg
 from .grouped import grouped_linear, grouped_linear_backward, group_ends
 from .optim import AdamW
+
+
+NETS = ('p', 'q', 'target_p', 'target_q')          # a trainer's networks
 
 
 def _linears(net):
@@ -33,7 +37,7 @@ class _Stack(object):
         layers = list(zip(*[_linears(net) for net in nets]))
         if any(len({m.out_features for m in layer}) != 1 for layer in layers[:2]):
             raise NotImplementedError('Learners: networks of one hidden width are supported')
-        self.w, self.b, self.n = [], [], len(nets)
+        self.w, self.b, self.n, self.nets = [], [], len(nets), list(nets)
         for k, layer in enumerate(layers):
             w0 = layer[0].weight
             if any(m.weight.dtype != torch.float32 or m.weight.device != w0.device for m in layer):
@@ -50,6 +54,13 @@ class _Stack(object):
                 m.bias.data = b[i, :m.out_features]
             self.w.append(w)
             self.b.append(b)
+        self.params = [t for net in nets for t in net.parameters()]
+        self.at = [t.data_ptr() for t in self.params]
+
+    def check(self, nets):
+        """The networks' variables are still this stack's memory."""
+        if any(a is not b for a, b in zip(nets, self.nets)) or list(map(torch.Tensor.data_ptr, self.params)) != self.at:
+            raise RuntimeError('Learners: a network was replaced or its variables moved (.to(), .data, other Learners): build Learners anew')
 
     def variables(self):
         """Every network's variables, each a contiguous tensor of its own (clipping is per variable)."""
@@ -148,6 +159,11 @@ class Learners(object):
             return torch.cat([self._wide([self._rows(obs_n[i], i), self._rows(act_n[i], i)], width) for i in range(self.n)])
         return self._wide(list(obs_n) + list(act_n), width)
 
+    def check(self):
+        """Raises where a trainer's networks are no longer the ones that are updated here."""
+        for name in NETS:
+            getattr(self, name).check([getattr(tr, name) for tr in self.trainers])
+
     def draw(self):
         """Every learner's batch indices, [n, batch]."""
         return torch.stack([tr.replay_buffer.make_index(self.batch) for tr in self.trainers])
@@ -172,6 +188,7 @@ class Learners(object):
         n, b = self.n, self.batch
         if tuple(index.shape) != (n, b):
             raise ValueError('Learners: index is [%d, %d], got %s' % (n, b, list(index.shape)))
+        self.check()
         flat = index.reshape(-1)
         obs_n, act_n, rew_n, next_n, done_n = zip(*[tr.replay_buffer.sample_index(flat) for tr in self.trainers])   # maddpg.py:173-177
         rew = torch.cat([self._rows(r, i) for i, r in enumerate(rew_n)])

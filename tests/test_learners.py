@@ -169,3 +169,29 @@ def test_networks_and_trainers_that_do_not_fit_are_refused():
     with pytest.raises(RuntimeError):
         CapturedLearners(learners)
     assert Learners(make(n=1)).n == 1
+
+
+def test_networks_that_left_the_stacks_are_refused():
+    """A second Learners takes the networks over: the first one's updates, eager or recorded, would change arrays that nobody acts
+    with.  The same for a network that was replaced or whose variables were."""
+    from marl_amd.graph import CapturedLearners
+    from marl_amd.learners import Learners
+    _, trainers = _setup()
+    first = Learners(trainers)
+    cap = CapturedLearners(first)
+    cap.replay()
+    second = Learners(trainers)
+    w = trainers[0].p[0].weight.detach().clone()
+    for call in (lambda: first.update(100), cap.replay, lambda: CapturedLearners(first)):
+        with pytest.raises(RuntimeError, match='build Learners anew'):
+            call()
+    assert torch.equal(trainers[0].p[0].weight, w)
+    assert second.update(100) is not None and not torch.equal(trainers[0].p[0].weight, w)
+    trainers[1].q[2].bias.data = trainers[1].q[2].bias.data.clone()
+    with pytest.raises(RuntimeError, match='build Learners anew'):
+        second.update(200)
+    third = Learners(trainers)
+    assert third.update(200) is not None
+    trainers[2].target_p = mlp_model(trainers[2].p[0].in_features, 5).cuda()
+    with pytest.raises(RuntimeError, match='build Learners anew'):
+        third.update(300)

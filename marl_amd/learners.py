@@ -11,7 +11,8 @@ update.  In the loop learner i already sees the target policies of learners < i 
 The trainers' networks become views of the stacked arrays (weights of narrower agents are padded with zeros, which stay
 zero), so acting, ``act_all`` and the trainers' own methods go on as before (an update finds and refuses networks that were
 taken out of the stacks since, as a second ``Learners`` of the same trainers does); the step is AdamW with ``weight_decay`` 0 unless
-given, which is the trainers' Adam.  Moments live here, not in the trainers' ``p_opt`` / ``q_opt``: use one or the other."""
+given, which is the trainers' Adam.  Moments live here (``Learners.p_opt`` / ``.q_opt``; they begin as the trainers' own, in 8 bits
+rounded), not in the trainers' ``p_opt`` / ``q_opt``, which stay as they were: use one or the other."""
 import torch
 from torch import nn
 
@@ -101,6 +102,13 @@ class Learners(object):
         if len({(tr.local_q_func, tr.args.batch_size, tr.args.lr, tr.args.gamma, tr.grad_norm_clipping, str(tr.device))
                 for tr in self.trainers}) != 1:
             raise NotImplementedError('Learners: trainers that share local_q_func, batch size, lr, gamma, clipping and device')
+        steps = {}
+        for kind in 'pq':
+            taken = {int(getattr(tr, kind + '_opt').state.get(t, {}).get('step', 0))
+                     for tr in self.trainers for t in getattr(tr, kind).parameters()}
+            if len(taken) != 1:
+                raise ValueError('Learners: the trainers have taken unlike numbers of steps: %s' % sorted(taken))
+            steps[kind] = taken.pop()
         self.device, self.batch, self.gamma, self.local = t0.device, t0.args.batch_size, t0.args.gamma, t0.local_q_func
         self.sizes = t0.sizes_n
         self.acts = [sum(s) for s in self.sizes]
@@ -110,6 +118,8 @@ class Learners(object):
                   polyak=1.0 - 1e-2, capturable=True)
         self.p_opt = AdamW(self.p.variables(), targets=self.target_p.variables(), seed=2 * seed, **kw)
         self.q_opt = AdamW(self.q.variables(), targets=self.target_q.variables(), seed=2 * seed + 1, **kw)
+        self._adopt(steps['p'], [tr.p_opt for tr in self.trainers], self.p, self.p_opt)
+        self._adopt(steps['q'], [tr.q_opt for tr in self.trainers], self.q, self.q_opt)
         b = self.batch
         self.ends = group_ends([b] * n, self.device)            # learner i's batch: rows i b .. (i + 1) b
         self.ends_all = group_ends([n * b] * n, self.device)    # agent j's observations of every learner's batch
@@ -123,6 +133,22 @@ class Learners(object):
         for i, s in enumerate(self.sizes):
             self.alike.setdefault(tuple(s), []).append(i)
         self.alike = [(list(s), torch.tensor(who, device=self.device)) for s, who in self.alike.items()]
+
+    @staticmethod
+    def _adopt(steps, opts, stack, opt):
+        """The step count and the moments of the trainers' own optimizers."""
+        if steps == 0:
+            return
+        states = [[o.state[t] for t in net.parameters()] for o, net in zip(opts, stack.nets)]
+        opt.step_count = steps
+        shapes = [p.shape for p in opt.param_groups[0]['params']]
+        for j, shape in enumerate(shapes):                      # variables as stacked: by layer, weight then bias, every network
+            st = states[j % stack.n][j // stack.n]
+            whole = []
+            for key in ('exp_avg', 'exp_avg_sq'):
+                whole.append(torch.zeros(shape, device=st[key].device))
+                whole[-1][tuple(slice(c) for c in st[key].shape)] = st[key]
+            opt._plans[0].set_moments(j, *whole)
 
     def _sample(self, logits):
         """Every agent's soft sample of its [rows, most] logits [n, rows, most]; columns it does not have are zero."""

@@ -50,6 +50,16 @@ def dequantize(codes, base, signed, dtype=torch.float32):
     return out
 
 
+def _encode(x, signed):
+    """Moments in 32 bits as codes and bases of 8 (rounded to nearest; a step rounds as the kernel does): ``x`` float32, flat."""
+    x = torch.nn.functional.pad(x, (0, -x.numel() % BLOCK))
+    top, bits = 127 if signed else 255, (x.view(torch.int32) & 0x7FFFFFFF).to(torch.int64)
+    base = ((bits >> 20).view(-1, BLOCK).amax(1) + 1 - top).clamp_(min=0)
+    code = (torch.clamp(bits + (1 << 19), max=0x7FFFFFFF) >> 20) - base.repeat_interleave(BLOCK)
+    code = code.clamp_(min=0) | (x < 0).to(torch.int64) << 7 if signed else torch.maximum(code, (bits > 0).to(torch.int64))
+    return code.to(torch.uint8), base.to(torch.int16)
+
+
 class _Plan(object):
     """One parameter group: its flat moments and what the kernels read about its variables."""
 
@@ -88,6 +98,17 @@ class _Plan(object):
             else:
                 out[name] = t[o:o + c].view(self.params[j].shape)
         return out
+
+    def set_moments(self, j, exp_avg, exp_avg_sq):
+        """Variable j's moments from float32 values of its shape."""
+        for name, value in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
+            have, value = self.views(j), value.to(self.device, torch.float32)
+            if self.bits == 32:
+                have[name].copy_(value)
+            else:
+                code, base = _encode(value.reshape(-1), name == 'exp_avg')
+                have[name].view(-1).copy_(code[:self.counts[j]])
+                have[name + '_base'].copy_(base)
 
     def build(self):
         """The host table of pointers and its device plan."""

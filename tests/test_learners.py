@@ -195,3 +195,42 @@ def test_networks_that_left_the_stacks_are_refused():
     trainers[2].target_p = mlp_model(trainers[2].p[0].in_features, 5).cuda()
     with pytest.raises(RuntimeError, match='build Learners anew'):
         third.update(300)
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_learners_of_trained_trainers_go_on_with_their_moments(bits, monkeypatch):
+    """Two updates of every trainer, then Learners: moments (8 bits: to half an eighth of a binade, or under the block's range,
+    2^-15 of its largest) and step count are the trainers', in their places; trainers with unlike step counts are refused."""
+    from marl_amd.learners import Learners
+    _fixed(monkeypatch)
+    _, trainers = _setup('S1L2F2_3Targets_100observe')
+    for k in range(2):
+        index = _index(trainers, k)
+        for i, tr in enumerate(trainers):
+            tr.update_from_index(trainers, index[i])
+    learners = Learners(trainers, state_bits=bits)
+    n = len(trainers)
+    for kind in 'pq':
+        opt = getattr(learners, kind + '_opt')
+        assert opt.step_count == 2
+        flats = opt.moments()[0]
+        for i, tr in enumerate(trainers):
+            for v, t in enumerate(getattr(tr, kind).parameters()):
+                plan, j = opt._plans[0], v * n + i
+                o, c, shape = plan.first[j], plan.counts[j], plan.params[j].shape
+                for key, flat in zip(('exp_avg', 'exp_avg_sq'), flats):
+                    got = flat[o:o + c].view(shape)
+                    part, want = got[tuple(slice(s) for s in t.shape)], getattr(tr, kind + '_opt').state[t][key]
+                    assert int((part != 0).sum()) == int((got != 0).sum())
+                    if bits == 32:
+                        assert torch.equal(part, want)
+                    else:
+                        assert bool(((part - want).abs() <= want.abs() / 16 + 2.0 ** -15 * want.abs().max()).all())
+    learners.update_from_index(_index(trainers, 2))
+    assert learners.p_opt.step_count == learners.q_opt.step_count == 3
+    _, trainers = _setup()
+    trainers[0].update_from_index(trainers, _index(trainers, 0)[0])
+    at = [t.data_ptr() for tr in trainers for t in tr.p.parameters()]
+    with pytest.raises(ValueError, match='unlike numbers of steps'):
+        Learners(trainers)
+    assert at == [t.data_ptr() for tr in trainers for t in tr.p.parameters()]

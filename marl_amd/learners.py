@@ -12,7 +12,8 @@ The trainers' networks become views of the stacked arrays (weights of narrower a
 zero), so acting, ``act_all`` and the trainers' own methods go on as before (an update finds and refuses networks that were
 taken out of the stacks since, as a second ``Learners`` of the same trainers does); the step is AdamW with ``weight_decay`` 0 unless
 given, which is the trainers' Adam.  Moments live here (``Learners.p_opt`` / ``.q_opt``; they begin as the trainers' own, in 8 bits
-rounded), not in the trainers' ``p_opt`` / ``q_opt``, which stay as they were: use one or the other."""
+rounded), not in the trainers' ``p_opt`` / ``q_opt``, which stay as they were: use one or the other,
+and save a run with ``Learners.state_dict`` (the trainers' optimizers no longer hold what a resumed run needs)."""
 import torch
 from torch import nn
 
@@ -22,6 +23,7 @@ from .optim import AdamW
 
 
 NETS = ('p', 'q', 'target_p', 'target_q')          # a trainer's networks
+OPTS = ('p_opt', 'q_opt')
 
 
 def _linears(net):
@@ -185,6 +187,40 @@ class Learners(object):
             return torch.cat([self._wide([self._rows(obs_n[i], i), self._rows(act_n[i], i)], width) for i in range(self.n)])
         return self._wide(list(obs_n) + list(act_n), width)
 
+    def state_dict(self):
+        """What a run needs to go on, copied: the networks (of every trainer, unpadded), the moments, step counts and settings.
+        (The trainers' networks lie in shared arrays: ``torch.save`` of one's own ``state_dict`` writes all of them.)"""
+        nets = {name: [{k: v.detach().clone() for k, v in net.state_dict().items()} for net in getattr(self, name).nets]
+                for name in NETS}
+        out = {'networks': nets}
+        for name in OPTS:
+            d = getattr(self, name).state_dict()
+            out[name] = dict(d, state={j: {k: v.clone() for k, v in st.items()} for j, st in d['state'].items()})
+        return out
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """Takes over a ``state_dict`` of Learners with the same networks and ``state_bits``; the arrays stay where they are, so
+        a recording goes on with them."""
+        self.check()
+        have = {name: [net.state_dict() for net in getattr(self, name).nets] for name in NETS}
+        for name in NETS:
+            got = state_dict['networks'][name]
+            if [{k: v.shape for k, v in d.items()} for d in got] != [{k: v.shape for k, v in d.items()} for d in have[name]]:
+                raise ValueError('Learners: the state dict is of other networks (%s)' % name)
+        for name in OPTS:
+            getattr(self, name).load_state_dict(state_dict[name])
+        for name in NETS:
+            for mine, got in zip(have[name], state_dict['networks'][name]):
+                for k, v in mine.items():
+                    v.copy_(got[k])
+        self._repack()
+
+    def _repack(self):
+        for tr in self.trainers:                                # refilled in place: recorded acting steps read it
+            if tr._packed is not None:
+                maddpg.pack_actor(tr.p, out=tr._packed)
+
     def check(self):
         """Raises where a trainer's networks are no longer the ones that are updated here."""
         for name in NETS:
@@ -251,9 +287,7 @@ class Learners(object):
         dlogits = self._softmax_backward(sample, da) + logits * self.real.unsqueeze(1) * (2e-3 / b / width)
         p_loss = -acts[3].view(n, b).mean(1) + 1e-3 * (logits.square() * self.real.unsqueeze(1)).sum((1, 2)) / (b * width.view(n))
         self._step(self.p_opt, self.p.gradients(pol, dlogits.reshape(n * b, -1), self.ends))
-        for tr in self.trainers:
-            if tr._packed is not None:
-                maddpg.pack_actor(tr.p, out=tr._packed)
+        self._repack()
 
         tq, tn = target.view(n, b), target_next.view(n, b)
         stats = torch.stack([q_loss, p_loss, tq.mean(1), rew.view(n, b).mean(1), tn.mean(1), tq.std(1, unbiased=False)], 1)

@@ -234,3 +234,59 @@ def test_learners_of_trained_trainers_go_on_with_their_moments(bits, monkeypatch
     with pytest.raises(ValueError, match='unlike numbers of steps'):
         Learners(trainers)
     assert at == [t.data_ptr() for tr in trainers for t in tr.p.parameters()]
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_saved_run_goes_on_as_if_it_had_not_stopped(bits, monkeypatch):
+    """Two updates, saved to a file's bytes and loaded by Learners of other random networks and another seed (its acting weights
+    packed before): the next updates, eager and recorded, equal the uninterrupted run's bit for bit."""
+    import io
+
+    from marl_amd.graph import CapturedLearners
+    from marl_amd.learners import Learners
+    _fixed(monkeypatch)
+    (env, ta), (_, tb) = _setup('S1L2F2_3Targets_100observe'), _setup('S1L2F2_3Targets_100observe')
+    for tr in tb:
+        for name in NETS:
+            for t in getattr(tr, name).parameters():
+                t.data.mul_(0.5)
+    la, lb = Learners(ta, state_bits=bits, seed=3), Learners(tb, state_bits=bits, seed=8)
+    for k in range(2):
+        la.update_from_index(_index(ta, k))
+    saved = la.state_dict()
+    file = io.BytesIO()
+    torch.save(saved, file)
+    held = sum(t.numel() * t.element_size() for tr in ta for name in NETS for t in getattr(tr, name).parameters())
+    assert len(file.getvalue()) < 2.5 * held + (1 << 20)                    # networks and moments, once
+    file.seek(0)
+    lb.load_state_dict(torch.load(file, weights_only=True))
+    cap = None
+    for k in range(2, 5):
+        want = [[float(x) for x in row] for row in la.update_from_index(_index(ta, k))]
+        if k == 3:
+            lb.draw = lambda: _index(tb, 3)
+            cap = CapturedLearners(lb)
+            got = cap.last
+        elif k == 4:
+            lb.draw = lambda: _index(tb, 4)
+            got = cap.replay()
+        else:
+            got = lb.update_from_index(_index(tb, k))
+        assert want == [[float(x) for x in row] for row in got], k
+    for a, b in zip(ta, tb):
+        for n in NETS:
+            assert all(torch.equal(x, y) for x, y in zip(getattr(a, n).parameters(), getattr(b, n).parameters())), n
+    lb.load_state_dict(saved)                                               # back to the saved state, which stayed as it was
+    got = [[float(x) for x in row] for row in cap.replay()]
+    la.load_state_dict(saved)
+    assert got == [[float(x) for x in row] for row in la.update_from_index(_index(ta, 4))]
+    assert la.p_opt.step_count == lb.p_opt.step_count == 3
+    for tr in tb:
+        assert torch.equal(tr._packed, maddpg.pack_actor(tr.p))
+    other = Learners(_setup()[1], state_bits=bits)
+    with pytest.raises(ValueError):
+        other.load_state_dict(saved)
+    before = [t.clone() for t in tb[0].p.parameters()]
+    with pytest.raises(ValueError):
+        lb.load_state_dict(dict(saved, networks=dict(saved['networks'], p=saved['networks']['q'])))
+    assert all(torch.equal(x, y) for x, y in zip(before, tb[0].p.parameters()))

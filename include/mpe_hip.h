@@ -573,8 +573,8 @@ int mpe_env_step_stats_static(const mpe_scenario_desc *desc, int64_t B, int64_t 
  * a call whose results are more than 2^23 - 8 tiles (64 x 64 and larger, a group's last one may be partial) is refused.
  * mpe_grouped_linear_workspace / mpe_grouped_backward_workspace: bytes that a call with these arrays needs (>= 0, or
  * MPE_ERR_*; no memory is read); the array is scratch of that call, 16-byte aligned; calls that may overlap (other streams,
- * concurrent graph replays) need one each.  What needs scratch: y beside large products, rows that lie 2^20 elements or more
- * apart, and dweight where its sums are split over the rows.
+ * concurrent graph replays) need one each.  What needs scratch: y beside large products, rows of x, dy or y that lie about
+ * 2^23 bytes (a tile's copies reach 2^31) or more apart, and dweight where its sums are split over the rows.
  */
 #define MPE_F32 0
 #define MPE_BF16 1

@@ -10,7 +10,9 @@ namespace {
 
 constexpr int kMaxGroups = 1024, kMaxWidth = 1 << 20;
 constexpr int64_t kMaxGrid = (1 << 23) - 1;  // workgroups: a launch has less than 2^32 threads, a workgroup up to 512
-static_assert((int64_t)kMaxWidth * 4 * 256 < (int64_t)kGroupedSpan, "a tile of packed rows spans less than a copy may reach");
+// rows this far apart (elements of `size` bytes): a tile of 256 of them spans less than a copy may reach
+constexpr bool copyable(int64_t ld, int size) { return ld < (int64_t)kGroupedSpan / (256 * size) - 16; }
+static_assert(copyable(kMaxWidth, 4) && copyable(kMaxWidth, 2), "packed rows and weights always are");
 
 int dtype_size(int dtype) { return dtype == MPE_F32 ? 4 : 2; }
 bool bad_align(const void *p, int size) { return p != nullptr && (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; }
@@ -47,7 +49,6 @@ struct Workspace {
 
   int chunk() const { return 16 / size; }
   int64_t packed_ld(const Matrix &m) const { return (m.cols + chunk() - 1) / chunk() * chunk(); }
-  bool copyable(int64_t ld) const { return ld < (int64_t)kGroupedSpan / (256 * size) - 16; }
   int64_t take(int64_t bytes) {
     const int64_t at = total;
     total += (bytes + 15) / 16 * 16;
@@ -55,7 +56,7 @@ struct Workspace {
   }
   // masks: the kernel that reads m applies its mask
   void plan(Matrix &m, bool masks = false) {
-    const bool as_it_is = copyable(m.ld) && (!m.mask || (masks && copyable(m.ld_mask)));
+    const bool as_it_is = copyable(m.ld, size) && (!m.mask || (masks && copyable(m.ld_mask, size)));
     m.at = m.lines > 0 && !as_it_is ? take(m.lines * packed_ld(m) * size) : -1;
   }
   // after the plan: the matrix as the kernels read it
@@ -216,33 +217,27 @@ GroupedArgs base_args(const mpe_grouped_desc *d) {
 }
 
 Matrix rows_of(const mpe_grouped_desc *d, const void *p, int64_t ld, int cols) { return Matrix{p, nullptr, ld, 0, d->rows, -1, cols}; }
-Matrix weight_of(const mpe_grouped_desc *d, const void *p) { return Matrix{p, nullptr, d->k, 0, (int64_t)d->groups * d->n, -1, d->k}; }
 
 struct Forward {
-  Matrix x, w;
+  Matrix x;
   Workspace ws;
-  Forward(const mpe_grouped_desc *d, const void *px, int64_t ld_x, const void *pw)
-      : x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)} {
-    ws.plan(x);
-    ws.plan(w);
-  }
+  Forward(const mpe_grouped_desc *d, const void *px, int64_t ld_x) : x(rows_of(d, px, ld_x, d->k)), ws{dtype_size(d->dtype)} { ws.plan(x); }
 };
 
 // The gradient of the result, the operands that are wanted, and the partial sums of dweight and dbias.
 struct Backward {
-  Matrix d_, x, w;
+  Matrix d_, x;
   Workspace ws;
   bool small;  // all tiles: one launch, which applies the mask itself
   int64_t part = 0, part_bias = 0;
-  Backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, const void *px, int64_t ld_x,
-           const void *pw, bool dx, bool dw)
-      : d_(rows_of(d, dy, ld_dy, d->n)), x(rows_of(d, px, ld_x, d->k)), w(weight_of(d, pw)), ws{dtype_size(d->dtype)},
+  Backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y, const void *px, int64_t ld_x, bool dx,
+           bool dw)
+      : d_(rows_of(d, dy, ld_dy, d->n)), x(rows_of(d, px, ld_x, d->k)), ws{dtype_size(d->dtype)},
         small((!dx || rows_tile(d, d->k) == SMALL) && (!dw || dw_tile(d) == SMALL)) {
     d_.mask = y;
     d_.ld_mask = ld_y;
     if (dx || dw) ws.plan(d_, small && d->k <= kMaskCols);
     if (dw) ws.plan(x);
-    if (dx) ws.plan(w);
     const int splits = dw_splits(d);
     if (dw && splits > 1) {
       const int64_t one = (int64_t)splits * d->groups * d->n * 4;
@@ -254,9 +249,9 @@ struct Backward {
 
 }  // namespace
 
-extern "C" int64_t mpe_grouped_linear_workspace(const mpe_grouped_desc *d, const void *x, int64_t ld_x, const void *weight) {
+extern "C" int64_t mpe_grouped_linear_workspace(const mpe_grouped_desc *d, const void *x, int64_t ld_x, const void * /*weight*/) {
   if (const int rc = grouped_check(d)) return rc;
-  return Forward(d, x, ld_x, weight).ws.total;
+  return Forward(d, x, ld_x).ws.total;
 }
 
 extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int64_t ld_x, const void *weight, const void *bias,
@@ -272,18 +267,17 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
   for (const void *p : {x, weight, bias, (const void *)y})
     if (bad_align(p, size)) return MPE_ERR_ALIGN;
   if (bad_align(workspace, 16)) return MPE_ERR_ALIGN;
-  Forward f(d, x, ld_x, weight);
+  Forward f(d, x, ld_x);
   if (f.ws.total > 0 && !workspace) return MPE_ERR_NULL;
   if (workspace_bytes < f.ws.total) return MPE_ERR_SCRATCH;
   hipStream_t s = (hipStream_t)stream;
   f.ws.place(f.x, workspace);
-  f.ws.place(f.w, workspace);
   if (const int rc = f.ws.run(d->dtype, s)) return rc;
   GroupedArgs a = base_args(d);
   a.a = f.x.p;
   a.ld_a = f.x.ld;
-  a.b = f.w.p;
-  a.ld_b = f.w.ld;
+  a.b = weight;
+  a.ld_b = d->k;
   a.bias = bias;
   a.out = y;
   a.ld_out = ld_y;
@@ -293,10 +287,10 @@ extern "C" int mpe_grouped_linear(const mpe_grouped_desc *d, const void *x, int6
 }
 
 extern "C" int64_t mpe_grouped_backward_workspace(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
-                                                  const void *x, int64_t ld_x, const void *weight, int with_dx, int with_dweight) {
+                                                  const void *x, int64_t ld_x, const void * /*weight*/, int with_dx, int with_dweight) {
   if (const int rc = grouped_check(d)) return rc;
   if (with_dx < 0 || with_dx > 1 || with_dweight < 0 || with_dweight > 1) return MPE_ERR_ARG;
-  return Backward(d, dy, ld_dy, y, ld_y, x, ld_x, weight, with_dx, with_dweight).ws.total;
+  return Backward(d, dy, ld_dy, y, ld_y, x, ld_x, with_dx, with_dweight).ws.total;
 }
 
 extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void *dy, int64_t ld_dy, const void *y, int64_t ld_y,
@@ -311,13 +305,12 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   for (const void *p : {dy, y, x, weight, (const void *)dx, (const void *)dweight, (const void *)dbias})
     if (bad_align(p, size)) return MPE_ERR_ALIGN;
   if (bad_align(workspace, 16)) return MPE_ERR_ALIGN;
-  Backward b(d, dy, ld_dy, y, ld_y, x, ld_x, weight, dx != nullptr, dweight != nullptr);
+  Backward b(d, dy, ld_dy, y, ld_y, x, ld_x, dx != nullptr, dweight != nullptr);
   if (b.ws.total > 0 && !workspace) return MPE_ERR_NULL;
   if (workspace_bytes < b.ws.total) return MPE_ERR_SCRATCH;
   hipStream_t s = (hipStream_t)stream;
   b.ws.place(b.d_, workspace);
   b.ws.place(b.x, workspace);
-  b.ws.place(b.w, workspace);
   if (const int rc = b.ws.run(d->dtype, s)) return rc;
   GroupedArgs a = base_args(d);
   a.a = b.d_.p;
@@ -326,8 +319,8 @@ extern "C" int mpe_grouped_linear_backward(const mpe_grouped_desc *d, const void
   a.ld_mask = b.d_.ld_mask;
   GroupedArgs gx = a, gw = a;
   if (dx && d->rows > 0) {
-    gx.b = b.w.p;
-    gx.ld_b = b.w.ld;
+    gx.b = weight;
+    gx.ld_b = d->k;
     gx.out = dx;
     gx.ld_out = ld_dx;
     gx.zero_tail = zero_tail;

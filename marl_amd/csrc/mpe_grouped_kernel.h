@@ -630,7 +630,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN <= 4 ? 2 : 1) void grouped_bo
 // Copies matrices into rows of whole chunks where their stride is too large for a tile's copies, and applies relu's mask to dy
 // on the way: d = dy where y is not <= 0, zero elsewhere.
 struct GroupedPack { const void *src, *mask; void *dst; int64_t ld, ld_mask, lines; int32_t cols, blocks; };
-struct GroupedPacks { GroupedPack job[3]; };
+struct GroupedPacks { GroupedPack job[2]; };  // x, dy
 
 // the chunk at element off, valid of it kept; end: elements of the whole matrix (a chunk may reach into the next line)
 template <typename T>
@@ -651,7 +651,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void grouped_pack_kernel(GroupedPacks a) {
   constexpr int CE = 16 / sizeof(T);
   uint32_t b = blockIdx.x, k = 0;
-  while (k < 2 && b >= (uint32_t)a.job[k].blocks) b -= a.job[k++].blocks;
+  if (b >= (uint32_t)a.job[0].blocks) b -= a.job[k++].blocks;
   const GroupedPack &j = a.job[k];
   // a workgroup: some whole lines of up to 256 chunks, or up to 256 chunks of one line; one chunk a thread
   const uint32_t chunks = (uint32_t)((j.cols + CE - 1) / CE), t = threadIdx.x;

@@ -478,3 +478,18 @@ def test_autograd_notices_a_write_to_out():
     with torch.inference_mode():
         again = grouped.grouped_linear(x, w, ends, bias=b, out=torch.empty(7, 5, device='cuda'))
     assert torch.equal(grows, out) and torch.equal(again, out)
+
+
+@pytest.mark.parametrize('dtype,size', [(_hip.F32, 4), (_hip.BF16, 2), (_hip.F16, 2)])
+def test_what_is_packed_into_scratch(dtype, size):
+    """Rows that lie further apart than 2^23 bytes less 100, and nothing else: the widest weight is read where it lies."""
+    L, p, far = _hip.lib, 1 << 20, (1 << 23) // size
+    d, wide = _desc(dtype=dtype), _desc(dtype=dtype, n=2047, k=1 << 20, groups=4)
+    for ld, packed in ((3, False), (far - 100, False), (far, True)):
+        assert (L.mpe_grouped_linear_workspace(d, p, ld, p) > 0) == packed
+        assert (L.mpe_grouped_backward_workspace(d, p, 5, None, 0, p, ld, p, 1, 1) > 0) == packed
+        assert (L.mpe_grouped_backward_workspace(d, p, ld + 5, None, 0, p, 3, p, 1, 0) > 0) == packed
+        assert (L.mpe_grouped_backward_workspace(d, p, 5, p, ld + 5, p, 3, p, 1, 0) > 0) == packed
+        assert L.mpe_grouped_backward_workspace(d, p, 5, None, 0, p, ld, p, 1, 0) == 0       # x is not read
+    assert L.mpe_grouped_linear_workspace(wide, p, 1 << 20, p) == 0
+    assert L.mpe_grouped_backward_workspace(wide, p, 2047, None, 0, p, 1 << 20, p, 1, 0) == 0

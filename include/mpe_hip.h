@@ -227,6 +227,8 @@ typedef struct mpe_buffers {
                         not NULL; ignored otherwise */
 } mpe_buffers;
 
+/* MPE_ABI_VERSION of the library.  It names the structs and the functions up to mpe_replay_gather_steps_*; the grouped products and
+   AdamW below were added to the same version: a caller that may meet an older build looks their names up. */
 int mpe_abi_version(void);
 const char *mpe_strerror(int code);
 /* sizeof(mpe_scenario_desc) as compiled into the library (bindings check their struct layout). */

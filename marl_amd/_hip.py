@@ -149,10 +149,18 @@ def _load():
             'marl_amd: %s not found. Build it with `make -C marl_amd/csrc` (hipcc, gfx950); '
             'there is no CPU fallback.' % _LIB_PATH)
     L = C.CDLL(_LIB_PATH)
+    try:
+        L.mpe_abi_version.restype, L.mpe_abi_version.argtypes = C.c_int, []
+        if L.mpe_abi_version() != ABI_VERSION:
+            raise ImportError('marl_amd: libmpe_hip.so ABI %d != expected %d' % (L.mpe_abi_version(), ABI_VERSION))
+        return _bind(L)
+    except AttributeError as e:      # an older build of the same ABI: functions are added without raising it
+        raise ImportError('marl_amd: %s lacks a function (%s); build it again with `make -C marl_amd/csrc`' % (_LIB_PATH, e)) from None
+
+
+def _bind(L):
     vp, i64, u64, u32, ci = C.c_void_p, C.c_int64, C.c_uint64, C.c_uint32, C.c_int
     dp = C.POINTER(ScenarioDesc)
-    L.mpe_abi_version.restype = ci
-    L.mpe_abi_version.argtypes = []
     L.mpe_strerror.restype = C.c_char_p
     L.mpe_strerror.argtypes = [ci]
     bp = C.POINTER(Buffers)
@@ -230,8 +238,6 @@ def _load():
     L.mpe_buffers_sizeof.argtypes = []
     L.mpe_residency_plan.restype = ci
     L.mpe_residency_plan.argtypes = [C.POINTER(ScenarioDesc), i64, ci]
-    if L.mpe_abi_version() != ABI_VERSION:
-        raise ImportError('marl_amd: libmpe_hip.so ABI %d != expected %d' % (L.mpe_abi_version(), ABI_VERSION))
     if L.mpe_desc_sizeof() != C.sizeof(ScenarioDesc):
         raise ImportError('marl_amd: mpe_scenario_desc layout mismatch (%d vs %d bytes)'
                           % (L.mpe_desc_sizeof(), C.sizeof(ScenarioDesc)))

@@ -493,3 +493,20 @@ def test_what_is_packed_into_scratch(dtype, size):
         assert L.mpe_grouped_backward_workspace(d, p, 5, None, 0, p, ld, p, 1, 0) == 0       # x is not read
     assert L.mpe_grouped_linear_workspace(wide, p, 1 << 20, p) == 0
     assert L.mpe_grouped_backward_workspace(wide, p, 2047, None, 0, p, 1 << 20, p, 1, 0) == 0
+
+
+@pytest.mark.parametrize('version,says', [(_hip.ABI_VERSION, 'lacks a function'), (_hip.ABI_VERSION - 1, 'ABI %d != expected' % (_hip.ABI_VERSION - 1))])
+def test_an_older_library_is_refused_in_words(version, says, tmp_path):
+    """One of the same ABI without the later functions, and one of an older ABI, which is told first."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    if shutil.which('gcc') is None:
+        pytest.skip('no C compiler')
+    (tmp_path / 'old.c').write_text('int mpe_abi_version(void) { return %d; }' % version)
+    subprocess.run(['gcc', '-shared', '-fPIC', '-o', str(tmp_path / 'old.so'), str(tmp_path / 'old.c')], check=True)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(_hip.__file__)))
+    run = subprocess.run([sys.executable, '-c', 'import marl_amd._hip'], cwd=root, capture_output=True, text=True,
+                         env=dict(os.environ, MARL_AMD_LIB=str(tmp_path / 'old.so')))
+    assert run.returncode == 1 and 'ImportError' in run.stderr and says in run.stderr

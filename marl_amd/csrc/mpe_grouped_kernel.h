@@ -391,9 +391,9 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
   // 2-byte elements in lines of odd width: an array's last element is half of a dword that the buffer's bounds cut off, and its copy
   // brings zero.  The thread of that copy puts it in place before its stage is multiplied (adding its product afterwards would not
   // undo a zero times an infinity).  fill_*: how far from c0 the element is multiplied, or -1; put_*: its place in the stage.
-  constexpr bool CUTS = EDGES && sizeof(T) == 2;
+  const bool cuts = EDGES && sizeof(T) == 2 && ((cols_a | cols_b) & 1);
   int fill_a = -1, fill_b = -1, put_a = 0, put_b = 0;
-  if constexpr (CUTS) {
+  if (cuts) {
     const int64_t last_b = lines_b - 1 - (MODE == GROUPED_DW ? 0 : (int64_t)g * a.n);  // B's last line: a c, or forward a j
     const int64_t ia = MODE == GROUPED_DW ? cols_a - 1 : a.rows - 1, ca = MODE == GROUPED_DW ? a.rows - 1 : cols_a - 1;
     const int64_t jb = MODE == GROUPED_FWD ? last_b : cols_b - 1, cb = MODE == GROUPED_FWD ? cols_b - 1 : last_b;
@@ -417,7 +417,7 @@ __device__ __forceinline__ void grouped_body(const GroupedArgs &a, int block, ui
       oa.trim(la, STAGES - 1);
       ob.trim(la + BM * KC, STAGES - 1);
     }
-    if constexpr (CUTS) {
+    if (cuts) {
       const int past = (int)(c - c0);
       if ((uint32_t)(fill_a - past) < (uint32_t)KE) {
         reinterpret_cast<T *>(la)[put_a] = pa[end_a - 1];

@@ -60,6 +60,12 @@ def _encode(x, signed):
     return code.to(torch.uint8), base.to(torch.int16)
 
 
+def _families(tensors):
+    """One of every family of views: they share the version that autograd looks at."""
+    bases = [t if t._base is None else t._base for t in tensors]
+    return list({id(b): t for b, t in zip(bases, tensors)}.values())
+
+
 class _Plan(object):
     """One parameter group: its flat moments and what the kernels read about its variables."""
 
@@ -70,7 +76,7 @@ class _Plan(object):
         self.like = ({p0.dtype}, {p0.get_device()})           # of every gradient
         self.tracked = [not p.is_inference() for p in self.params]     # tensors of inference mode have no version
         self.moved = [t for t in self.targets or [] if not t.is_inference()]
-        self.written = [p for p, on in zip(self.params, self.tracked) if on] + self.moved
+        self.written = _families([p for p, on in zip(self.params, self.tracked) if on] + self.moved)
         self.counts = [p.numel() for p in self.params]
         self.first, total = [], 0
         for c in self.counts:                       # every variable starts at a multiple of BLOCK

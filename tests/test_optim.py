@@ -780,3 +780,22 @@ def test_load_hooks_run():
     gone.remove()
     opt.load_state_dict(saved)
     assert seen == ['first', 'halve', (True, 0.25)] and saved['param_groups'][0]['lr'] == 0.5
+
+
+@pytest.mark.gpu
+def test_views_of_one_array_move_its_version():
+    """Parameters that are views of one array share its version: autograd notices a step through any of them and through it."""
+    flat, lone = torch.ones(300, device='cuda'), torch.nn.Parameter(torch.ones(30, device='cuda'))
+    ps = [flat[:100], flat[128:200], flat[200:300].view(10, 10), lone]
+    opt = optim.AdamW(ps, lr=0.5, targets=[p.detach().clone() for p in ps])
+    scale = torch.ones(300, device='cuda', requires_grad=True)
+    for saved in (lambda: (flat * scale).sum(), lambda: (ps[1] * scale[:72]).sum(), lambda: (ps[2].view(-1) * scale[:100]).sum(),
+                  lambda: (lone * lone).sum()):
+        loss = saved()
+        seen = [p._version for p in ps]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        assert all(p._version > v for p, v in zip(ps, seen))
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()

@@ -400,4 +400,5 @@ class CapturedLearners(object):
         self.learners.check()
         self._draw()
         self.graph.replay()
+        self.learners.written()
         return self.last

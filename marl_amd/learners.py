@@ -65,6 +65,10 @@ class _Stack(object):
         if any(a is not b for a, b in zip(nets, self.nets)) or list(map(torch.Tensor.data_ptr, self.params)) != self.at:
             raise RuntimeError('Learners: a network was replaced or its variables moved (.to(), .data, other Learners): build Learners anew')
 
+    def written(self):
+        """The networks' variables share the stacks' memory, not their versions: graphs that saved them are told of a step here."""
+        torch.autograd.graph.increment_version(self.params)
+
     def variables(self):
         """Every network's variables, each a contiguous tensor of its own (clipping is per variable)."""
         return [t[i] for w, b in zip(self.w, self.b) for t in (w, b) for i in range(self.n)]
@@ -216,6 +220,11 @@ class Learners(object):
                     v.copy_(got[k])
         self._repack()
 
+    def written(self):
+        """For autograd: every network was written."""
+        for name in NETS:
+            getattr(self, name).written()
+
     def _repack(self):
         for tr in self.trainers:                                # refilled in place: recorded acting steps read it
             if tr._packed is not None:
@@ -288,6 +297,7 @@ class Learners(object):
         p_loss = -acts[3].view(n, b).mean(1) + 1e-3 * (logits.square() * self.real.unsqueeze(1)).sum((1, 2)) / (b * width.view(n))
         self._step(self.p_opt, self.p.gradients(pol, dlogits.reshape(n * b, -1), self.ends))
         self._repack()
+        self.written()
 
         tq, tn = target.view(n, b), target_next.view(n, b)
         stats = torch.stack([q_loss, p_loss, tq.mean(1), rew.view(n, b).mean(1), tn.mean(1), tq.std(1, unbiased=False)], 1)

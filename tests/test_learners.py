@@ -290,3 +290,32 @@ def test_a_saved_run_goes_on_as_if_it_had_not_stopped(bits, monkeypatch):
     with pytest.raises(ValueError):
         lb.load_state_dict(dict(saved, networks=dict(saved['networks'], p=saved['networks']['q'])))
     assert all(torch.equal(x, y) for x, y in zip(before, tb[0].p.parameters()))
+
+
+def test_autograd_notices_an_update():
+    """Graphs of any network that was saved before an update, eager or recorded, raise in their backward pass, as they do with the
+    trainers' own updates."""
+    from marl_amd.graph import CapturedLearners
+    from marl_amd.learners import Learners
+    _, trainers = _setup()
+    learners = Learners(trainers)
+
+    def losses():
+        return [getattr(tr, n)(torch.randn(8, getattr(tr, n)[0].in_features, device='cuda')).square().sum() for tr in trainers for n in NETS]
+
+    def stale(found):
+        for loss in found:
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                loss.backward()
+    for loss in losses():
+        loss.backward()                                                     # nothing happened in between
+    saved = losses()
+    learners.update(100)
+    stale(saved)
+    cap = CapturedLearners(learners)
+    saved = losses()
+    cap.replay()
+    stale(saved)
+    saved = losses()
+    learners.load_state_dict(learners.state_dict())
+    stale(saved)

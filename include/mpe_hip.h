@@ -511,7 +511,7 @@ typedef struct mpe_actor_job {
   int32_t in_dim, s0, s1;
   uint64_t seed;
 } mpe_actor_job;
-#define MPE_ACTOR_AUTO 0 /* the library's choice: the matrix-core kernel (1.6-2.5x the vector one, 1 Ki .. 1 Mi envs) */
+#define MPE_ACTOR_AUTO 0 /* the library's choice: the matrix-core kernel (1.8-2.5x the vector one, 1 Ki .. 1 Mi envs) */
 #define MPE_ACTOR_VALU 1 /* vector kernel: one env per lane, f32 FMAs, weights through the scalar cache */
 #define MPE_ACTOR_MFMA 2 /* v_mfma_f32_32x32x16_bf16 on exact three-way bf16 splits of the f32 operands, six partial
                             products per product: the error of an f32 dot product; 32 envs per tile on the lane axis */

@@ -86,23 +86,45 @@ __global__ __launch_bounds__(256) MPE_ACTOR_ATTR void actor_forward_kernel(int64
   // layer 2 in blocks of KB output units (j unrolled: static h1 registers), each block folded into layer 3 at
   // once, so h2 never exists as an array; the block loop stays a real loop, which bounds what the scheduler
   // may hoist (fully unrolled, it pulls all 5 200 scalar weight loads to the top and spills 5 000 SGPRs).
-  // Measured, 1 Mi envs, 16 inputs: weights as LDS broadcast reads 424 us (the LDS pipe, shared by the four
-  // SIMDs, is the bound), as scalar loads 199 us, scalar loads + packed FMAs 185 us.
-  constexpr int KB = 8;
+  // The loop body still has 512 scalar loads that the scheduler would pull to its top (545 SGPR spills, 994 us): four units'
+  // weights are fetched behind the first FMAs of the four before them (whose wait, on scalar loads, is for all that are under
+  // way), and nothing moves across.  Measured, 1 Mi envs, 16 inputs: 208 us; two units ahead 220, no load ahead, only the bounds,
+  // 233; 4 096 envs 23, 29, 40.  Weights as LDS broadcast reads 424 us (the LDS pipe, shared by the four SIMDs, is the bound).
+  constexpr int KB = 8, JB = 4;
   f2 out2[O / 2];
 #pragma unroll
   for (int m = 0; m < O / 2; ++m) out2[m] = f2{out[2 * m], out[2 * m + 1]};
 #pragma unroll 1
   for (int kb = 0; kb < H; kb += KB) {
-    f2 acc[KB / 2];
+    f2 acc[KB / 2], ahead[JB][KB / 2];
 #pragma unroll
     for (int q = 0; q < KB / 2; ++q) acc[q] = f2{b2[kb + 2 * q], b2[kb + 2 * q + 1]};
+    const auto fetch = [&](int j0) {
 #pragma unroll
-    for (int j = 0; j < H; ++j) {
-      const f2 hj = f2{h1[j], h1[j]};
+      for (int j = 0; j < JB; ++j)
 #pragma unroll
-      for (int q = 0; q < KB / 2; ++q)
-        acc[q] = __builtin_elementwise_fma(f2{W2[j * H + kb + 2 * q], W2[j * H + kb + 2 * q + 1]}, hj, acc[q]);
+        for (int q = 0; q < KB / 2; ++q) ahead[j][q] = f2{W2[(j0 + j) * H + kb + 2 * q], W2[(j0 + j) * H + kb + 2 * q + 1]};
+    };
+    fetch(0);
+#pragma unroll
+    for (int j0 = 0; j0 < H; j0 += JB) {
+      f2 w[JB][KB / 2];
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int q = 0; q < KB / 2; ++q) w[j][q] = ahead[j][q];
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        const f2 hj = f2{h1[j0 + j], h1[j0 + j]};
+#pragma unroll
+        for (int q = 0; q < KB / 2; ++q) acc[q] = __builtin_elementwise_fma(w[j][q], hj, acc[q]);
+        if (j == 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (j0 + JB < H) fetch(j0 + JB);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int kk = 0; kk < KB; ++kk) {
@@ -163,16 +185,16 @@ __global__ __launch_bounds__(256) MPE_ACTOR_ATTR void actor_forward_kernel(int64
 // ------------------------------------------------------------------------------------------------------------------
 // The same actor on the matrix cores, at f32 accuracy from bf16 MFMAs ("bf16x6").
 //
-// f32 MFMA has the vector rate (v_mfma_f32_32x32x2_f32: 256 flop / cycle / CU, the same as v_pk_fma_f32): round 2's first
-// matrix-core form, built on it, tied with the vector kernel above (170.8 vs 158.1 us per agent at 1 Mi envs).  The bf16
+// f32 MFMA has the vector rate of packed FMAs (v_mfma_f32_32x32x2_f32: 256 flop / cycle / CU), twice that of plain ones: a first
+// matrix-core form, built on it, took 170.8 us per agent at 1 Mi envs.  The bf16
 // MFMA is 16x faster per k (v_mfma_f32_32x32x16_bf16: 32 cycles for 16 k), so every f32 operand is split EXACTLY into
 // three bf16 pieces, x = hi + mid + lo (the next 8 significant bits each: truncation, so the residuals are exact and
 // the range is f32's), and a product is the six partial products whose weight is >= 2^-16 of the leading one:
 //     x w = hi hi + hi mid + mid hi + mid mid + hi lo + lo hi        (+ mid lo + lo mid + lo lo < 2^-23 |x w|, dropped)
 // Each partial product is exact in the f32 accumulator (8 x 8 bits), so the result carries the error of an f32 dot
 // product (tests: <= 1e-5 against PyTorch f32, the vector kernel's bar).  Six MFMAs of 32 cycles replace eight of 64.
-// Measured (r2 MI355X, tools/actor_bench.py, 16 -> 64 -> 64 -> 5): 1 Mi envs 91.5 us vs 161.6 us for the vector kernel
-// (34 inputs: 127.0 vs 228.6), 262 144 envs 25.7 vs 43.9, 4 096 envs 11.9 vs 20.1 (the vector kernel's floor is its
+// Measured (MI355X, tools/actor_bench.py, 16 -> 64 -> 64 -> 5): 1 Mi envs 90.5 us vs 208 us for the vector kernel
+// (34 inputs: 131.7 vs 278), 262 144 envs 26.1 vs 57.6, 4 096 envs 11.5 vs 22.9 (the vector kernel's floor is its
 // 5 000-FMA dependent chain per lane).  What bounds it now is vector ISSUE, not the matrix pipe: per 32-env tile 84 MFMAs
 // (2 688 matrix-pipe cycles, 8 issue cycles each) beside ~860 vector instructions -- the operand splits (5.5 per value:
 // and, subtract, and, subtract, 1.5 permutes), relu as an integer max, Philox, the softmax; SQ counters: vector issue
@@ -204,7 +226,7 @@ __device__ __forceinline__ Bf16x3 split_bf16x3(const float (&x)[8]) {
   Bf16x3 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // (plain subtractions: packed v_pk_add_f32 is an anti-lever beside MFMAs, MI355X_MICROARCH.md cycle constants)
+    // (plain subtractions: the build has no packed f32 instructions)
     const uint32_t a0 = __float_as_uint(x[2 * i]), a1 = __float_as_uint(x[2 * i + 1]);
     const float r0 = x[2 * i] - __uint_as_float(a0 & 0xFFFF0000u), r1 = x[2 * i + 1] - __uint_as_float(a1 & 0xFFFF0000u);
     const uint32_t b0 = __float_as_uint(r0), b1 = __float_as_uint(r1);

@@ -610,7 +610,8 @@ int mpe_grouped_linear_backward(const mpe_grouped_desc *desc, const void *dy, in
  *   mpe_adamw_step   tensors: the same host array; grads: host array of device pointers, NULL = no gradient (only the
  *                    target moves).  step >= 1 counts this step, or clock (device, 32 bytes: int64 step, then 16 bytes that
  *                    the call writes) holds the steps taken so far and is moved on by one (for graph capture).
- *                    max_norm 0: no clip.  The plan holds the clip's scratch: steps on one plan must not overlap
+ *                    max_norm 0: no clip, else a normal float.  Of 16-bit parameters with 8-bit moments the root and the quotient are to
+ *                    one last place of 32 bits (where eps drowns a subnormal second moment), elsewhere correctly rounded.  The plan holds the clip's scratch: steps on one plan must not overlap
  *   mpe_adamw_moments  the byte codes of count (a multiple of 128) elements as the values they stand for (MPE_F32 / MPE_BF16);
  *                    out NULL or out_sq NULL: not that one
  */

@@ -18,7 +18,7 @@
 // One pass: every value is read and written once (with a clip, gradients of more than one work item are read twice).  Work items
 // of 8 192 values: 8 values a thread a turn, 16-byte accesses, no tensor shares an item, so the smallest and the largest tensors
 // need one launch together.  Bound by memory: 62 M f32 values with clip and target (2.2 GB) 540 us = 4.2 TB/s, 302 M bf16
-// values with 8-bit moments (3.0 GB) 620 us = 4.9 TB/s, the vector units 91 % active; 48 variables of 4 learners 9 us, 26 from
+// values with 8-bit moments (3.0 GB) 623 us = 4.9 TB/s, the vector units 92 % active; 48 variables of 4 learners 9 us, 28 from
 // Python.
 #pragma once
 #include <hip/hip_runtime.h>

@@ -89,7 +89,9 @@ constexpr int kTile[3] = {64, 128, 256};
 
 // A 16-bit product is bound by what the tiles read per matrix instruction: the largest tile that still leaves every CU a
 // workgroup and does not mostly overhang its group's rows.  f32 matrix instructions are 16 times slower: small tiles.
-// mean_rows: of a group; rows: of all; others: independent products.
+// mean_rows: of a group; rows: of all; others: independent products.  The host knows the mean only (`ends` is on the device); forward
+// and dx count their tiles on the device and hold their speed where one group has all rows (32 768 x 512 x 512 bf16 in 64: 30 us even,
+// 40 with half of the rows in one group, 30 with all of them).
 // bf16 forward, us (small / middle / large, rows x k x n in groups): 4 096 x 512 x 512 in 16 8.6 / 11.1 / 22, 8 192 x 1 024 x 1 024 in
 // 16 37 / 28 / 36, 16 384 x 512 x 512 in 16 22 / 18 / 26, 32 768 x 512 x 512 in 32 41 / 32 / 28; dweight: 8 192 x 1 024 x 1 024 in 16
 // 43 / 33 / 30, 32 768 x 512 x 512 in 32 34 / 27 / 42.  The large tile has no registers for n or k that end inside a chunk.
@@ -111,6 +113,9 @@ int64_t dw_tiles(const mpe_grouped_desc *d) {
 // joined.  The join is a launch (4 us) and 8 bytes a partial sum: the split with the least sum of both, from the rows a tile gets
 // through per us.  f32 65 536 x 64 x 64 in 64 groups 28 us as one, 15 in eight parts; bf16 4 096 x 256 x 256 in 8 7.2 as one, 12 in
 // four, 8 192 x 512 x 512 in 4 17 as one, 19 in two.  Large tiles are enough by pick_tile's rule.
+// Its limit: the split is for groups of the mean size.  A group of most of the rows runs through them in the same few parts while the
+// chip idles (dweight, us, even groups / half of the rows in one / all: f32 65 536 x 64 x 64 in 64 16 / 104 / 195, in 1 024 16 / 747 /
+// 1 486; bf16 65 536 x 256 x 256 in 64 23 / 443 / 889, 16 384 x 1 024 x 1 024 in 16 48 / 224 / 436).
 int dw_splits(const mpe_grouped_desc *d) {
   const Tile tile = dw_tile(d);
   if (tile == LARGE) return 1;

@@ -14,7 +14,8 @@
 // whatever it holds, no row belongs to two groups and no access leaves the arrays.
 //
 // What bounds it (one MI355X; a copy of 4 GiB moves 4.76 TB/s, one library product of 8 192^3 1 274 TFLOP/s bf16, 154 f32):
-//     small calls        launch and one trip to memory: 4 096 x 16 x 64 f32 6 us, 5 003 x 333 x 517 f16 in 7 groups 12
+//     small calls        launch and one trip to memory: 4 096 x 16 x 64 f32 6 us, 5 003 x 333 x 517 f16 in 7 groups 12 (six
+//                        stages of 64 elements of c, two buffers: each waits for most of a trip to memory)
 //     few rows           the weights: 13 rows over 16 of 1 024 x 2 048 bf16, 55 MB, 13 us = 4.2 TB/s
 //     f32                the matrix units: 65 536 x 14 752 x 64 in 64 groups 1 100 us, 3.7 TB/s, matrix units busy 78 % of the time
 //     16-bit, many rows  32 768 x 2 048 x 2 048 bf16 in 32 unlike groups 333 us = 825 TFLOP/s (even groups 288, one group 256), matrix

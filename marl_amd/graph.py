@@ -354,7 +354,8 @@ class CapturedUpdates(object):
 
 class CapturedLearners(object):
     """``CapturedUpdates`` for a ``marl_amd.learners.Learners``: all learners' updates of a due step (grouped products, one
-    AdamW step per network kind) as ONE HIP-graph replay, whose launch count does not grow with the number of agents.
+    AdamW step per network kind) as ONE HIP-graph replay (153 nodes for 4 learners, 254 for 8: products and steps are of all
+    learners together, gathers and copies per learner).
 
     Construct it at a step where the update is due: the constructor performs that update eagerly and records the same calls;
     ``replay()`` performs one update per call.  Batch indices are drawn outside the graph; nothing of it goes through

@@ -173,7 +173,9 @@ def grouped_linear(x, weight, ends, bias=None, relu=False, out=None):
 def grouped_linear_backward(grad, x, weight, ends, y=None, need_dx=True, need_dweight=True, need_dbias=True):
     """``(dx, dweight, dbias)`` of ``grouped_linear`` for the gradient ``grad`` ``[rows, n]`` of its result; ``y``: the
     result itself where it was made with ``relu=True`` (``grad`` counts where ``y`` is not <= 0).  An entry that is not needed
-    is None.  ``dx`` is zero in rows of no group, ``dweight`` / ``dbias`` are zero for groups without rows."""
+    is None.  ``dx`` is zero in rows of no group, ``dweight`` / ``dbias`` are zero for groups without rows.  ``dbias`` comes with
+    ``dweight``: alone it costs the same.  Groups may have any rows, but dweight's work is split for groups of the mean size: one
+    group with most of the rows is slow (``dw_splits`` in mpe_grouped.hip has figures)."""
     if torch.is_tensor(ends) and not ends.is_contiguous():
         ends = ends.contiguous()
     desc, index, rows, n, k = _check(x, weight, ends)

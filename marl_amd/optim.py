@@ -15,7 +15,7 @@ place of 32 bits, elsewhere correctly rounded.)  ``state_bits=32`` holds the mom
 each, plus one int16 for 128 of them: a logarithmic code (eighths of a binade; m 16 binades and a sign, v 32 binades) below
 the largest element of its block, rounded stochastically from (seed, step, tensor, element), so that a moment is right on
 average and a run repeats bit for bit.  A gradient that is not finite makes its element (32 bits) or its block of 128
-(8 bits) useless, as it does any Adam."""
+(8 bits) useless, as it does any Adam; with ``max_norm`` its whole variable, whose norm it is part of."""
 import collections
 import ctypes as C
 from operator import attrgetter

@@ -14,7 +14,8 @@ The trainers' networks become views of the stacked arrays (weights of narrower a
 zero), so acting, ``act_all`` and the trainers' own methods go on as before (an update finds and refuses networks that were
 taken out of the stacks since, as a second ``Learners`` of the same trainers does); the step is AdamW with ``weight_decay`` 0 unless
 given, which is the trainers' Adam.  Moments live here (``Learners.p_opt`` / ``.q_opt``; they begin as the trainers' own, in 8 bits
-rounded), not in the trainers' ``p_opt`` / ``q_opt``, which stay as they were: use one or the other,
+rounded), not in the trainers' ``p_opt`` / ``q_opt``, which stay as they were: use one or the other
+(a second ``Learners`` of the same trainers goes on where the first was with its ``state_dict``),
 and save a run with ``Learners.state_dict`` (the trainers' optimizers no longer hold what a resumed run needs)."""
 import torch
 from torch import nn
@@ -214,6 +215,8 @@ class Learners(object):
             got = state_dict['networks'][name]
             if [{k: v.shape for k, v in d.items()} for d in got] != [{k: v.shape for k, v in d.items()} for d in have[name]]:
                 raise ValueError('Learners: the state dict is of other networks (%s)' % name)
+        for name in OPTS:                                       # all of it or nothing
+            getattr(self, name).fits(state_dict[name])
         for name in OPTS:
             getattr(self, name).load_state_dict(state_dict[name])
         for name in NETS:

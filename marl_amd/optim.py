@@ -299,7 +299,7 @@ class AdamW(torch.optim.Optimizer):
                 if clock is not None:
                     clock.record_stream(torch.cuda.current_stream(plan.device))
             args = _hip.AdamArgs(group['lr'], *group['betas'], group['eps'], group['weight_decay'], group['max_norm'] or 0.0,
-                                 group['polyak'], group['step'] + 1, _hip.ptr(clock), group['seed'] & _SEED, index0, _DTYPES[plan.dtype],
+                                 group['polyak'], group['step'] + 1, _hip.ptr(clock), int(group['seed']) & _SEED, index0, _DTYPES[plan.dtype],
                                  self._bits)
             _hip.check(_hip.launch(plan.device.index, _hip.lib.mpe_adamw_step, args, len(plan.params), plan.table,
                                    plan.plan_ptr, plan.grads), 'mpe_adamw_step')
@@ -344,13 +344,8 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups[i]['step'] = self._steps(i)
         return super().state_dict()
 
-    def load_state_dict(self, state_dict):
-        """Settings, step counts and moments of an optimizer with the same groups, shapes and ``state_bits``; the moments are
-        copied into this optimizer's arrays, which stay where they are."""
-        state_dict = dict(state_dict)
-        for hook in list(self._before_load.values()):
-            changed = hook(self, state_dict)
-            state_dict = state_dict if changed is None else changed
+    def fits(self, state_dict):
+        """Raises where ``load_state_dict`` would refuse this one; the pairs of arrays to copy."""
         groups = state_dict['param_groups']
         if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
             raise ValueError('AdamW: the state dict has other parameter groups')
@@ -364,6 +359,17 @@ class AdamW(torch.optim.Optimizer):
                 todo += [(have[k], got[k]) for k in have]
         for saved in groups:
             self._check_group(saved)
+        return todo
+
+    def load_state_dict(self, state_dict):
+        """Settings, step counts and moments of an optimizer with the same groups, shapes and ``state_bits``; the moments are
+        copied into this optimizer's arrays, which stay where they are."""
+        state_dict = dict(state_dict)
+        for hook in list(self._before_load.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        todo = self.fits(state_dict)
+        groups = state_dict['param_groups']
         for dst, src in todo:
             dst.copy_(src)
         for i, (group, saved) in enumerate(zip(self.param_groups, groups)):

@@ -319,3 +319,23 @@ def test_autograd_notices_an_update():
     saved = losses()
     learners.load_state_dict(learners.state_dict())
     stale(saved)
+
+
+def test_a_state_dict_is_taken_whole_or_not_at_all(monkeypatch):
+    """One optimizer's part that does not fit: nothing of the rest is loaded.  A second Learners goes on with the first one's."""
+    from marl_amd.learners import Learners
+    _fixed(monkeypatch)
+    _, trainers = _setup()
+    first = Learners(trainers)
+    saved = first.state_dict()
+    first.update_from_index(_index(trainers, 0))
+    held = [t.clone() for t in first.p_opt.buffers()[0].values()] + [t.detach().clone() for t in trainers[0].p.parameters()]
+    with pytest.raises(ValueError):
+        first.load_state_dict(dict(saved, q_opt=saved['p_opt']))
+    assert all(torch.equal(x, y) for x, y in zip(held, list(first.p_opt.buffers()[0].values()) + list(trainers[0].p.parameters())))
+    assert first.p_opt.step_count == 1
+    now = first.state_dict()
+    want = [[float(x) for x in row] for row in first.update_from_index(_index(trainers, 1))]
+    second = Learners(trainers)
+    second.load_state_dict(now)
+    assert want == [[float(x) for x in row] for row in second.update_from_index(_index(trainers, 1))]
